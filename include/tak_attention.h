@@ -322,6 +322,118 @@ int tak_csa_indexer_topk(const void* q, const int64_t* q_strides, const void* co
  * to 128 x the element size. */
 int64_t tak_csa_indexer_workspace_size(int64_t total_tokens, int64_t max_comp_per_seq, int dtype);
 
+/*
+ * ---------------------------------------------------------------------------
+ * Positions and an 8-bit KV cache.  No counterpart in the reference: additions
+ * for serving loops whose caches should hold half the bytes.
+ * ---------------------------------------------------------------------------
+ */
+
+/*
+ * Rotary positions with several axes.  q [T,H,D] and k [T,H_kv,D] (either may
+ * have no heads) are written to q_out / k_out (the same tensors for an
+ * in-place call; otherwise not overlapping).  positions [T, num_axes] int32;
+ * inv_freq [rot_dim / 2] float32; sections [num_axes] is a HOST array of pair
+ * counts that add up to rot_dim / 2: pair i turns by positions[t, axis(i)] *
+ * inv_freq[i].  Pairs are (i, i + rot_dim / 2), or (2i, 2i + 1) with
+ * interleaved != 0; elements past rot_dim are copied.  inverse != 0 turns the
+ * other way: the gradient of the forward call.  The angle is formed in 64
+ * bits, the rotation in 32, with one rounding to the element type.
+ */
+int tak_rotary_nd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                  const int32_t* positions, const int64_t* pos_strides, const float* inv_freq,
+                  const int32_t* sections, int64_t num_axes, void* q_out, const int64_t* q_out_strides, void* k_out,
+                  const int64_t* k_out_strides, int64_t total_tokens, int64_t num_q_heads, int64_t num_kv_heads,
+                  int64_t head_dim, int64_t rot_dim, int interleaved, int inverse, int dtype, void* stream);
+
+enum { TAK_KV8_INT8 = 0, TAK_KV8_E4M3 = 1 };
+
+/*
+ * A paged KV cache held in 8 bits.  k_cache / v_cache [num_blocks, H_kv,
+ * block_size, D] hold codes (int8 in [-127, 127], or e4m3), k_scale / v_scale
+ * [num_blocks, H_kv, block_size / group] float32 one non-negative scale for
+ * each page, KV head and group of `group` consecutive rows: an element's value
+ * is code * scale.  Strides are in elements.  block_tables [num_seqs,
+ * max_blocks] int32.  Rows past the block table, or on a page id outside
+ * [0, num_blocks), are never read or written: they read as zero rows (score 0,
+ * value 0), and writes to them are dropped.  Limits: D <= 640, group <= 256
+ * and dividing block_size, num_seqs and H_kv <= 65535,
+ * max_blocks * block_size < 2^31.
+ */
+typedef struct tak_kv8_cache {
+  void* k_cache; int64_t k_strides[4];
+  void* v_cache; int64_t v_strides[4];
+  float* k_scale; int64_t k_scale_strides[3];
+  float* v_scale; int64_t v_scale_strides[3];
+  const int32_t* block_tables; int64_t bt_strides[2];
+  int64_t num_blocks, num_kv_heads, block_size, head_dim, group, num_seqs, max_blocks;
+  int64_t code_type; /* TAK_KV8_INT8 or TAK_KV8_E4M3 */
+} tak_kv8_cache;
+
+/*
+ * Writes rows into the cache: rows cu_seqlens[s] .. cu_seqlens[s + 1] of k / v
+ * [T,H_kv,D] (fp16, bf16 or fp32) go to positions start_lens[s] .. of sequence
+ * s; cu_seqlens = NULL writes one row per sequence (a decode step).  Positions
+ * before start_lens[s] must have been written.  A group's scale is its largest
+ * magnitude / 127 (int8) or / 448 (e4m3); a group that already holds rows keeps
+ * the larger of its scale and the new rows', and rows held under a smaller
+ * scale are rounded again into it.  Codes are rounded to nearest even.  A group
+ * whose magnitudes are all below 2^-100 is held as zeros; one that receives an
+ * infinity or a NaN gets a NaN scale (its rows read back as NaN).  Two
+ * sequences of one call must not write to the same page.
+ */
+int tak_kv8_write(const tak_kv8_cache* cache, const void* k, const int64_t* k_strides, const void* v,
+                  const int64_t* v_strides, const int32_t* start_lens, const int32_t* cu_seqlens,
+                  int64_t total_tokens, int dtype, void* stream);
+
+/*
+ * Reads rows back as fp16, bf16 or fp32: rows cu_seqlens[s] .. of k / v
+ * [T,H_kv,D] receive positions start_lens[s] .. (start_lens = NULL: from 0) of
+ * sequence s, e.g. the cached prefix of a prompt that tak_flash_attention_prefill
+ * continues.  Rows outside every sequence get zeros.
+ */
+int tak_kv8_read(const tak_kv8_cache* cache, const int32_t* cu_seqlens, const int32_t* start_lens,
+                 int64_t total_tokens, void* k, const int64_t* k_strides, void* v, const int64_t* v_strides,
+                 int dtype, void* stream);
+
+/*
+ * Attention of num_queries query rows per sequence over the cache.  q and out
+ * [num_seqs, num_queries, H, D]; context_lens [num_seqs] counts the cached rows,
+ * the queries' own among them: query row i sees the first context_lens[s] -
+ * num_queries + 1 + i rows (none: output 0, lse -inf).  KV head h / (H / H_kv).
+ * softcap > 0 replaces a scaled score z by softcap * tanh(z / softcap).
+ * lse (may be NULL) [num_seqs, num_queries, H] float32.  weights (may be NULL)
+ * [num_seqs, H_kv, weights_width] float32: each key's attention weight, summed
+ * over the query rows and the heads that share the KV head, is ADDED to it
+ * (keys at or past weights_width are left out).  workspace: at least
+ * tak_kv8_attention_workspace_size() bytes, 16-byte aligned, no initialisation
+ * needed; pass that function weights_width = 0 when weights is NULL.  It
+ * returns -1 for arguments that the call would refuse.
+ */
+int64_t tak_kv8_attention_workspace_size(const tak_kv8_cache* cache, int64_t num_q_heads, int64_t num_queries,
+                                         int64_t weights_width, int dtype);
+int tak_kv8_attention(const tak_kv8_cache* cache, const void* q, const int64_t* q_strides,
+                      const int32_t* context_lens, void* out, const int64_t* out_strides, float* lse,
+                      float* weights, const int64_t* weights_strides, int64_t weights_width, int64_t num_q_heads,
+                      int64_t num_queries, float scale, float softcap, int dtype, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/*
+ * Evicts rows in place.  For each sequence and KV head with n = min(
+ * context_lens[s], weights_width, max_blocks * block_size) > budget rows, the
+ * last `recent` rows stay and, of the others, the budget - recent with the
+ * largest weights [num_seqs, H_kv, weights_width] (ties to the lowest position;
+ * NaN counts as largest).  Kept rows move to the front in ascending order, and
+ * so do their weights; weights of the places freed become 0.  A group of the
+ * result takes the largest scale of its rows, and rows from a smaller scale are
+ * rounded again into it.  kept [num_seqs, H_kv, budget] receives the positions
+ * that stayed (-1 past the end), new_lens [num_seqs] min(n, budget).  The pages
+ * past new_lens are free afterwards.  Sequences must not share pages.
+ */
+int tak_kv8_evict(const tak_kv8_cache* cache, const int32_t* context_lens, float* weights,
+                  const int64_t* weights_strides, int64_t weights_width, int64_t budget, int64_t recent,
+                  int32_t* kept, int32_t* new_lens, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -55,6 +55,14 @@ _SIGS = {
     "tak_csa_indexer_topk": ([_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                               _P, _I64, _I32, _P, _I64, _I64, _P], _I32),
     "tak_csa_indexer_workspace_size": ([_I64, _I64, _I32], _I64),
+    "tak_rotary_nd": ([_P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I32,
+                       _I32, _I32, _P], _I32),
+    "tak_kv8_write": ([_P, _P, _P, _P, _P, _P, _P, _I64, _I32, _P], _I32),
+    "tak_kv8_read": ([_P, _P, _P, _I64, _P, _P, _P, _P, _I32, _P], _I32),
+    "tak_kv8_attention_workspace_size": ([_P, _I64, _I64, _I64, _I32], _I64),
+    "tak_kv8_attention": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _F32, _F32, _I32, _P, _I64, _P],
+                          _I32),
+    "tak_kv8_evict": ([_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P], _I32),
 }
 
 

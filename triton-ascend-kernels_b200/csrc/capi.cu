@@ -41,6 +41,8 @@ int num_sms() {
   return n > 0 ? n : 148;
 }
 
+int kernel_path() { return g_kernel_path; }
+
 int ensure_smem_attr(const void* func, int bytes) {
   static std::mutex mu;
   static std::map<std::pair<const void*, int>, int> done;

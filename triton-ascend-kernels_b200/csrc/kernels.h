@@ -18,6 +18,7 @@ void note_kernel(const char* name);
 // cudaGetLastError after a launch: 0, or status 3 with the CUDA error as message
 int check_launch(const char* what);
 int num_sms();
+int kernel_path();  // tak_set_kernel_path's value: 1 = generic kernels only
 // cudaFuncAttributeMaxDynamicSharedMemorySize of `func` on the current device,
 // raised to at least `bytes` (set once per device and kernel, cached)
 int ensure_smem_attr(const void* func, int bytes);
@@ -188,5 +189,18 @@ bool csa_select_warp_launch(const IndexerArgs& a, cudaStream_t st);
 // Top-k selection of decode rows (one per sequence) from provided scores, one
 // 512-thread CTA per row (at most 2048 slots); false when it does not apply.
 bool csa_select_block_launch(const IndexerArgs& a, int rows, cudaStream_t st);
+
+// Rotary positions with several axes; q and k share one launch.
+struct RotaryArgs {
+  const void* q; int64_t sq[3];
+  const void* k; int64_t sk[3];        // null when num_kv_heads == 0
+  void* q_out; int64_t sqo[3];
+  void* k_out; int64_t sko[3];
+  const int32_t* positions; int64_t sp[2];
+  const float* inv_freq;               // [rot_dim / 2]
+  int section_end[8];                  // pair index one past each axis's section
+  int axes, total_tokens, num_q_heads, num_kv_heads, head_dim, rot_dim, interleaved, inverse, dtype;
+};
+int rotary_nd_launch(const RotaryArgs& a, cudaStream_t st);
 
 }  // namespace tak
