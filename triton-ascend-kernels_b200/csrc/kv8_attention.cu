@@ -1,0 +1,838 @@
+// Attention over the 8-bit KV cache: split over the keys, one pass.
+//
+// Mathematics.  With codes Kc, Vc and a scale for each group of rows, a row's
+// score against key j is s_j = scale * ks_g (q . Kc_j) and its output
+// sum_j p_j vs_g Vc_j.  Both scales are constant over a tile of 16 keys (groups
+// are multiples of 16), so K's scale multiplies a tile's scores and V's goes
+// into the exponent: with lv = log2(vs),
+//   P_j = 2^(s_j + lv - M),  O = sum_j P_j Vc_j,  l = sum_j P_j / vs,  out = O / l,
+// where M is the running maximum of s_j + lv.  P stays within fp16 whatever the
+// scales are (a small V under a large weight and a large V under a small weight
+// are compared by their product), and codes are exact in fp16, so both products
+// run on fp16 tensor cores with fp32 sums; q is brought to fp16 by a power of
+// two per row, which is exact for elements within 2^-22 of the row's largest.
+//
+// Work split.  A (sequence, KV head, chunk of query rows) is an item; an item is
+// cut into chunks of CH keys.  The chunks of all items, in order, are dealt out
+// evenly: CTA c of N takes chunks [U c / N, U (c + 1) / N), so ragged contexts
+// cost no idle SM and the host needs no lengths.  An item inside one CTA is
+// finished there; the parts of a cut one go to the workspace (each CTA has at
+// most two) and a second grid joins them in order.
+//
+// A CTA: one producer warp streams chunks through a ring of TMA loads (K and V
+// codes, page ids from the block table) with the tiles' scales beside them; NW
+// warps consume: WM of them across the query rows (16 each), NW / WM across the
+// key tiles.
+#include <cstdio>
+
+#include "kv8.cuh"
+
+namespace tak {
+
+int kv8_attention_generic_launch(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st);
+
+struct Kv8TcParams {
+  Kv8View c;
+  const void* q; int64_t sq[4];
+  const int32_t* context_lens;
+  void* out; int64_t so[4];
+  float* lse;
+  int bf16;          // q and out are bf16 (else fp16)
+  int H, Lq, G, rows, chunks;  // rows = G * Lq query rows per KV head, in `chunks` chunks
+  int box_rows;      // rows of one TMA box: the largest power of two dividing block_size, at most CH
+  float scale;       // softmax scale * log2(e); with a cap: softmax scale
+  float cap2, inv_cap;  // softcap * log2(e), 2 log2(e) / softcap; 0: no cap
+  // workspace
+  int4* bound;       // [N] first chunk of each CTA: {sequence, item of it, chunk of the item, chunks of the item}
+  float* part_o;     // [N][2][16 WM][DP]
+  float* part_ml;    // [N][2][16 WM][2]
+  float* lse2;       // [B, Hkv, rows] (weights only)
+  float* scores;     // [B, Hkv, rows, score_ld] (weights only)
+  int64_t score_ld;
+};
+
+// P is held times 2^kPBias: with the running maximum allowed to lag by kLag it
+// reaches 2^15 (fp16 ends at 2^16), and weights down to 2^-27 of the largest
+// keep fp16's full precision.  l holds sums of P / vs * 2^-kLBias, where P is
+// unbiased: that keeps it in range for V scales down to kMinVs over long
+// contexts.
+constexpr float kPBias = 13.f;
+constexpr float kLag = 2.f;
+constexpr float kLBias = 10.f;
+constexpr float kLBiasInv = 1.1920928955078125e-7f;  // 2^-(kPBias + kLBias)
+constexpr float kMinVs = 6.162975822039155e-33f;  // 2^-107: the smallest scale that the write makes
+
+template <int DP, int WM> struct Kv8Cfg {
+  static constexpr int NW = DP >= 256 ? 8 : 4;          // consumer warps
+  static constexpr int CH = DP == 128 ? 64 : 128;       // keys of a chunk
+  static constexpr int NT = CH / 16;                    // key tiles of a chunk
+  static constexpr int CB = DP >= 256 ? 2 : 1;          // column blocks of a row
+  static constexpr int ROWB = DP >= 128 ? 128 : 64;     // bytes of a row in a column block
+  static constexpr int PLANE = CH * DP;                 // bytes of K (or V) in a stage
+  static constexpr int STAGE = 2 * PLANE;
+  static constexpr int NS = DP >= 256 ? 2 : 4;
+  static constexpr int DH = DP < 128 ? DP : 128;        // columns merged at a time
+  static constexpr int MERGE = NW * 16 * DH * 4;
+  static constexpr int META_OFF = NS * STAGE;           // [NS][3][NT] floats: ks, log2 vs, 2^-23 / vs
+  static constexpr int OBUF_OFF = META_OFF + NS * 3 * NT * 4;
+  static constexpr int ML_OFF = OBUF_OFF + MERGE;       // [NW][16][2]
+  // 256 columns of O take 128 registers a thread: Q's fragments then live in
+  // shared memory, [WM][DP / 16][32 lanes] of 16 bytes, and are loaded per use
+  static constexpr bool QSMEM = DP >= 256;
+  static constexpr int Q_OFF = ML_OFF + NW * 16 * 2 * 4;
+  static constexpr int BAR_OFF = Q_OFF + (QSMEM ? WM * (DP / 16) * 512 : 0);
+  static constexpr int SMEM = BAR_OFF + 2 * NS * 8 + 64 + 1024;
+  static constexpr int CTAS = DP >= 256 ? 1 : 2;        // per SM
+  static_assert(SMEM * CTAS <= 227 * 1024, "shared memory");
+};
+
+// byte offset of 16-byte piece `c` of row `r` in a column block
+template <int DP> __device__ __forceinline__ uint32_t kv8_sw(uint32_t r, uint32_t c) {
+  if (DP >= 128) return r * 128u + ((c ^ (r & 7u)) << 4);
+  return r * 64u + ((c ^ ((r >> 1) & 3u)) << 4);
+}
+
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  uint32_t d;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
+  return d;
+}
+__device__ __forceinline__ uint32_t hsub2_1152(uint32_t x) {
+  const __half2 k = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+  __half2 h = __hsub2(*reinterpret_cast<__half2*>(&x), k);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+// Four codes to two fp16 pairs.  int8: the byte with its sign bit flipped goes
+// into the mantissa of 1024 (fp16 0x6400, where an ulp is 1): 1024 + 128 + x,
+// less 1152.  PAIR = 0 pairs bytes (0,1) (2,3), PAIR = 1 bytes (0,2) (1,3).
+template <int CODE, int PAIR>
+__device__ __forceinline__ void codes_to_half(uint32_t r, uint32_t& lo, uint32_t& hi) {
+  if (CODE == kI8) {
+    const uint32_t x = r ^ 0x80808080u;
+    lo = hsub2_1152(prmt(x, 0x64646464u, PAIR ? 0x4240 : 0x4140));
+    hi = hsub2_1152(prmt(x, 0x64646464u, PAIR ? 0x4341 : 0x4342));
+  } else {
+    const uint32_t x = PAIR ? prmt(r, 0, 0x3120) : r;
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(x));
+  }
+}
+
+__device__ __forceinline__ int kv8_ctx(const Kv8TcParams& p, int s) {
+  const int64_t n = min(static_cast<int64_t>(p.context_lens[s]), p.c.max_rows);
+  return n > 0 ? static_cast<int>(n) : 0;
+}
+
+// Walks a CTA's chunks in order: item `r` of sequence `s`, chunk `j` of `n`.
+template <int CH> struct Kv8Walk {
+  int s, r, j, n, ctx;
+  __device__ __forceinline__ void load(const Kv8TcParams& p) {
+    ctx = kv8_ctx(p, s);
+    n = (ctx + CH - 1) / CH;
+  }
+  __device__ __forceinline__ void next(const Kv8TcParams& p, int items) {
+    if (++j < n) return;
+    j = 0;
+    if (++r < items) return;
+    r = 0;
+    do {
+      if (++s >= p.c.num_seqs) return;
+      load(p);
+    } while (n == 0);
+  }
+};
+
+template <int CODE, int DP, int WM>
+__global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>::CTAS)
+    kv8_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                            const __grid_constant__ Kv8TcParams p) {
+  using C = Kv8Cfg<DP, WM>;
+  constexpr int NW = C::NW, CH = C::CH, NT = C::NT, NS = C::NS, WK = NW / WM, RT = 16 * WM;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* meta = reinterpret_cast<float*>(smem + C::META_OFF);
+  float* obuf = reinterpret_cast<float*>(smem + C::OBUF_OFF);
+  float* mlbuf = reinterpret_cast<float*>(smem + C::ML_OFF);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* empty = full + NS;
+  __shared__ int64_t sh_sum[NW + 1];
+  __shared__ int64_t sh_base;
+  __shared__ int sh_seq;
+  constexpr int THREADS = (NW + 1) * 32;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int B = p.c.num_seqs, items = p.c.Hkv * p.chunks;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], NW);
+    }
+    fence_barrier_init();
+  }
+
+  // ---- where this CTA's chunks begin: prefix sums of the sequences' chunks ----
+  const int seg = (B + THREADS - 1) / THREADS;
+  const int s_lo = min(B, tid * seg), s_hi = min(B, s_lo + seg);
+  int64_t mine = 0;
+  for (int s = s_lo; s < s_hi; ++s) mine += (kv8_ctx(p, s) + CH - 1) / CH;
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
+  if (lane == 31) sh_sum[warp] = incl;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w <= NW; ++w) {
+    if (w < warp) before += sh_sum[w];
+    total += sh_sum[w];
+  }
+  const int64_t U = total * items;
+  const int64_t u0 = U * blockIdx.x / gridDim.x, u1 = U * (blockIdx.x + 1) / gridDim.x;
+  before += incl - mine;  // chunks (of one item) before this thread's sequences
+  if (u0 < U && mine > 0 && before * items <= u0 && u0 < (before + mine) * items) {
+    int s = s_lo;
+    int64_t b = before;
+    for (;; ++s) {
+      const int n = (kv8_ctx(p, s) + CH - 1) / CH;
+      if (u0 < (b + n) * items) break;
+      b += n;
+    }
+    sh_seq = s;
+    sh_base = b * items;
+  }
+  __syncthreads();
+
+  // sequences without a key: zeros (their rows belong to no chunk)
+  for (int s = blockIdx.x; s < B; s += gridDim.x) {
+    if (kv8_ctx(p, s) > 0) continue;
+    for (int e = tid; e < p.Lq * p.H * p.c.D; e += THREADS) {
+      const int d = e % p.c.D, h = e / p.c.D % p.H, i = e / p.c.D / p.H;
+      static_cast<uint16_t*>(p.out)[s * p.so[0] + i * p.so[1] + h * p.so[2] + d * p.so[3]] = 0;
+    }
+    for (int e = tid; e < p.Lq * p.H; e += THREADS)
+      if (p.lse) p.lse[static_cast<int64_t>(s) * p.Lq * p.H + e] = -INFINITY;
+  }
+  if (u0 >= u1) {
+    if (tid == 0) p.bound[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
+  Kv8Walk<CH> w0;
+  w0.s = sh_seq;
+  w0.load(p);
+  w0.r = static_cast<int>((u0 - sh_base) / w0.n);
+  w0.j = static_cast<int>((u0 - sh_base) % w0.n);
+  if (tid == 0) p.bound[blockIdx.x] = make_int4(w0.s, w0.r, w0.j, w0.n);
+  const int count = static_cast<int>(u1 - u0);
+
+  if (warp == NW) {
+    // ---------------- producer ----------------
+    // lane t < NT looks after tile t of a chunk: its page and scales are loaded
+    // one and two chunks ahead, so that no chunk waits on them
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    const int nbox = CH / p.box_rows, tiles_per_box = p.box_rows / 16;
+    struct Meta { int64_t page; int row, kvh, ctx, tok0; float ks, vs; };
+    auto fetch_page = [&](const Kv8Walk<CH>& w, bool live) {
+      Meta m{};
+      m.page = -1;
+      m.ctx = w.ctx;
+      m.tok0 = w.j * CH;
+      m.kvh = w.r / p.chunks;
+      const int tok = m.tok0 + lane * 16;
+      if (live && lane < NT && tok < w.ctx) {
+        const int lp = tok / p.c.P;
+        m.row = tok - lp * p.c.P;
+        m.page = p.c.block_tables[w.s * p.c.sbt[0] + lp * p.c.sbt[1]];
+      }
+      return m;
+    };
+    auto fetch_scales = [&](Meta& m) {
+      m.ks = m.vs = 0.f;
+      if (m.page >= 0 && m.page < p.c.num_blocks) {
+        const int g = m.row / p.c.group;
+        m.ks = *kv8_scale(p.c.plane[0], m.page, m.kvh, g);
+        m.vs = *kv8_scale(p.c.plane[1], m.page, m.kvh, g);
+      }
+    };
+    Kv8Walk<CH> w = w0;
+    Meta cur = fetch_page(w, true);
+    w.next(p, items);
+    Meta nxt = fetch_page(w, count > 1);
+    fetch_scales(cur);
+    for (int it = 0; it < count; ++it) {
+      if (it + 1 < count) w.next(p, items);
+      Meta far = fetch_page(w, it + 2 < count);
+      fetch_scales(nxt);
+      const int st = it % NS;
+      if (it >= NS && !__all_sync(0xffffffffu, mbar_wait_sleep(&empty[st], ((it / NS) - 1) & 1))) break;
+      if (lane < NT) {
+        float* mt = meta + st * 3 * NT;
+        const bool bad = !(cur.vs < INFINITY);  // NaN or inf
+        const float v = bad ? 1.f : fmaxf(cur.vs, kMinVs);
+        mt[lane] = cur.ks;
+        mt[NT + lane] = bad ? __uint_as_float(0x7fffffffu) : log2f(v) + kPBias;
+        mt[2 * NT + lane] = kLBiasInv / v;
+      }
+      __syncwarp();
+      const int boxes = min(nbox, (cur.ctx - cur.tok0 + p.box_rows - 1) / p.box_rows);
+      if (lane == 0) mbar_arrive_expect_tx(&full[st], boxes * 2 * C::CB * p.box_rows * C::ROWB);
+      __syncwarp();
+      const int src = lane < nbox ? lane * tiles_per_box : 0;
+      const int page = static_cast<int>(__shfl_sync(0xffffffffu, cur.page, src));
+      const int row = __shfl_sync(0xffffffffu, cur.row, src);
+      if (lane < boxes) {
+        uint8_t* k = smem + st * C::STAGE + lane * p.box_rows * C::ROWB;
+#pragma unroll
+        for (int cb = 0; cb < C::CB; ++cb) {
+          tma_load_4d(k + cb * CH * C::ROWB, &tmK, &full[st], cb * 128, row, cur.kvh, page);
+          tma_load_4d(k + C::PLANE + cb * CH * C::ROWB, &tmV, &full[st], cb * 128, row, cur.kvh, page);
+        }
+      }
+      cur = nxt;
+      nxt = far;
+    }
+    return;
+  }
+
+  // ---------------- consumers ----------------
+  const int wm = warp % WM, wk = warp / WM, g = lane >> 2, t4 = lane & 3, mi = lane >> 3, rr = lane & 7;
+  const uint32_t sbase = smem_u32(smem);
+  Kv8Walk<CH> w = w0;
+  int it = 0;
+  while (it < count) {
+    // one item: chunks [w.j, j_end) of it are this CTA's
+    const int j0 = w.j, j_end = min(w.n, w.j + (count - it)), s = w.s, ctx = w.ctx;
+    const int kvh = w.r / p.chunks, rc = w.r - kvh * p.chunks;
+
+    // ---- query rows to fp16 A fragments, each row scaled by a power of two ----
+    // k order: thread t4 of a quad holds elements 4 t4 .. 4 t4 + 3 of each 16, the
+    // order in which one 32-bit word of codes has them
+    uint32_t qa[C::QSMEM ? 1 : DP / 16][4];
+    uint4* const qs = reinterpret_cast<uint4*>(smem + C::Q_OFF) + wm * (DP / 16) * 32 + lane;
+    float fac[2];
+    int lim[2], row_id[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int row = rc * RT + wm * 16 + g + half * 8;
+      const bool real = row < p.rows;
+      row_id[half] = real ? row : -1;
+      const int i = real ? row / p.G : 0, hh = real ? row - i * p.G : 0;
+      lim[half] = real ? ctx - p.Lq + i + 1 : 0;
+      const uint16_t* src = static_cast<const uint16_t*>(p.q) + s * p.sq[0] + i * p.sq[1] + (kvh * p.G + hh) * p.sq[2];
+      auto element = [&](int e) {
+        const int d = (e >> 2) * 16 + 4 * t4 + (e & 3);
+        const uint16_t raw = real && d < p.c.D ? src[d * p.sq[3]] : 0;
+        return p.bf16 ? __uint_as_float(static_cast<uint32_t>(raw) << 16) : __half2float(__ushort_as_half(raw));
+      };
+      float top = 0.f;
+      bool odd = false;
+#pragma unroll 16
+      for (int e = 0; e < DP / 4; ++e) {
+        const float x = element(e);
+        top = fmaxf(top, fabsf(x));
+        odd |= !(fabsf(x) < INFINITY);
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      odd |= __shfl_xor_sync(0xffffffffu, odd, 1);
+      odd |= __shfl_xor_sync(0xffffffffu, odd, 2);
+      // 2^e <= top < 2^(e+1); the row's largest comes to [2^8, 2^9)
+      const int e2 = odd || top == 0.f ? 8 : max(-110, static_cast<int>(__float_as_uint(top) >> 23) - 127);
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + 8 - e2) << 23);
+      fac[half] = p.scale * __uint_as_float(static_cast<uint32_t>(127 - 8 + e2) << 23);
+#pragma unroll
+      for (int e = 0; e < DP / 4; e += 2) {  // read again (L1): held, they would cost the registers
+        const uint32_t v = Elem<__half>::pack2(element(e) * up, element(e + 1) * up);
+        if (!C::QSMEM) qa[C::QSMEM ? 0 : e >> 2][half + (e & 2)] = v;
+        else if (wk == 0) reinterpret_cast<uint32_t*>(qs + (e >> 2) * 32)[half + (e & 2)] = v;
+      }
+    }
+    // (the last item's readers are past its closing barriers)
+    if (C::QSMEM) asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");
+
+    float o[DP / 8][4];
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const int open = ctx - p.Lq + 1;  // keys below it are seen by every row
+
+    for (int j = j0; j < j_end; ++j, ++it) {
+      const int st = it % NS;
+      if (!mbar_wait(&full[st], (it / NS) & 1)) {
+        it = count;
+        break;
+      }
+      const uint32_t kbase = sbase + st * C::STAGE, vbase = kbase + C::PLANE;
+      const float* mt = meta + st * 3 * NT;
+#pragma unroll 1
+      for (int t = wk; t < NT; t += WK) {
+        const int tok = j * CH + t * 16;
+        if (tok >= ctx) break;
+        const int r0 = t * 16;
+        if (CODE == kE4M3 && tok + 16 > ctx) {
+          // rows past the end may hold NaN codes: zero their V rows (several
+          // warps may write the same zeros)
+          uint8_t* vt = smem + st * C::STAGE + C::PLANE;
+          for (int i = lane; i < 16 * C::CB * (C::ROWB / 16); i += 32) {
+            const int r = i / (C::CB * (C::ROWB / 16)), cc = i % (C::CB * (C::ROWB / 16));
+            if (tok + r >= ctx)
+              *reinterpret_cast<uint4*>(vt + (cc / 8) * CH * C::ROWB + kv8_sw<DP>(r0 + r, cc % 8)) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        // ---- S = Q Kc^T for 16 keys ----
+        float sacc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll(C::QSMEM ? 2 : DP / 32)
+        for (int kb = 0; kb < DP / 32; ++kb) {
+          const int piece = 2 * kb + (mi & 1);
+          uint32_t r[4];
+          ldsm_x4(kbase + (piece >> 3) * CH * C::ROWB + kv8_sw<DP>(r0 + (mi >> 1) * 8 + rr, piece & 7), r[0], r[1], r[2], r[3]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {  // k16 step; r[x]: the first eight keys, r[x + 2]: the others
+            uint32_t b0, b1, qf[4];
+            if (C::QSMEM) *reinterpret_cast<uint4*>(qf) = qs[(2 * kb + x) * 32];
+            const uint32_t* q4 = C::QSMEM ? qf : qa[C::QSMEM ? 0 : 2 * kb + x];
+            codes_to_half<CODE, 0>(r[x], b0, b1);
+            Mma<__half>::run(sacc[0], q4, b0, b1);
+            codes_to_half<CODE, 0>(r[x + 2], b0, b1);
+            Mma<__half>::run(sacc[1], q4, b0, b1);
+          }
+        }
+        // ---- scores, base 2 ----
+        const float ks = mt[t], lvt = mt[NT + t], ivs = mt[2 * NT + t];
+        const bool v_bad = lvt != lvt;
+        const float lv = v_bad ? kPBias : lvt;  // + kPBias
+        const bool masked = tok + 16 > open;
+        float x[2][4];
+        const float f0 = fac[0] * ks, f1 = fac[1] * ks;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float z = sacc[nt][e] * (e < 2 ? f0 : f1);
+            if (p.inv_cap > 0.f) {
+              // cap * tanh(z / cap) = cap * (1 - 2 / (1 + e^(2 z / cap)))
+              const float ez = fast_exp2(z * p.inv_cap);
+              z = p.cap2 * (1.f - __fdividef(2.f, 1.f + ez));
+            }
+            if (masked && tok + nt * 8 + 2 * t4 + (e & 1) >= lim[e >> 1]) z = -INFINITY;
+            x[nt][e] = z;
+          }
+        if (p.scores && tok < p.score_ld) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            if (row_id[half] >= 0) {
+              float* sp = p.scores + ((static_cast<int64_t>(s) * p.c.Hkv + kvh) * p.rows + row_id[half]) * p.score_ld + tok + 2 * t4;
+              *reinterpret_cast<float2*>(sp) = make_float2(x[0][2 * half], x[0][2 * half + 1]);
+              *reinterpret_cast<float2*>(sp + 8) = make_float2(x[1][2 * half], x[1][2 * half + 1]);
+            }
+        }
+        // ---- running maximum: raised only when a score passes it by 2^kLag ----
+        float c0 = lv - (m[0] == -INFINITY ? 0.f : m[0]), c1 = lv - (m[1] == -INFINITY ? 0.f : m[1]);
+        const float y0 = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
+        const float y1 = fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3]));
+        const bool up = y0 + c0 > (m[0] == -INFINITY ? -INFINITY : kLag + kPBias) || y1 + c1 > (m[1] == -INFINITY ? -INFINITY : kLag + kPBias);
+        if (__any_sync(0xffffffffu, up)) {
+          float mx[2] = {y0 + (lv - kPBias), y1 + (lv - kPBias)}, al[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+            const float mn = fmaxf(m[r], mx[r]), mu = mn == -INFINITY ? 0.f : mn;
+            al[r] = fast_exp2(m[r] - mu);
+            m[r] = mn;
+            l[r] *= al[r];
+          }
+          c0 = lv - (m[0] == -INFINITY ? 0.f : m[0]);
+          c1 = lv - (m[1] == -INFINITY ? 0.f : m[1]);
+#pragma unroll
+          for (int i = 0; i < DP / 8; ++i) {
+            o[i][0] *= al[0];
+            o[i][1] *= al[0];
+            o[i][2] *= al[1];
+            o[i][3] *= al[1];
+          }
+        }
+        float ps[2] = {0.f, 0.f};
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[nt][e] = fast_exp2(x[nt][e] + (e < 2 ? c0 : c1));
+            ps[e >> 1] += x[nt][e];
+          }
+        l[0] = fmaf(ps[0], ivs, l[0]);
+        l[1] = fmaf(ps[1], ivs, l[1]);
+        uint32_t pa[4];
+        pa[0] = Elem<__half>::pack2(x[0][0], x[0][1]);
+        pa[1] = Elem<__half>::pack2(x[0][2], x[0][3]);
+        pa[2] = Elem<__half>::pack2(x[1][0], x[1][1]);
+        pa[3] = Elem<__half>::pack2(x[1][2], x[1][3]);
+        if (v_bad) {  // a NaN or infinite V scale: NaN for the rows that see a key of the tile
+          pa[0] = pa[2] = tok < lim[0] ? 0x7fff7fffu : 0u;
+          pa[1] = pa[3] = tok < lim[1] ? 0x7fff7fffu : 0u;
+        }
+        // ---- O += P Vc: words transposed by the load pair two keys of columns
+        // 2 g and 2 g + 1, so even and odd columns are two n tiles ----
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) {
+          const int piece = 2 * db + (mi >> 1);
+          uint32_t r[4];
+          ldsm_x4_t(vbase + (piece >> 3) * CH * C::ROWB + kv8_sw<DP>(r0 + (mi & 1) * 8 + rr, piece & 7), r[0], r[1], r[2], r[3]);
+#pragma unroll
+          for (int x2 = 0; x2 < 2; ++x2) {
+            uint32_t e0, o0, e1, o1;
+            codes_to_half<CODE, 1>(r[2 * x2], e0, o0);
+            codes_to_half<CODE, 1>(r[2 * x2 + 1], e1, o1);
+            Mma<__half>::run(o[4 * db + 2 * x2], pa, e0, e1);
+            Mma<__half>::run(o[4 * db + 2 * x2 + 1], pa, o0, o1);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+
+    // ---- join the warps that shared the rows, then finish or store a part ----
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+    const bool whole = j0 == 0 && j_end == w.n;
+    const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (j0 == 0 ? 1 : 0)) * RT;
+#pragma unroll
+    for (int dh = 0; dh < DP / C::DH; ++dh) {
+      asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");  // the buffer is free again
+#pragma unroll
+      for (int i = 0; i < C::DH / 16; ++i) {
+        const float(*ot)[4] = &o[dh * (C::DH / 8) + 2 * i];
+        float* dst = obuf + (warp * 16 + g) * C::DH + i * 16 + 4 * t4;
+        *reinterpret_cast<float4*>(dst) = make_float4(ot[0][0], ot[1][0], ot[0][1], ot[1][1]);
+        *reinterpret_cast<float4*>(dst + 8 * C::DH) = make_float4(ot[0][2], ot[1][2], ot[0][3], ot[1][3]);
+      }
+      if (dh == 0 && t4 == 0) {
+        mlbuf[(warp * 16 + g) * 2] = m[0];
+        mlbuf[(warp * 16 + g) * 2 + 1] = l[0];
+        mlbuf[(warp * 16 + g + 8) * 2] = m[1];
+        mlbuf[(warp * 16 + g + 8) * 2 + 1] = l[1];
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");
+      for (int e = tid; e < RT * (C::DH / 4); e += NW * 32) {
+        const int row = e / (C::DH / 4), d = (e - row * (C::DH / 4)) * 4;
+        const int grow = rc * RT + row;
+        if (grow >= p.rows) continue;
+        const int tile = row >> 4, r16 = row & 15;
+        float M = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < WK; ++k) M = fmaxf(M, mlbuf[((k * WM + tile) * 16 + r16) * 2]);
+        const float Mu = M == -INFINITY ? 0.f : M;
+        float L = 0.f;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < WK; ++k) {
+          const int at = (k * WM + tile) * 16 + r16;
+          const float f = fast_exp2(mlbuf[at * 2] - Mu);
+          L = fmaf(mlbuf[at * 2 + 1], f, L);
+          const float4 v = *reinterpret_cast<const float4*>(obuf + at * C::DH + d);
+          a.x = fmaf(v.x, f, a.x);
+          a.y = fmaf(v.y, f, a.y);
+          a.z = fmaf(v.z, f, a.z);
+          a.w = fmaf(v.w, f, a.w);
+        }
+        const int dd = dh * C::DH + d;
+        if (whole) {
+          const int i = grow / p.G, h = kvh * p.G + grow - i * p.G;
+          const float inv = L != 0.f ? kLBiasInv / L : 0.f;
+          uint16_t* out = static_cast<uint16_t*>(p.out) + s * p.so[0] + i * p.so[1] + h * p.so[2];
+          const float f[4] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (dd + k < p.c.D)
+              out[(dd + k) * p.so[3]] = p.bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f[k])) : __half_as_ushort(__float2half_rn(f[k]));
+          if (dd == 0) {
+            const float v = L != 0.f ? M + kLBias + log2f(L) : -INFINITY;
+            if (p.lse) p.lse[(static_cast<int64_t>(s) * p.Lq + i) * p.H + h] = v * kLn2;
+            if (p.lse2) p.lse2[(static_cast<int64_t>(s) * p.c.Hkv + kvh) * p.rows + grow] = v;
+          }
+        } else {
+          *reinterpret_cast<float4*>(p.part_o + (slot + row) * DP + dd) = a;
+          if (dd == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + row) * 2) = make_float2(M, L);
+        }
+      }
+    }
+    // the next item
+    w.j = j_end - 1;
+    w.next(p, items);
+  }
+}
+
+// Joins the parts of the items that the split cut.  CTA (c, y) looks at the
+// boundary before the main grid's CTA c: if it is the first one inside its item,
+// it merges the item's parts, in order, for four query rows.
+template <int DP>
+__global__ void __launch_bounds__(128) kv8_attention_join_kernel(const Kv8TcParams p, int RT, int N) {
+  constexpr int MAXP = 512;
+  __shared__ float wt[4][MAXP];
+  __shared__ int ids[MAXP];
+  __shared__ int sh_n;
+  __shared__ float sh_inv[4];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c = blockIdx.x + 1, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int4 b = p.bound[c];
+  if (b.z == 0) return;  // an item begins here, or the CTA had no chunk
+  // parts: the CTA in which the item begins (slot 1), then the CTAs up to its
+  // end (slot 0); those in between cover it without a gap
+  if (warp == 0) {
+    int prev = c - 1;
+    while (prev > 0 && p.bound[prev].w == 0) --prev;  // CTAs without a chunk
+    const int4 a = p.bound[prev];
+    const bool first = !(a.x == b.x && a.y == b.y && a.z > 0);
+    int n = 0;
+    if (first) {
+      if (lane == 0) ids[0] = prev * 2 + 1;
+      n = 1;
+      for (int k0 = c; k0 < N; k0 += 32) {
+        const int k = k0 + lane;
+        const int4 e = k < N ? p.bound[k] : make_int4(-1, 0, 1, 1);
+        const bool in = e.w > 0 && e.x == b.x && e.y == b.y && e.z > 0;
+        const bool stop = e.w > 0 && !in;
+        const unsigned mi = __ballot_sync(0xffffffffu, in), ms = __ballot_sync(0xffffffffu, stop);
+        if (in && n + __popc(mi & ((1u << lane) - 1)) < MAXP) ids[n + __popc(mi & ((1u << lane) - 1))] = k * 2;
+        n += __popc(mi);
+        if (ms) break;
+      }
+    }
+    if (lane == 0) sh_n = min(n, MAXP);
+  }
+  __syncthreads();
+  const int n = sh_n;
+  if (n == 0) return;
+  const int s = b.x, kvh = b.y / p.chunks, rc = b.y - kvh * p.chunks, row0 = blockIdx.y * 4;
+  {
+    const int row = row0 + warp;
+    float M = -INFINITY;
+    for (int k = lane; k < n; k += 32) M = fmaxf(M, p.part_ml[(static_cast<int64_t>(ids[k]) * RT + row) * 2]);
+    M = warp_max(M);
+    const float Mu = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    for (int k = lane; k < n; k += 32) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (static_cast<int64_t>(ids[k]) * RT + row) * 2);
+      const float f = fast_exp2(ml.x - Mu);
+      wt[warp][k] = f;
+      L = fmaf(ml.y, f, L);
+    }
+    L = warp_sum(L);
+    const int grow = rc * RT + row;
+    if (lane == 0) {
+      sh_inv[warp] = L != 0.f ? kLBiasInv / L : 0.f;
+      if (grow < p.rows) {
+        const float v = L != 0.f ? M + kLBias + log2f(L) : -INFINITY;
+        const int i = grow / p.G, h = kvh * p.G + grow - i * p.G;
+        if (p.lse) p.lse[(static_cast<int64_t>(s) * p.Lq + i) * p.H + h] = v * kLn2;
+        if (p.lse2) p.lse2[(static_cast<int64_t>(s) * p.c.Hkv + kvh) * p.rows + grow] = v;
+      }
+    }
+  }
+  __syncthreads();
+  for (int e = tid; e < 4 * (DP / 4); e += 128) {
+    const int r = e / (DP / 4), d = (e - r * (DP / 4)) * 4, grow = rc * RT + row0 + r;
+    if (grow >= p.rows) continue;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < n; k0 += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (k0 + u < n) v[u] = *reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(ids[k0 + u]) * RT + row0 + r) * DP + d);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (k0 + u < n) {
+          const float f = wt[r][k0 + u];
+          a.x = fmaf(v[u].x, f, a.x);
+          a.y = fmaf(v[u].y, f, a.y);
+          a.z = fmaf(v[u].z, f, a.z);
+          a.w = fmaf(v[u].w, f, a.w);
+        }
+    }
+    const float inv = sh_inv[r];
+    const int i = grow / p.G, h = kvh * p.G + grow - i * p.G;
+    uint16_t* out = static_cast<uint16_t*>(p.out) + s * p.so[0] + i * p.so[1] + h * p.so[2];
+    const float f[4] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (d + k < p.c.D)
+        out[(d + k) * p.so[3]] = p.bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f[k])) : __half_as_ushort(__float2half_rn(f[k]));
+  }
+}
+
+// Attention weights from the stored scores: each thread owns keys, so every
+// weight is added to once, in the order of the rows.
+__global__ void __launch_bounds__(256) kv8_attention_weights_kernel(const Kv8TcParams p, float* weights, int64_t w0,
+                                                                    int64_t w1, int64_t w2, int64_t width) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int kvh = blockIdx.y, s = blockIdx.z;
+  const int64_t n = min(static_cast<int64_t>(kv8_ctx(p, s)), width);
+  const int64_t pos = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (pos >= n) return;
+  const int64_t item = static_cast<int64_t>(s) * p.c.Hkv + kvh;
+  const float* sc = p.scores + item * p.rows * p.score_ld + pos;
+  const float* ls = p.lse2 + item * p.rows;
+  float sum = 0.f;
+  for (int r = 0; r < p.rows; ++r) {
+    const float L = ls[r];
+    const float e = fast_exp2(sc[r * p.score_ld] - L);
+    sum += L == -INFINITY ? 0.f : e;
+  }
+  weights[s * w0 + kvh * w1 + pos * w2] += sum;
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+static bool tc_ok(const Kv8View& c, const Kv8AttnArgs& a) {
+  if (a.force_generic || a.dtype == kF32 || c.D > 256 || c.P % 16 || c.group % 16) return false;
+  if (c.num_blocks == 0 || c.max_blocks == 0) return false;
+  for (const Kv8Plane& pl : c.plane) {
+    if (pl.sc[3] != 1 || (reinterpret_cast<uintptr_t>(pl.code) & 15)) return false;
+    for (int i = 0; i < 3; ++i)
+      if (pl.sc[i] <= 0 || pl.sc[i] % 16 || pl.sc[i] >= (int64_t{1} << 40)) return false;
+  }
+  return true;
+}
+static int tc_dp(const Kv8View& c) { return c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256; }
+// query rows a CTA holds: 16 per warp row, as many warp rows as the rows fill
+static int tc_wm(const Kv8View& c, const Kv8AttnArgs& a) {
+  const int64_t rows = static_cast<int64_t>(a.H / c.Hkv) * a.Lq;
+  return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+}
+struct TcSizes { int N, RT, DP; int64_t bound, ml, o, lse2, scores, total, score_ld; };
+static int64_t up16(int64_t x) { return (x + 255) / 256 * 256; }
+static TcSizes tc_sizes(const Kv8View& c, const Kv8AttnArgs& a) {
+  TcSizes z{};
+  z.DP = tc_dp(c);
+  z.N = num_sms() * (z.DP >= 256 ? 1 : 2);
+  z.RT = 16 * tc_wm(c, a);
+  const int64_t rows = static_cast<int64_t>(a.H / c.Hkv) * a.Lq, all = rows * c.Hkv * c.num_seqs;
+  int64_t at = 0;
+  z.bound = at; at += up16(static_cast<int64_t>(z.N) * 16);
+  z.ml = at; at += up16(static_cast<int64_t>(z.N) * 2 * z.RT * 8);
+  z.o = at; at += up16(static_cast<int64_t>(z.N) * 2 * z.RT * z.DP * 4);
+  if (a.weights) {
+    const int64_t w = a.weights_width < c.max_rows ? a.weights_width : c.max_rows;
+    z.score_ld = (w + 15) / 16 * 16;
+    z.lse2 = at; at += up16(all * 4);
+    z.scores = at; at += up16(all * z.score_ld * 4);
+  }
+  z.total = at + 256;
+  return z;
+}
+
+int64_t kv8_attention_ws_bytes(const Kv8View& c, const Kv8AttnArgs& a) {
+  if (tc_ok(c, a)) return tc_sizes(c, a).total;
+  return a.weights ? static_cast<int64_t>(c.num_seqs) * a.Lq * a.H * 4 : 0;
+}
+
+static int encode_codes(CUtensorMap* map, const Kv8View& c, int w, int box_cols, int box_rows) {
+  const Kv8Plane& pl = c.plane[w];
+  const uint64_t dims[4] = {static_cast<uint64_t>(c.D), static_cast<uint64_t>(c.P), static_cast<uint64_t>(c.Hkv),
+                            static_cast<uint64_t>(c.num_blocks)};
+  const uint64_t strides[3] = {static_cast<uint64_t>(pl.sc[2]), static_cast<uint64_t>(pl.sc[1]),
+                               static_cast<uint64_t>(pl.sc[0])};
+  const uint32_t box[4] = {static_cast<uint32_t>(box_cols), static_cast<uint32_t>(box_rows), 1, 1};
+  const uint32_t es[4] = {1, 1, 1, 1};
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, pl.code, dims, strides, box, es,
+                      box_cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+template <typename K, typename... A>
+static int launch_dependent(K kern, dim3 grid, int threads, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (e == cudaSuccess) return 0;
+  char buf[160];
+  std::snprintf(buf, sizeof(buf), "kv8 attention: launch failed: %s", cudaGetErrorString(e));
+  return set_error(3, buf);
+}
+
+template <int CODE, int DP, int WM>
+static int launch_tc(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
+  using C = Kv8Cfg<DP, WM>;
+  const TcSizes z = tc_sizes(c, a);
+  Kv8TcParams p{};
+  p.c = c;
+  p.q = a.q;
+  p.out = a.out;
+  for (int i = 0; i < 4; ++i) { p.sq[i] = a.sq[i]; p.so[i] = a.so[i]; }
+  p.context_lens = a.context_lens;
+  p.lse = a.lse;
+  p.bf16 = a.dtype == kBF16;
+  p.H = a.H; p.Lq = a.Lq; p.G = a.H / c.Hkv; p.rows = p.G * a.Lq;
+  p.chunks = (p.rows + z.RT - 1) / z.RT;
+  p.box_rows = c.P & -c.P;
+  if (p.box_rows > C::CH) p.box_rows = C::CH;
+  p.scale = a.softcap > 0.f ? a.scale : a.scale * kLog2e;
+  p.cap2 = a.softcap * kLog2e;
+  p.inv_cap = a.softcap > 0.f ? 2.f * kLog2e / a.softcap : 0.f;
+  uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(a.workspace) + 255) & ~uintptr_t(255));
+  p.bound = reinterpret_cast<int4*>(ws + z.bound);
+  p.part_ml = reinterpret_cast<float*>(ws + z.ml);
+  p.part_o = reinterpret_cast<float*>(ws + z.o);
+  if (a.weights) {
+    p.lse2 = reinterpret_cast<float*>(ws + z.lse2);
+    p.scores = reinterpret_cast<float*>(ws + z.scores);
+    p.score_ld = z.score_ld;
+  }
+  CUtensorMap mk, mv;
+  if (const int r = encode_codes(&mk, c, 0, C::ROWB, p.box_rows)) return r;
+  if (const int r = encode_codes(&mv, c, 1, C::ROWB, p.box_rows)) return r;
+  auto kern = kv8_attention_tc_kernel<CODE, DP, WM>;
+  if (const int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::SMEM)) return r;
+  kern<<<z.N, (C::NW + 1) * 32, C::SMEM, st>>>(mk, mv, p);
+  note_kernel("kv8_attention_tc");
+  if (const int r = launch_dependent(kv8_attention_join_kernel<DP>, dim3(z.N - 1, z.RT / 4), 128, st, p, z.RT, z.N)) return r;
+  if (a.weights) {
+    const int64_t w = a.weights_width < c.max_rows ? a.weights_width : c.max_rows;
+    return launch_dependent(kv8_attention_weights_kernel, dim3(static_cast<unsigned>((w + 255) / 256), c.Hkv, c.num_seqs),
+                            256, st, p, a.weights, a.sw[0], a.sw[1], a.sw[2], w);
+  }
+  return 0;
+}
+
+template <int CODE, int DP>
+static int launch_wm(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
+  switch (tc_wm(c, a)) {
+    case 1: return launch_tc<CODE, DP, 1>(c, a, st);
+    case 2: return launch_tc<CODE, DP, 2>(c, a, st);
+    default: return launch_tc<CODE, DP, 4>(c, a, st);
+  }
+}
+
+int kv8_attention_launch(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
+  if (kv8_attention_ws_bytes(c, a) > a.workspace_bytes) return set_error(2, "kv8 attention: workspace too small");
+  if (!tc_ok(c, a)) return kv8_attention_generic_launch(c, a, st);
+  TAK_BY_CODE(a.code_type, {
+    switch (tc_dp(c)) {
+      case 64: return launch_wm<CODE, 64>(c, a, st);
+      case 128: return launch_wm<CODE, 128>(c, a, st);
+      default: return launch_wm<CODE, 256>(c, a, st);
+    }
+  });
+  return 0;
+}
+
+}  // namespace tak

@@ -172,13 +172,4 @@ int kv8_attention_generic_launch(const Kv8View& c, const Kv8AttnArgs& a, cudaStr
   return 0;
 }
 
-int64_t kv8_attention_ws_bytes(const Kv8View& c, const Kv8AttnArgs& a) {
-  return a.weights ? static_cast<int64_t>(c.num_seqs) * a.Lq * a.H * 4 : 0;
-}
-
-int kv8_attention_launch(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
-  if (kv8_attention_ws_bytes(c, a) > a.workspace_bytes) return set_error(2, "kv8 attention: workspace too small");
-  return kv8_attention_generic_launch(c, a, st);
-}
-
 }  // namespace tak
