@@ -38,6 +38,7 @@ struct Kv8TcParams {
   void* out; int64_t so[4];
   float* lse;
   int bf16;          // q and out are bf16 (else fp16)
+  int q_vec;         // four consecutive elements of q are one aligned 8-byte word
   int H, Lq, G, rows, chunks;  // rows = G * Lq query rows per KV head, in `chunks` chunks
   int box_rows;      // rows of one TMA box: the largest power of two dividing block_size, at most CH
   float scale;       // softmax scale * log2(e); with a cap: softmax scale
@@ -60,18 +61,20 @@ constexpr float kPBias = 13.f;
 constexpr float kLag = 2.f;
 constexpr float kLBias = 10.f;
 constexpr float kLBiasInv = 1.1920928955078125e-7f;  // 2^-(kPBias + kLBias)
+constexpr float kHalfMin = 6.103515625e-5f;  // 2^-14: fp16's smallest normal number
 constexpr float kMinVs = 6.162975822039155e-33f;  // 2^-107: the smallest scale that the write makes
 
 template <int DP, int WM> struct Kv8Cfg {
   static constexpr int NW = DP >= 256 ? 8 : 4;          // consumer warps
-  static constexpr int CH = DP == 128 ? 64 : 128;       // keys of a chunk
+  static constexpr int CH = 128;                        // keys of a chunk
+  static constexpr int TP = DP >= 256 ? 1 : 2;          // key tiles of a warp's step (two: independent MMA chains)
   static constexpr int NT = CH / 16;                    // key tiles of a chunk
   static constexpr int CB = DP >= 256 ? 2 : 1;          // column blocks of a row
   static constexpr int ROWB = DP >= 128 ? 128 : 64;     // bytes of a row in a column block
   static constexpr int PLANE = CH * DP;                 // bytes of K (or V) in a stage
   static constexpr int STAGE = 2 * PLANE;
-  static constexpr int NS = DP >= 256 ? 2 : 4;
-  static constexpr int DH = DP < 128 ? DP : 128;        // columns merged at a time
+  static constexpr int NS = DP >= 256 ? 2 : DP == 128 ? 3 : 5;
+  static constexpr int DH = DP >= 256 ? 128 : DP == 128 ? 32 : 64; // columns merged at a time
   static constexpr int MERGE = NW * 16 * DH * 4;
   static constexpr int META_OFF = NS * STAGE;           // [NS][3][NT] floats: ks, log2 vs, 2^-23 / vs
   static constexpr int OBUF_OFF = META_OFF + NS * 3 * NT * 4;
@@ -83,7 +86,7 @@ template <int DP, int WM> struct Kv8Cfg {
   static constexpr int BAR_OFF = Q_OFF + (QSMEM ? WM * (DP / 16) * 512 : 0);
   static constexpr int SMEM = BAR_OFF + 2 * NS * 8 + 64 + 1024;
   static constexpr int CTAS = DP >= 256 ? 1 : 2;        // per SM
-  static_assert(SMEM * CTAS <= 227 * 1024, "shared memory");
+  static_assert((SMEM + 1024) * CTAS <= 228 * 1024, "shared memory");
 };
 
 // byte offset of 16-byte piece `c` of row `r` in a column block
@@ -102,6 +105,7 @@ __device__ __forceinline__ uint32_t hsub2_1152(uint32_t x) {
   __half2 h = __hsub2(*reinterpret_cast<__half2*>(&x), k);
   return *reinterpret_cast<uint32_t*>(&h);
 }
+__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
 // Four codes to two fp16 pairs.  int8: the byte with its sign bit flipped goes
 // into the mantissa of 1024 (fp16 0x6400, where an ulp is 1): 1024 + 128 + x,
 // less 1152.  PAIR = 0 pairs bytes (0,1) (2,3), PAIR = 1 bytes (0,2) (1,3).
@@ -124,15 +128,26 @@ __device__ __forceinline__ int kv8_ctx(const Kv8TcParams& p, int s) {
   return n > 0 ? static_cast<int>(n) : 0;
 }
 
-// Walks a CTA's chunks in order: item `r` of sequence `s`, chunk `j` of `n`.
+// Positions in the work list: an item of n chunks takes n + kItemCost places, the
+// last kItemCost of them empty.  They stand for what an item costs besides its
+// chunks (query rows, joining the warps, the output), so that CTAs with many
+// short items get fewer chunks.
+constexpr int kItemCost = 2;
+template <int CH> __device__ __forceinline__ int64_t kv8_places(int ctx) {
+  return ctx > 0 ? (ctx + CH - 1) / CH + kItemCost : 0;
+}
+
+// Walks a CTA's chunks in order: item `r` of sequence `s`, chunk `j` of `n`, at
+// place `at`.
 template <int CH> struct Kv8Walk {
+  int64_t at;
   int s, r, j, n, ctx;
   __device__ __forceinline__ void load(const Kv8TcParams& p) {
     ctx = kv8_ctx(p, s);
     n = (ctx + CH - 1) / CH;
   }
-  __device__ __forceinline__ void next(const Kv8TcParams& p, int items) {
-    if (++j < n) return;
+  __device__ __forceinline__ void next_item(const Kv8TcParams& p, int items) {
+    at += n - j + kItemCost;
     j = 0;
     if (++r < items) return;
     r = 0;
@@ -141,6 +156,15 @@ template <int CH> struct Kv8Walk {
       load(p);
     } while (n == 0);
   }
+  __device__ __forceinline__ void next(const Kv8TcParams& p, int items) {
+    if (j + 1 < n) {
+      ++j;
+      ++at;
+    } else {
+      next_item(p, items);
+    }
+  }
+  __device__ __forceinline__ bool live(const Kv8TcParams& p, int64_t end) const { return at < end && s < p.c.num_seqs; }
 };
 
 template <int CODE, int DP, int WM>
@@ -148,7 +172,7 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
     kv8_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                             const __grid_constant__ Kv8TcParams p) {
   using C = Kv8Cfg<DP, WM>;
-  constexpr int NW = C::NW, CH = C::CH, NT = C::NT, NS = C::NS, WK = NW / WM, RT = 16 * WM;
+  constexpr int NW = C::NW, CH = C::CH, NT = C::NT, TP = C::TP, NS = C::NS, WK = NW / WM, RT = 16 * WM;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* meta = reinterpret_cast<float*>(smem + C::META_OFF);
@@ -172,11 +196,11 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
     fence_barrier_init();
   }
 
-  // ---- where this CTA's chunks begin: prefix sums of the sequences' chunks ----
+  // ---- where this CTA's chunks begin: prefix sums of the sequences' places ----
   const int seg = (B + THREADS - 1) / THREADS;
   const int s_lo = min(B, tid * seg), s_hi = min(B, s_lo + seg);
   int64_t mine = 0;
-  for (int s = s_lo; s < s_hi; ++s) mine += (kv8_ctx(p, s) + CH - 1) / CH;
+  for (int s = s_lo; s < s_hi; ++s) mine += kv8_places<CH>(kv8_ctx(p, s));
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -193,12 +217,12 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
   }
   const int64_t U = total * items;
   const int64_t u0 = U * blockIdx.x / gridDim.x, u1 = U * (blockIdx.x + 1) / gridDim.x;
-  before += incl - mine;  // chunks (of one item) before this thread's sequences
+  before += incl - mine;  // places (of one item) before this thread's sequences
   if (u0 < U && mine > 0 && before * items <= u0 && u0 < (before + mine) * items) {
     int s = s_lo;
     int64_t b = before;
     for (;; ++s) {
-      const int n = (kv8_ctx(p, s) + CH - 1) / CH;
+      const int64_t n = kv8_places<CH>(kv8_ctx(p, s));
       if (u0 < (b + n) * items) break;
       b += n;
     }
@@ -224,10 +248,13 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
   Kv8Walk<CH> w0;
   w0.s = sh_seq;
   w0.load(p);
-  w0.r = static_cast<int>((u0 - sh_base) / w0.n);
-  w0.j = static_cast<int>((u0 - sh_base) % w0.n);
-  if (tid == 0) p.bound[blockIdx.x] = make_int4(w0.s, w0.r, w0.j, w0.n);
-  const int count = static_cast<int>(u1 - u0);
+  w0.at = u0;
+  w0.r = static_cast<int>((u0 - sh_base) / (w0.n + kItemCost));
+  w0.j = static_cast<int>((u0 - sh_base) % (w0.n + kItemCost));
+  if (w0.j >= w0.n) w0.next_item(p, items);  // u0 lies on an item's empty places
+  const bool any = w0.live(p, u1);
+  if (tid == 0) p.bound[blockIdx.x] = any ? make_int4(w0.s, w0.r, w0.j, w0.n) : make_int4(0, 0, 0, 0);
+  if (!any) return;
 
   if (warp == NW) {
     // ---------------- producer ----------------
@@ -260,13 +287,19 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
       }
     };
     Kv8Walk<CH> w = w0;
+    bool more = true, more2;  // chunks one and two ahead
     Meta cur = fetch_page(w, true);
     w.next(p, items);
-    Meta nxt = fetch_page(w, count > 1);
+    more = w.live(p, u1);
+    Meta nxt = fetch_page(w, more);
     fetch_scales(cur);
-    for (int it = 0; it < count; ++it) {
-      if (it + 1 < count) w.next(p, items);
-      Meta far = fetch_page(w, it + 2 < count);
+    for (int it = 0;; ++it) {
+      more2 = more;
+      if (more) {
+        w.next(p, items);
+        more2 = w.live(p, u1);
+      }
+      Meta far = fetch_page(w, more2);
       fetch_scales(nxt);
       const int st = it % NS;
       if (it >= NS && !__all_sync(0xffffffffu, mbar_wait_sleep(&empty[st], ((it / NS) - 1) & 1))) break;
@@ -293,8 +326,10 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
           tma_load_4d(k + C::PLANE + cb * CH * C::ROWB, &tmV, &full[st], cb * 128, row, cur.kvh, page);
         }
       }
+      if (!more) break;
       cur = nxt;
       nxt = far;
+      more = more2;
     }
     return;
   }
@@ -304,9 +339,10 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
   const uint32_t sbase = smem_u32(smem);
   Kv8Walk<CH> w = w0;
   int it = 0;
-  while (it < count) {
+  bool ok = true;
+  while (ok && w.live(p, u1)) {
     // one item: chunks [w.j, j_end) of it are this CTA's
-    const int j0 = w.j, j_end = min(w.n, w.j + (count - it)), s = w.s, ctx = w.ctx;
+    const int j0 = w.j, j_end = static_cast<int>(min(static_cast<int64_t>(w.n), w.j + (u1 - w.at))), s = w.s, ctx = w.ctx;
     const int kvh = w.r / p.chunks, rc = w.r - kvh * p.chunks;
 
     // ---- query rows to fp16 A fragments, each row scaled by a power of two ----
@@ -324,18 +360,36 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
       const int i = real ? row / p.G : 0, hh = real ? row - i * p.G : 0;
       lim[half] = real ? ctx - p.Lq + i + 1 : 0;
       const uint16_t* src = static_cast<const uint16_t*>(p.q) + s * p.sq[0] + i * p.sq[1] + (kvh * p.G + hh) * p.sq[2];
-      auto element = [&](int e) {
-        const int d = (e >> 2) * 16 + 4 * t4 + (e & 3);
-        const uint16_t raw = real && d < p.c.D ? src[d * p.sq[3]] : 0;
-        return p.bf16 ? __uint_as_float(static_cast<uint32_t>(raw) << 16) : __half2float(__ushort_as_half(raw));
+      auto to_float = [&](uint32_t raw) {
+        return p.bf16 ? __uint_as_float(raw << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(raw)));
       };
+      // four elements of 16-element block b
+      auto four = [&](int b) {
+        uint2 v = make_uint2(0, 0);
+        const int d = b * 16 + 4 * t4;
+        if (p.q_vec) {
+          if (real && d < p.c.D) v = *reinterpret_cast<const uint2*>(src + d);
+        } else {
+          uint32_t e[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) e[k] = real && d + k < p.c.D ? src[(d + k) * p.sq[3]] : 0;
+          v = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
+        }
+        return v;
+      };
+      uint2 raw[C::QSMEM ? 1 : DP / 16];
       float top = 0.f;
       bool odd = false;
-#pragma unroll 16
-      for (int e = 0; e < DP / 4; ++e) {
-        const float x = element(e);
-        top = fmaxf(top, fabsf(x));
-        odd |= !(fabsf(x) < INFINITY);
+#pragma unroll
+      for (int b = 0; b < DP / 16; ++b) {
+        const uint2 v = four(b);
+        if (!C::QSMEM) raw[C::QSMEM ? 0 : b] = v;  // 256 columns are read again instead: held, they would cost the registers
+        const float f[4] = {to_float(v.x & 0xffff), to_float(v.x >> 16), to_float(v.y & 0xffff), to_float(v.y >> 16)};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          top = fmaxf(top, fabsf(f[k]));
+          odd |= !(fabsf(f[k]) < INFINITY);
+        }
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -346,10 +400,17 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
       const float up = __uint_as_float(static_cast<uint32_t>(127 + 8 - e2) << 23);
       fac[half] = p.scale * __uint_as_float(static_cast<uint32_t>(127 - 8 + e2) << 23);
 #pragma unroll
-      for (int e = 0; e < DP / 4; e += 2) {  // read again (L1): held, they would cost the registers
-        const uint32_t v = Elem<__half>::pack2(element(e) * up, element(e + 1) * up);
-        if (!C::QSMEM) qa[C::QSMEM ? 0 : e >> 2][half + (e & 2)] = v;
-        else if (wk == 0) reinterpret_cast<uint32_t*>(qs + (e >> 2) * 32)[half + (e & 2)] = v;
+      for (int b = 0; b < DP / 16; ++b) {
+        const uint2 v = C::QSMEM ? four(b) : raw[C::QSMEM ? 0 : b];
+        const uint32_t q01 = Elem<__half>::pack2(to_float(v.x & 0xffff) * up, to_float(v.x >> 16) * up);
+        const uint32_t q23 = Elem<__half>::pack2(to_float(v.y & 0xffff) * up, to_float(v.y >> 16) * up);
+        if (!C::QSMEM) {
+          qa[C::QSMEM ? 0 : b][half] = q01;
+          qa[C::QSMEM ? 0 : b][half + 2] = q23;
+        } else if (wk == 0) {
+          reinterpret_cast<uint32_t*>(qs + b * 32)[half] = q01;
+          reinterpret_cast<uint32_t*>(qs + b * 32)[half + 2] = q23;
+        }
       }
     }
     // (the last item's readers are past its closing barriers)
@@ -364,21 +425,20 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
     for (int j = j0; j < j_end; ++j, ++it) {
       const int st = it % NS;
       if (!mbar_wait(&full[st], (it / NS) & 1)) {
-        it = count;
+        ok = false;
         break;
       }
       const uint32_t kbase = sbase + st * C::STAGE, vbase = kbase + C::PLANE;
       const float* mt = meta + st * 3 * NT;
 #pragma unroll 1
-      for (int t = wk; t < NT; t += WK) {
-        const int tok = j * CH + t * 16;
+      for (int t = wk * TP; t < NT; t += WK * TP) {
+        const int tok = j * CH + t * 16, r0 = t * 16;
         if (tok >= ctx) break;
-        const int r0 = t * 16;
-        if (CODE == kE4M3 && tok + 16 > ctx) {
+        if (CODE == kE4M3 && tok + 16 * TP > ctx) {
           // rows past the end may hold NaN codes: zero their V rows (several
           // warps may write the same zeros)
           uint8_t* vt = smem + st * C::STAGE + C::PLANE;
-          for (int i = lane; i < 16 * C::CB * (C::ROWB / 16); i += 32) {
+          for (int i = lane; i < 16 * TP * C::CB * (C::ROWB / 16); i += 32) {
             const int r = i / (C::CB * (C::ROWB / 16)), cc = i % (C::CB * (C::ROWB / 16));
             if (tok + r >= ctx)
               *reinterpret_cast<uint4*>(vt + (cc / 8) * CH * C::ROWB + kv8_sw<DP>(r0 + r, cc % 8)) = make_uint4(0, 0, 0, 0);
@@ -386,60 +446,81 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
           fence_proxy_async_smem();
           __syncwarp();
         }
-        // ---- S = Q Kc^T for 16 keys ----
-        float sacc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        // ---- S = Q Kc^T for TP tiles of 16 keys ----
+        float x[TP][2][4];
+#pragma unroll
+        for (int u = 0; u < TP; ++u)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[u][e >> 2][e & 3] = 0.f;
 #pragma unroll(C::QSMEM ? 2 : DP / 32)
         for (int kb = 0; kb < DP / 32; ++kb) {
           const int piece = 2 * kb + (mi & 1);
-          uint32_t r[4];
-          ldsm_x4(kbase + (piece >> 3) * CH * C::ROWB + kv8_sw<DP>(r0 + (mi >> 1) * 8 + rr, piece & 7), r[0], r[1], r[2], r[3]);
+          uint32_t r[TP][4];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {  // k16 step; r[x]: the first eight keys, r[x + 2]: the others
+          for (int u = 0; u < TP; ++u)
+            ldsm_x4(kbase + (piece >> 3) * CH * C::ROWB + kv8_sw<DP>(r0 + u * 16 + (mi >> 1) * 8 + rr, piece & 7), r[u][0],
+                    r[u][1], r[u][2], r[u][3]);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {  // k16 step; r[.][k]: the first eight keys, r[.][k + 2]: the others
             uint32_t b0, b1, qf[4];
-            if (C::QSMEM) *reinterpret_cast<uint4*>(qf) = qs[(2 * kb + x) * 32];
-            const uint32_t* q4 = C::QSMEM ? qf : qa[C::QSMEM ? 0 : 2 * kb + x];
-            codes_to_half<CODE, 0>(r[x], b0, b1);
-            Mma<__half>::run(sacc[0], q4, b0, b1);
-            codes_to_half<CODE, 0>(r[x + 2], b0, b1);
-            Mma<__half>::run(sacc[1], q4, b0, b1);
+            if (C::QSMEM) *reinterpret_cast<uint4*>(qf) = qs[(2 * kb + k) * 32];
+            const uint32_t* q4 = C::QSMEM ? qf : qa[C::QSMEM ? 0 : 2 * kb + k];
+#pragma unroll
+            for (int u = 0; u < TP; ++u) {
+              codes_to_half<CODE, 0>(r[u][k], b0, b1);
+              Mma<__half>::run(x[u][0], q4, b0, b1);
+              codes_to_half<CODE, 0>(r[u][k + 2], b0, b1);
+              Mma<__half>::run(x[u][1], q4, b0, b1);
+            }
           }
         }
         // ---- scores, base 2 ----
-        const float ks = mt[t], lvt = mt[NT + t], ivs = mt[2 * NT + t];
-        const bool v_bad = lvt != lvt;
-        const float lv = v_bad ? kPBias : lvt;  // + kPBias
-        const bool masked = tok + 16 > open;
-        float x[2][4];
-        const float f0 = fac[0] * ks, f1 = fac[1] * ks;
+        const bool masked = tok + 16 * TP > open;
+        float lv[TP], ivs[TP], y0 = -INFINITY, y1 = -INFINITY;  // y: largest score + log2 vs + kPBias
+        bool v_bad[TP];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+        for (int u = 0; u < TP; ++u) {
+          const float ks = mt[t + u], lvt = mt[NT + t + u], f0 = fac[0] * ks, f1 = fac[1] * ks;
+          ivs[u] = mt[2 * NT + t + u];
+          v_bad[u] = lvt != lvt;
+          lv[u] = v_bad[u] ? kPBias : lvt;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float z = sacc[nt][e] * (e < 2 ? f0 : f1);
-            if (p.inv_cap > 0.f) {
-              // cap * tanh(z / cap) = cap * (1 - 2 / (1 + e^(2 z / cap)))
-              const float ez = fast_exp2(z * p.inv_cap);
-              z = p.cap2 * (1.f - __fdividef(2.f, 1.f + ez));
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float z = x[u][nt][e] * (e < 2 ? f0 : f1);
+              if (p.inv_cap > 0.f) {
+                // cap * tanh(z / cap) = cap * (1 - 2 / (1 + e^(2 z / cap)))
+                const float ez = fast_exp2(z * p.inv_cap);
+                z = p.cap2 * (1.f - __fdividef(2.f, 1.f + ez));
+              }
+              x[u][nt][e] = z;
             }
-            if (masked && tok + nt * 8 + 2 * t4 + (e & 1) >= lim[e >> 1]) z = -INFINITY;
-            x[nt][e] = z;
+          if (masked) {
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (tok + u * 16 + nt * 8 + 2 * t4 + (e & 1) >= lim[e >> 1]) x[u][nt][e] = -INFINITY;
           }
-        if (p.scores && tok < p.score_ld) {
+          y0 = fmaxf(y0, lv[u] + fmaxf(fmaxf(x[u][0][0], x[u][0][1]), fmaxf(x[u][1][0], x[u][1][1])));
+          y1 = fmaxf(y1, lv[u] + fmaxf(fmaxf(x[u][0][2], x[u][0][3]), fmaxf(x[u][1][2], x[u][1][3])));
+          if (p.scores && tok + u * 16 < p.score_ld) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
-            if (row_id[half] >= 0) {
-              float* sp = p.scores + ((static_cast<int64_t>(s) * p.c.Hkv + kvh) * p.rows + row_id[half]) * p.score_ld + tok + 2 * t4;
-              *reinterpret_cast<float2*>(sp) = make_float2(x[0][2 * half], x[0][2 * half + 1]);
-              *reinterpret_cast<float2*>(sp + 8) = make_float2(x[1][2 * half], x[1][2 * half + 1]);
-            }
+            for (int half = 0; half < 2; ++half)
+              if (row_id[half] >= 0) {
+                float* sp = p.scores + ((static_cast<int64_t>(s) * p.c.Hkv + kvh) * p.rows + row_id[half]) * p.score_ld +
+                            tok + u * 16 + 2 * t4;
+                *reinterpret_cast<float2*>(sp) = make_float2(x[u][0][2 * half], x[u][0][2 * half + 1]);
+                *reinterpret_cast<float2*>(sp + 8) = make_float2(x[u][1][2 * half], x[u][1][2 * half + 1]);
+              }
+          }
         }
         // ---- running maximum: raised only when a score passes it by 2^kLag ----
-        float c0 = lv - (m[0] == -INFINITY ? 0.f : m[0]), c1 = lv - (m[1] == -INFINITY ? 0.f : m[1]);
-        const float y0 = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
-        const float y1 = fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3]));
-        const bool up = y0 + c0 > (m[0] == -INFINITY ? -INFINITY : kLag + kPBias) || y1 + c1 > (m[1] == -INFINITY ? -INFINITY : kLag + kPBias);
+        float mu0 = m[0] == -INFINITY ? 0.f : m[0], mu1 = m[1] == -INFINITY ? 0.f : m[1];
+        const bool up = y0 > m[0] + (kLag + kPBias) || y1 > m[1] + (kLag + kPBias);
         if (__any_sync(0xffffffffu, up)) {
-          float mx[2] = {y0 + (lv - kPBias), y1 + (lv - kPBias)}, al[2];
+          float mx[2] = {y0 - kPBias, y1 - kPBias}, al[2];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
@@ -449,8 +530,8 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
             m[r] = mn;
             l[r] *= al[r];
           }
-          c0 = lv - (m[0] == -INFINITY ? 0.f : m[0]);
-          c1 = lv - (m[1] == -INFINITY ? 0.f : m[1]);
+          mu0 = m[0] == -INFINITY ? 0.f : m[0];
+          mu1 = m[1] == -INFINITY ? 0.f : m[1];
 #pragma unroll
           for (int i = 0; i < DP / 8; ++i) {
             o[i][0] *= al[0];
@@ -459,39 +540,107 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
             o[i][3] *= al[1];
           }
         }
-        float ps[2] = {0.f, 0.f};
+        uint32_t pa[TP][4];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+        for (int u = 0; u < TP; ++u) {
+          const float c0 = lv[u] - mu0, c1 = lv[u] - mu1;
+          float ps[2] = {0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[nt][e] = fast_exp2(x[nt][e] + (e < 2 ? c0 : c1));
-            ps[e >> 1] += x[nt][e];
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[u][nt][e] = fast_exp2(x[u][nt][e] + (e < 2 ? c0 : c1));
+              ps[e >> 1] += x[u][nt][e];
+            }
+          l[0] = fmaf(ps[0], ivs[u], l[0]);
+          l[1] = fmaf(ps[1], ivs[u], l[1]);
+          pa[u][0] = Elem<__half>::pack2(x[u][0][0], x[u][0][1]);
+          pa[u][1] = Elem<__half>::pack2(x[u][0][2], x[u][0][3]);
+          pa[u][2] = Elem<__half>::pack2(x[u][1][0], x[u][1][1]);
+          pa[u][3] = Elem<__half>::pack2(x[u][1][2], x[u][1][3]);
+        }
+        // ---- weights below fp16's normal range (2^-27 of the largest; masked
+        // keys among them): they go through the product apart, times 2^24, so
+        // that a column in which the heavy keys have zeros keeps its precision ----
+        __half2 least = as_half2(pa[0][0]);
+#pragma unroll
+        for (int i = 1; i < 4 * TP; ++i) least = __hmin2(least, as_half2(pa[i >> 2][i & 3]));
+        const float2 least2 = __half22float2(least);
+        if (__any_sync(0xffffffffu, fminf(least2.x, least2.y) < kHalfMin)) {
+          uint32_t pb[TP][4];
+          bool some = false;
+#pragma unroll
+          for (int u = 0; u < TP; ++u) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // pa[.][i] holds keys of n tile i >> 1, row i & 1
+              float f[2], t[2];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float v = x[u][i >> 1][2 * (i & 1) + k];
+                const bool small = v < kHalfMin;
+                f[k] = small ? v * 16777216.f : 0.f;
+                t[k] = small ? 0.f : v;
+                some |= f[k] > 0.f;
+              }
+              pb[u][i] = Elem<__half>::pack2(f[0], f[1]);
+              pa[u][i] = Elem<__half>::pack2(t[0], t[1]);
+            }
           }
-        l[0] = fmaf(ps[0], ivs, l[0]);
-        l[1] = fmaf(ps[1], ivs, l[1]);
-        uint32_t pa[4];
-        pa[0] = Elem<__half>::pack2(x[0][0], x[0][1]);
-        pa[1] = Elem<__half>::pack2(x[0][2], x[0][3]);
-        pa[2] = Elem<__half>::pack2(x[1][0], x[1][1]);
-        pa[3] = Elem<__half>::pack2(x[1][2], x[1][3]);
-        if (v_bad) {  // a NaN or infinite V scale: NaN for the rows that see a key of the tile
-          pa[0] = pa[2] = tok < lim[0] ? 0x7fff7fffu : 0u;
-          pa[1] = pa[3] = tok < lim[1] ? 0x7fff7fffu : 0u;
+          if (__any_sync(0xffffffffu, some)) {
+#pragma unroll 1
+            for (int db = 0; db < DP / 32; ++db) {
+              const int piece = 2 * db + (mi >> 1);
+              float a[4][4];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) a[i >> 2][i & 3] = 0.f;
+#pragma unroll
+              for (int u = 0; u < TP; ++u) {
+                uint32_t r[4];
+                ldsm_x4_t(vbase + (piece >> 3) * CH * C::ROWB + kv8_sw<DP>(r0 + u * 16 + (mi & 1) * 8 + rr, piece & 7), r[0],
+                          r[1], r[2], r[3]);
+#pragma unroll
+                for (int x2 = 0; x2 < 2; ++x2) {
+                  uint32_t e0, o0, e1, o1;
+                  codes_to_half<CODE, 1>(r[2 * x2], e0, o0);
+                  codes_to_half<CODE, 1>(r[2 * x2 + 1], e1, o1);
+                  Mma<__half>::run(a[2 * x2], pb[u], e0, e1);
+                  Mma<__half>::run(a[2 * x2 + 1], pb[u], o0, o1);
+                }
+              }
+#pragma unroll
+              for (int d2 = 0; d2 < DP / 32; ++d2)  // o stays in registers: a constant index under a uniform test
+                if (d2 == db) {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) o[4 * d2 + (i >> 2)][i & 3] = fmaf(a[i >> 2][i & 3], 5.9604644775390625e-8f, o[4 * d2 + (i >> 2)][i & 3]);
+                }
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < TP; ++u) {
+          if (v_bad[u]) {  // a NaN or infinite V scale: NaN for the rows that see a key of the tile
+            pa[u][0] = pa[u][2] = tok + u * 16 < lim[0] ? 0x7fff7fffu : 0u;
+            pa[u][1] = pa[u][3] = tok + u * 16 < lim[1] ? 0x7fff7fffu : 0u;
+          }
         }
         // ---- O += P Vc: words transposed by the load pair two keys of columns
         // 2 g and 2 g + 1, so even and odd columns are two n tiles ----
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db) {
           const int piece = 2 * db + (mi >> 1);
-          uint32_t r[4];
-          ldsm_x4_t(vbase + (piece >> 3) * CH * C::ROWB + kv8_sw<DP>(r0 + (mi & 1) * 8 + rr, piece & 7), r[0], r[1], r[2], r[3]);
 #pragma unroll
-          for (int x2 = 0; x2 < 2; ++x2) {
-            uint32_t e0, o0, e1, o1;
-            codes_to_half<CODE, 1>(r[2 * x2], e0, o0);
-            codes_to_half<CODE, 1>(r[2 * x2 + 1], e1, o1);
-            Mma<__half>::run(o[4 * db + 2 * x2], pa, e0, e1);
-            Mma<__half>::run(o[4 * db + 2 * x2 + 1], pa, o0, o1);
+          for (int u = 0; u < TP; ++u) {
+            uint32_t r[4];
+            ldsm_x4_t(vbase + (piece >> 3) * CH * C::ROWB + kv8_sw<DP>(r0 + u * 16 + (mi & 1) * 8 + rr, piece & 7), r[0], r[1],
+                      r[2], r[3]);
+#pragma unroll
+            for (int x2 = 0; x2 < 2; ++x2) {
+              uint32_t e0, o0, e1, o1;
+              codes_to_half<CODE, 1>(r[2 * x2], e0, o0);
+              codes_to_half<CODE, 1>(r[2 * x2 + 1], e1, o1);
+              Mma<__half>::run(o[4 * db + 2 * x2], pa[u], e0, e1);
+              Mma<__half>::run(o[4 * db + 2 * x2 + 1], pa[u], o0, o1);
+            }
           }
         }
       }
@@ -568,8 +717,7 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
       }
     }
     // the next item
-    w.j = j_end - 1;
-    w.next(p, items);
+    w.next_item(p, items);
   }
 }
 
@@ -587,7 +735,7 @@ __global__ void __launch_bounds__(128) kv8_attention_join_kernel(const Kv8TcPara
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x + 1, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int4 b = p.bound[c];
-  if (b.z == 0) return;  // an item begins here, or the CTA had no chunk
+  if (b.z == 0) return;  // an item begins here, or the CTA has no chunk
   // parts: the CTA in which the item begins (slot 1), then the CTAs up to its
   // end (slot 0); those in between cover it without a gap
   if (warp == 0) {
@@ -781,6 +929,8 @@ static int launch_tc(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
   p.context_lens = a.context_lens;
   p.lse = a.lse;
   p.bf16 = a.dtype == kBF16;
+  p.q_vec = a.sq[3] == 1 && c.D % 4 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 7) == 0 &&
+            ((a.sq[0] | a.sq[1] | a.sq[2]) & 3) == 0;
   p.H = a.H; p.Lq = a.Lq; p.G = a.H / c.Hkv; p.rows = p.G * a.Lq;
   p.chunks = (p.rows + z.RT - 1) / z.RT;
   p.box_rows = c.P & -c.P;
