@@ -62,6 +62,7 @@ constexpr float kLag = 2.f;
 constexpr float kLBias = 10.f;
 constexpr float kLBiasInv = 1.1920928955078125e-7f;  // 2^-(kPBias + kLBias)
 constexpr float kHalfMin = 6.103515625e-5f;  // 2^-14: fp16's smallest normal number
+constexpr int kFew = 8;
 constexpr float kMinVs = 6.162975822039155e-33f;  // 2^-107: the smallest scale that the write makes
 
 template <int DP, int WM> struct Kv8Cfg {
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
       const bool real = row < p.rows;
       row_id[half] = real ? row : -1;
       const int i = real ? row / p.G : 0, hh = real ? row - i * p.G : 0;
-      lim[half] = real ? ctx - p.Lq + i + 1 : 0;
+      lim[half] = real ? ctx - p.Lq + i + 1 : ctx;  // rows that pad the tile see every key, so they never look masked
       const uint16_t* src = static_cast<const uint16_t*>(p.q) + s * p.sq[0] + i * p.sq[1] + (kvh * p.G + hh) * p.sq[2];
       auto to_float = [&](uint32_t raw) {
         return p.bf16 ? __uint_as_float(raw << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(raw)));
@@ -420,6 +421,8 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
 #pragma unroll
     for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    int above[2] = {0, 0};  // keys counted in fp16's normal range since the maximum last rose
+    bool many = false;      // every row of the warp has kFew of them
     const int open = ctx - p.Lq + 1;  // keys below it are seen by every row
 
     for (int j = j0; j < j_end; ++j, ++it) {
@@ -529,7 +532,9 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
             al[r] = fast_exp2(m[r] - mu);
             m[r] = mn;
             l[r] *= al[r];
+            above[r] = 0;
           }
+          many = false;
           mu0 = m[0] == -INFINITY ? 0.f : m[0];
           mu1 = m[1] == -INFINITY ? 0.f : m[1];
 #pragma unroll
@@ -559,14 +564,31 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
           pa[u][2] = Elem<__half>::pack2(x[u][1][0], x[u][1][1]);
           pa[u][3] = Elem<__half>::pack2(x[u][1][2], x[u][1][3]);
         }
-        // ---- weights below fp16's normal range (2^-27 of the largest; masked
-        // keys among them): they go through the product apart, times 2^24, so
-        // that a column in which the heavy keys have zeros keeps its precision ----
-        __half2 least = as_half2(pa[0][0]);
+        // ---- weights below fp16's normal range (2^-27 of the largest): while a row
+        // of the warp has fewer than kFew keys above it, they go through the
+        // product apart, times 2^24, so that a column in which those few keys have
+        // zeros keeps its precision.  Ordinary rows pass kFew in their first step ----
+        bool apart = false;
+        if (!many) {
+          float least = 1.f;
+          int n0 = 0, n1 = 0;
 #pragma unroll
-        for (int i = 1; i < 4 * TP; ++i) least = __hmin2(least, as_half2(pa[i >> 2][i & 3]));
-        const float2 least2 = __half22float2(least);
-        if (__any_sync(0xffffffffu, fminf(least2.x, least2.y) < kHalfMin)) {
+          for (int u = 0; u < TP; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float v = x[u][e >> 2][e & 3];
+              least = fminf(least, v);
+              if ((e & 3) < 2) n0 += v >= kHalfMin;
+              else n1 += v >= kHalfMin;
+            }
+          n0 += __shfl_xor_sync(0xffffffffu, n0, 1);
+          n1 += __shfl_xor_sync(0xffffffffu, n1, 1);
+          above[0] += n0 + __shfl_xor_sync(0xffffffffu, n0, 2);
+          above[1] += n1 + __shfl_xor_sync(0xffffffffu, n1, 2);
+          many = __all_sync(0xffffffffu, min(above[0], above[1]) >= kFew);
+          apart = !many && __any_sync(0xffffffffu, least < kHalfMin);
+        }
+        if (apart) {
           uint32_t pb[TP][4];
           bool some = false;
 #pragma unroll
