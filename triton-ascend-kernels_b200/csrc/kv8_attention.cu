@@ -74,19 +74,21 @@ template <int DP, int WM> struct Kv8Cfg {
   static constexpr int ROWB = DP >= 128 ? 128 : 64;     // bytes of a row in a column block
   static constexpr int PLANE = CH * DP;                 // bytes of K (or V) in a stage
   static constexpr int STAGE = 2 * PLANE;
-  static constexpr int NS = DP >= 256 ? 2 : DP == 128 ? 3 : 5;
-  static constexpr int DH = DP >= 256 ? 128 : DP == 128 ? 32 : 64; // columns merged at a time
+  // Q's fragments live in shared memory, [WM][DP / 16][32 lanes] of 16 bytes, and
+  // are loaded per use, where the registers they would take cost more: at 256
+  // columns (O alone takes 128) and at 128 (without them three CTAs fit an SM).
+  // The region is the joining buffer's: an item's Q is dead when its warps join.
+  static constexpr bool QSMEM = DP >= 256 || (DP == 128 && WM < 4);
+  static constexpr int CTAS = DP >= 256 ? 1 : DP == 128 && WM == 4 ? 2 : 3;  // per SM
+  static constexpr int NS = DP >= 256 ? 2 : DP == 128 ? (WM == 4 ? 3 : 2) : 4;
+  static constexpr int DH = DP >= 256 ? 128 : 32;       // columns joined at a time
   static constexpr int MERGE = NW * 16 * DH * 4;
+  static constexpr int QBYTES = QSMEM ? WM * (DP / 16) * 512 : 0;
   static constexpr int META_OFF = NS * STAGE;           // [NS][3][NT] floats: ks, log2 vs, 2^-23 / vs
   static constexpr int OBUF_OFF = META_OFF + NS * 3 * NT * 4;
-  static constexpr int ML_OFF = OBUF_OFF + MERGE;       // [NW][16][2]
-  // 256 columns of O take 128 registers a thread: Q's fragments then live in
-  // shared memory, [WM][DP / 16][32 lanes] of 16 bytes, and are loaded per use
-  static constexpr bool QSMEM = DP >= 256;
-  static constexpr int Q_OFF = ML_OFF + NW * 16 * 2 * 4;
-  static constexpr int BAR_OFF = Q_OFF + (QSMEM ? WM * (DP / 16) * 512 : 0);
+  static constexpr int ML_OFF = OBUF_OFF + (MERGE > QBYTES ? MERGE : QBYTES);  // [NW][16][2]
+  static constexpr int BAR_OFF = ML_OFF + NW * 16 * 2 * 4;
   static constexpr int SMEM = BAR_OFF + 2 * NS * 8 + 64 + 1024;
-  static constexpr int CTAS = DP >= 256 ? 1 : 2;        // per SM
   static_assert((SMEM + 1024) * CTAS <= 228 * 1024, "shared memory");
 };
 
@@ -129,11 +131,17 @@ __device__ __forceinline__ int kv8_ctx(const Kv8TcParams& p, int s) {
   return n > 0 ? static_cast<int>(n) : 0;
 }
 
+// query row `row` (token row / G, head kvh * G + row % G) of a KV head
+__device__ __forceinline__ const uint16_t* kv8_q_row(const Kv8TcParams& p, int s, int kvh, int row) {
+  const int i = row / p.G;
+  return static_cast<const uint16_t*>(p.q) + s * p.sq[0] + i * p.sq[1] + (kvh * p.G + row - i * p.G) * p.sq[2];
+}
+
 // Positions in the work list: an item of n chunks takes n + kItemCost places, the
 // last kItemCost of them empty.  They stand for what an item costs besides its
 // chunks (query rows, joining the warps, the output), so that CTAs with many
 // short items get fewer chunks.
-constexpr int kItemCost = 2;
+constexpr int kItemCost = 3;
 template <int CH> __device__ __forceinline__ int64_t kv8_places(int ctx) {
   return ctx > 0 ? (ctx + CH - 1) / CH + kItemCost : 0;
 }
@@ -299,6 +307,14 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
       if (more) {
         w.next(p, items);
         more2 = w.live(p, u1);
+        if (more2 && w.j == 0) {  // an item begins two chunks ahead: its query rows to L2
+          const int kvh = w.r / p.chunks, row0 = (w.r - kvh * p.chunks) * RT, lines = DP / 64;
+          for (int e = lane; e < RT * lines; e += 32) {
+            const int row = row0 + e / lines, d = e % lines * 64;
+            if (row < p.rows && d < p.c.D)
+              asm volatile("prefetch.global.L2 [%0];" ::"l"(kv8_q_row(p, w.s, kvh, row) + d * p.sq[3]));
+          }
+        }
       }
       Meta far = fetch_page(w, more2);
       fetch_scales(nxt);
@@ -350,24 +366,25 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
     // k order: thread t4 of a quad holds elements 4 t4 .. 4 t4 + 3 of each 16, the
     // order in which one 32-bit word of codes has them
     uint32_t qa[C::QSMEM ? 1 : DP / 16][4];
-    uint4* const qs = reinterpret_cast<uint4*>(smem + C::Q_OFF) + wm * (DP / 16) * 32 + lane;
+    uint4* const qs = reinterpret_cast<uint4*>(smem + C::OBUF_OFF) + wm * (DP / 16) * 32 + lane;
     float fac[2];
     int lim[2], row_id[2];
+    auto to_float = [&](uint32_t raw) {
+      return p.bf16 ? __uint_as_float(raw << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(raw)));
+    };
+    uint2 raw[2][DP / 16];  // four elements of each 16-element block, both rows' loads in flight at once
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int row = rc * RT + wm * 16 + g + half * 8;
       const bool real = row < p.rows;
       row_id[half] = real ? row : -1;
-      const int i = real ? row / p.G : 0, hh = real ? row - i * p.G : 0;
+      const int i = real ? row / p.G : 0;
       lim[half] = real ? ctx - p.Lq + i + 1 : ctx;  // rows that pad the tile see every key, so they never look masked
-      const uint16_t* src = static_cast<const uint16_t*>(p.q) + s * p.sq[0] + i * p.sq[1] + (kvh * p.G + hh) * p.sq[2];
-      auto to_float = [&](uint32_t raw) {
-        return p.bf16 ? __uint_as_float(raw << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(raw)));
-      };
-      // four elements of 16-element block b
-      auto four = [&](int b) {
-        uint2 v = make_uint2(0, 0);
+      const uint16_t* src = kv8_q_row(p, s, kvh, real ? row : 0);
+#pragma unroll
+      for (int b = 0; b < DP / 16; ++b) {
         const int d = b * 16 + 4 * t4;
+        uint2 v = make_uint2(0, 0);
         if (p.q_vec) {
           if (real && d < p.c.D) v = *reinterpret_cast<const uint2*>(src + d);
         } else {
@@ -376,15 +393,18 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
           for (int k = 0; k < 4; ++k) e[k] = real && d + k < p.c.D ? src[(d + k) * p.sq[3]] : 0;
           v = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
         }
-        return v;
-      };
-      uint2 raw[C::QSMEM ? 1 : DP / 16];
+        raw[half][b] = v;
+      }
+    }
+    // the last item's joining buffer has been read: Q may take its place
+    if (C::QSMEM) asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
       float top = 0.f;
       bool odd = false;
 #pragma unroll
       for (int b = 0; b < DP / 16; ++b) {
-        const uint2 v = four(b);
-        if (!C::QSMEM) raw[C::QSMEM ? 0 : b] = v;  // 256 columns are read again instead: held, they would cost the registers
+        const uint2 v = raw[half][b];
         const float f[4] = {to_float(v.x & 0xffff), to_float(v.x >> 16), to_float(v.y & 0xffff), to_float(v.y >> 16)};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -402,7 +422,7 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
       fac[half] = p.scale * __uint_as_float(static_cast<uint32_t>(127 - 8 + e2) << 23);
 #pragma unroll
       for (int b = 0; b < DP / 16; ++b) {
-        const uint2 v = C::QSMEM ? four(b) : raw[C::QSMEM ? 0 : b];
+        const uint2 v = raw[half][b];
         const uint32_t q01 = Elem<__half>::pack2(to_float(v.x & 0xffff) * up, to_float(v.x >> 16) * up);
         const uint32_t q23 = Elem<__half>::pack2(to_float(v.y & 0xffff) * up, to_float(v.y >> 16) * up);
         if (!C::QSMEM) {
@@ -414,7 +434,6 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
         }
       }
     }
-    // (the last item's readers are past its closing barriers)
     if (C::QSMEM) asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");
 
     float o[DP / 8][4];
@@ -455,7 +474,7 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
         for (int u = 0; u < TP; ++u)
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[u][e >> 2][e & 3] = 0.f;
-#pragma unroll(C::QSMEM ? 2 : DP / 32)
+#pragma unroll(DP >= 256 ? 2 : DP / 32)
         for (int kb = 0; kb < DP / 32; ++kb) {
           const int piece = 2 * kb + (mi & 1);
           uint32_t r[TP][4];
@@ -887,8 +906,9 @@ static int64_t up16(int64_t x) { return (x + 255) / 256 * 256; }
 static TcSizes tc_sizes(const Kv8View& c, const Kv8AttnArgs& a) {
   TcSizes z{};
   z.DP = tc_dp(c);
-  z.N = num_sms() * (z.DP >= 256 ? 1 : 2);
-  z.RT = 16 * tc_wm(c, a);
+  const int wm = tc_wm(c, a);
+  z.N = num_sms() * (z.DP >= 256 ? 1 : z.DP == 128 && wm == 4 ? 2 : 3);  // Kv8Cfg::CTAS
+  z.RT = 16 * wm;
   const int64_t rows = static_cast<int64_t>(a.H / c.Hkv) * a.Lq, all = rows * c.Hkv * c.num_seqs;
   int64_t at = 0;
   z.bound = at; at += up16(static_cast<int64_t>(z.N) * 16);
