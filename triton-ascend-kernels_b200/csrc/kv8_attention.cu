@@ -21,8 +21,8 @@
 //
 // A CTA: one producer warp streams chunks through a ring of TMA loads (K and V
 // codes, page ids from the block table) with the tiles' scales beside them; NW
-// warps consume: WM of them across the query rows (16 each), NW / WM across the
-// key tiles.
+// warps consume: WM of them across the query rows (8 or 16 each), NW / WM across
+// the key tiles.
 #include <cstdio>
 
 #include "kv8.cuh"
@@ -45,8 +45,8 @@ struct Kv8TcParams {
   float cap2, inv_cap;  // softcap * log2(e), 2 log2(e) / softcap; 0: no cap
   // workspace
   int4* bound;       // [N] first chunk of each CTA: {sequence, item of it, chunk of the item, chunks of the item}
-  float* part_o;     // [N][2][16 WM][DP]
-  float* part_ml;    // [N][2][16 WM][2]
+  float* part_o;     // [N][2][8 NR WM][DP]
+  float* part_ml;    // [N][2][8 NR WM][2]
   float* lse2;       // [B, Hkv, rows] (weights only)
   float* scores;     // [B, Hkv, rows, score_ld] (weights only)
   int64_t score_ld;
@@ -65,8 +65,11 @@ constexpr float kHalfMin = 6.103515625e-5f;  // 2^-14: fp16's smallest normal nu
 constexpr int kFew = 8;
 constexpr float kMinVs = 6.162975822039155e-33f;  // 2^-107: the smallest scale that the write makes
 
-template <int DP, int WM> struct Kv8Cfg {
+// DP: head dim rounded up to 64, 128 or 256.  A warp holds 8 NR query rows, WM
+// warps stand across the rows, the rest across the key tiles.
+template <int DP, int NR, int WM> struct Kv8Cfg {
   static constexpr int NW = DP >= 256 ? 8 : 4;          // consumer warps
+  static constexpr int RW = 8 * NR;                     // query rows of a warp
   static constexpr int CH = 128;                        // keys of a chunk
   static constexpr int TP = DP >= 256 ? 1 : 2;          // key tiles of a warp's step (two: independent MMA chains)
   static constexpr int NT = CH / 16;                    // key tiles of a chunk
@@ -74,20 +77,21 @@ template <int DP, int WM> struct Kv8Cfg {
   static constexpr int ROWB = DP >= 128 ? 128 : 64;     // bytes of a row in a column block
   static constexpr int PLANE = CH * DP;                 // bytes of K (or V) in a stage
   static constexpr int STAGE = 2 * PLANE;
-  // Q's fragments live in shared memory, [WM][DP / 16][32 lanes] of 16 bytes, and
-  // are loaded per use, where the registers they would take cost more: at 256
-  // columns (O alone takes 128) and at 128 (without them three CTAs fit an SM).
-  // The region is the joining buffer's: an item's Q is dead when its warps join.
-  static constexpr bool QSMEM = DP >= 256 || (DP == 128 && WM < 4);
+  // With 16 rows a warp Q's fragments live in shared memory ([WM][DP / 16][32
+  // lanes] of 16 bytes) and are loaded per use: in registers they would cost the
+  // third CTA of an SM.  The region is the joining buffer's: an item's Q is dead
+  // when its warps join.
+  static constexpr bool QSMEM = NR == 2 && DP == 128 && WM < 4;
   static constexpr int CTAS = DP >= 256 ? 1 : DP == 128 && WM == 4 ? 2 : 3;  // per SM
   static constexpr int NS = DP >= 256 ? 2 : DP == 128 ? (WM == 4 ? 3 : 2) : 4;
-  static constexpr int DH = DP >= 256 ? 128 : 32;       // columns joined at a time
-  static constexpr int MERGE = NW * 16 * DH * 4;
+  static constexpr int DH = NR == 2 && (WM < 4 || DP == 64) ? 16 : 32;  // columns joined at a time
+  static constexpr int OLD = DH + 8;                    // row stride of the joining buffer (bank spread)
+  static constexpr int MERGE = NW * RW * OLD * 4;
   static constexpr int QBYTES = QSMEM ? WM * (DP / 16) * 512 : 0;
-  static constexpr int META_OFF = NS * STAGE;           // [NS][3][NT] floats: ks, log2 vs, 2^-23 / vs
+  static constexpr int META_OFF = NS * STAGE;           // [NS][3][NT] floats: ks, log2 vs + kPBias, 2^-23 / vs
   static constexpr int OBUF_OFF = META_OFF + NS * 3 * NT * 4;
-  static constexpr int ML_OFF = OBUF_OFF + (MERGE > QBYTES ? MERGE : QBYTES);  // [NW][16][2]
-  static constexpr int BAR_OFF = ML_OFF + NW * 16 * 2 * 4;
+  static constexpr int ML_OFF = OBUF_OFF + (MERGE > QBYTES ? MERGE : QBYTES);  // [NW][RW][2]
+  static constexpr int BAR_OFF = ML_OFF + NW * RW * 2 * 4;
   static constexpr int SMEM = BAR_OFF + 2 * NS * 8 + 64 + 1024;
   static_assert((SMEM + 1024) * CTAS <= 228 * 1024, "shared memory");
 };
@@ -108,7 +112,12 @@ __device__ __forceinline__ uint32_t hsub2_1152(uint32_t x) {
   __half2 h = __hsub2(*reinterpret_cast<__half2*>(&x), k);
   return *reinterpret_cast<uint32_t*>(&h);
 }
-__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+// transpose of an 8 x 8 matrix of 16-bit elements held as the MMA fragments are
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
+}
 // Four codes to two fp16 pairs.  int8: the byte with its sign bit flipped goes
 // into the mantissa of 1024 (fp16 0x6400, where an ulp is 1): 1024 + 128 + x,
 // less 1152.  PAIR = 0 pairs bytes (0,1) (2,3), PAIR = 1 bytes (0,2) (1,3).
@@ -176,12 +185,12 @@ template <int CH> struct Kv8Walk {
   __device__ __forceinline__ bool live(const Kv8TcParams& p, int64_t end) const { return at < end && s < p.c.num_seqs; }
 };
 
-template <int CODE, int DP, int WM>
-__global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>::CTAS)
+template <int CODE, int DP, int NR, int WM>
+__global__ void __launch_bounds__((Kv8Cfg<DP, NR, WM>::NW + 1) * 32, Kv8Cfg<DP, NR, WM>::CTAS)
     kv8_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                             const __grid_constant__ Kv8TcParams p) {
-  using C = Kv8Cfg<DP, WM>;
-  constexpr int NW = C::NW, CH = C::CH, NT = C::NT, TP = C::TP, NS = C::NS, WK = NW / WM, RT = 16 * WM;
+  using C = Kv8Cfg<DP, NR, WM>;
+  constexpr int NW = C::NW, CH = C::CH, NT = C::NT, TP = C::TP, NS = C::NS, WK = NW / WM, RW = C::RW, RT = RW * WM;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* meta = reinterpret_cast<float*>(smem + C::META_OFF);
@@ -362,24 +371,20 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
     const int j0 = w.j, j_end = static_cast<int>(min(static_cast<int64_t>(w.n), w.j + (u1 - w.at))), s = w.s, ctx = w.ctx;
     const int kvh = w.r / p.chunks, rc = w.r - kvh * p.chunks;
 
-    // ---- query rows to fp16 A fragments, each row scaled by a power of two ----
-    // k order: thread t4 of a quad holds elements 4 t4 .. 4 t4 + 3 of each 16, the
-    // order in which one 32-bit word of codes has them
-    uint32_t qa[C::QSMEM ? 1 : DP / 16][4];
+    // ---- query rows to fp16 B fragments, each row scaled by a power of two ----
+    // The keys are the M side of both products (S^T = Kc Q^T, O^T = Vc^T P^T), so
+    // eight query rows fill an MMA.  k order: thread t4 of a quad holds elements
+    // 4 t4 .. 4 t4 + 3 of each 16, the order in which a 32-bit word of codes has them.
+    uint32_t qb[C::QSMEM ? 1 : NR * DP / 16][2];
     uint4* const qs = reinterpret_cast<uint4*>(smem + C::OBUF_OFF) + wm * (DP / 16) * 32 + lane;
-    float fac[2];
-    int lim[2], row_id[2];
     auto to_float = [&](uint32_t raw) {
       return p.bf16 ? __uint_as_float(raw << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(raw)));
     };
-    uint2 raw[2][DP / 16];  // four elements of each 16-element block, both rows' loads in flight at once
+    uint2 raw[NR][DP / 16];  // all loads in flight at once
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int row = rc * RT + wm * 16 + g + half * 8;
+    for (int nr = 0; nr < NR; ++nr) {
+      const int row = rc * RT + wm * RW + nr * 8 + g;
       const bool real = row < p.rows;
-      row_id[half] = real ? row : -1;
-      const int i = real ? row / p.G : 0;
-      lim[half] = real ? ctx - p.Lq + i + 1 : ctx;  // rows that pad the tile see every key, so they never look masked
       const uint16_t* src = kv8_q_row(p, s, kvh, real ? row : 0);
 #pragma unroll
       for (int b = 0; b < DP / 16; ++b) {
@@ -393,18 +398,28 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
           for (int k = 0; k < 4; ++k) e[k] = real && d + k < p.c.D ? src[(d + k) * p.sq[3]] : 0;
           v = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
         }
-        raw[half][b] = v;
+        raw[nr][b] = v;
       }
     }
+    // scores come out with this thread's rows 2 t4 and 2 t4 + 1 (of each eight)
+    float fac[NR][2];
+    int lim[NR][2];  // keys that a row sees
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int row = rc * RT + wm * RW + nr * 8 + 2 * t4 + k;
+        lim[nr][k] = row < p.rows ? ctx - p.Lq + row / p.G + 1 : ctx;  // rows that pad the tile see every key
+      }
     // the last item's joining buffer has been read: Q may take its place
     if (C::QSMEM) asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int nr = 0; nr < NR; ++nr) {
       float top = 0.f;
       bool odd = false;
 #pragma unroll
       for (int b = 0; b < DP / 16; ++b) {
-        const uint2 v = raw[half][b];
+        const uint2 v = raw[nr][b];
         const float f[4] = {to_float(v.x & 0xffff), to_float(v.x >> 16), to_float(v.y & 0xffff), to_float(v.y >> 16)};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -419,29 +434,39 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
       // 2^e <= top < 2^(e+1); the row's largest comes to [2^8, 2^9)
       const int e2 = odd || top == 0.f ? 8 : max(-110, static_cast<int>(__float_as_uint(top) >> 23) - 127);
       const float up = __uint_as_float(static_cast<uint32_t>(127 + 8 - e2) << 23);
-      fac[half] = p.scale * __uint_as_float(static_cast<uint32_t>(127 - 8 + e2) << 23);
+      const float f = p.scale * __uint_as_float(static_cast<uint32_t>(127 - 8 + e2) << 23);
+      fac[nr][0] = __shfl_sync(0xffffffffu, f, 8 * t4);
+      fac[nr][1] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
 #pragma unroll
       for (int b = 0; b < DP / 16; ++b) {
-        const uint2 v = raw[half][b];
+        const uint2 v = raw[nr][b];
         const uint32_t q01 = Elem<__half>::pack2(to_float(v.x & 0xffff) * up, to_float(v.x >> 16) * up);
         const uint32_t q23 = Elem<__half>::pack2(to_float(v.y & 0xffff) * up, to_float(v.y >> 16) * up);
         if (!C::QSMEM) {
-          qa[C::QSMEM ? 0 : b][half] = q01;
-          qa[C::QSMEM ? 0 : b][half + 2] = q23;
+          qb[C::QSMEM ? 0 : nr * (DP / 16) + b][0] = q01;
+          qb[C::QSMEM ? 0 : nr * (DP / 16) + b][1] = q23;
         } else if (wk == 0) {
-          reinterpret_cast<uint32_t*>(qs + b * 32)[half] = q01;
-          reinterpret_cast<uint32_t*>(qs + b * 32)[half + 2] = q23;
+          reinterpret_cast<uint2*>(qs + b * 32)[nr] = make_uint2(q01, q23);
         }
       }
     }
     if (C::QSMEM) asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");
 
-    float o[DP / 8][4];
+    float o[NR][DP / 16][4];  // (column 2 g, 2 g + 1 of each 16) x (row 2 t4, 2 t4 + 1): c0 c1 / c2 c3
+    float m[NR][2], l[NR][2];
+    int above[NR][2];   // keys counted in fp16's normal range since the maximum last rose
+    bool many = false;  // every row of the warp has kFew of them
 #pragma unroll
-    for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    int above[2] = {0, 0};  // keys counted in fp16's normal range since the maximum last rose
-    bool many = false;      // every row of the warp has kFew of them
+    for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) o[nr][i][0] = o[nr][i][1] = o[nr][i][2] = o[nr][i][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        m[nr][k] = -INFINITY;
+        l[nr][k] = 0.f;
+        above[nr][k] = 0;
+      }
+    }
     const int open = ctx - p.Lq + 1;  // keys below it are seen by every row
 
     for (int j = j0; j < j_end; ++j, ++it) {
@@ -468,121 +493,124 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
           fence_proxy_async_smem();
           __syncwarp();
         }
-        // ---- S = Q Kc^T for TP tiles of 16 keys ----
-        float x[TP][2][4];
+        // ---- S^T = Kc Q^T for TP tiles of 16 keys ----
+        float x[TP][NR][4];  // c0 c1: key g, rows 2 t4, 2 t4 + 1; c2 c3: key g + 8
 #pragma unroll
         for (int u = 0; u < TP; ++u)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[u][e >> 2][e & 3] = 0.f;
-#pragma unroll(DP >= 256 ? 2 : DP / 32)
+          for (int nr = 0; nr < NR; ++nr) x[u][nr][0] = x[u][nr][1] = x[u][nr][2] = x[u][nr][3] = 0.f;
+#pragma unroll
         for (int kb = 0; kb < DP / 32; ++kb) {
-          const int piece = 2 * kb + (mi & 1);
+          const int piece = 2 * kb + (mi >> 1);
           uint32_t r[TP][4];
 #pragma unroll
           for (int u = 0; u < TP; ++u)
-            ldsm_x4(kbase + (piece >> 3) * CH * C::ROWB + kv8_sw<DP>(r0 + u * 16 + (mi >> 1) * 8 + rr, piece & 7), r[u][0],
+            ldsm_x4(kbase + (piece >> 3) * CH * C::ROWB + kv8_sw<DP>(r0 + u * 16 + (mi & 1) * 8 + rr, piece & 7), r[u][0],
                     r[u][1], r[u][2], r[u][3]);
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {  // k16 step; r[.][k]: the first eight keys, r[.][k + 2]: the others
-            uint32_t b0, b1, qf[4];
+          for (int k = 0; k < 2; ++k) {  // k16 step; r[.][2 k]: the first eight keys, r[.][2 k + 1]: the others
+            uint32_t qf[4];
             if (C::QSMEM) *reinterpret_cast<uint4*>(qf) = qs[(2 * kb + k) * 32];
-            const uint32_t* q4 = C::QSMEM ? qf : qa[C::QSMEM ? 0 : 2 * kb + k];
 #pragma unroll
             for (int u = 0; u < TP; ++u) {
-              codes_to_half<CODE, 0>(r[u][k], b0, b1);
-              Mma<__half>::run(x[u][0], q4, b0, b1);
-              codes_to_half<CODE, 0>(r[u][k + 2], b0, b1);
-              Mma<__half>::run(x[u][1], q4, b0, b1);
+              uint32_t af[4];
+              codes_to_half<CODE, 0>(r[u][2 * k], af[0], af[2]);
+              codes_to_half<CODE, 0>(r[u][2 * k + 1], af[1], af[3]);
+#pragma unroll
+              for (int nr = 0; nr < NR; ++nr) {
+                const uint32_t* q2 = C::QSMEM ? qf + 2 * nr : qb[C::QSMEM ? 0 : nr * (DP / 16) + 2 * kb + k];
+                Mma<__half>::run(x[u][nr], af, q2[0], q2[1]);
+              }
             }
           }
         }
         // ---- scores, base 2 ----
         const bool masked = tok + 16 * TP > open;
-        float lv[TP], ivs[TP], y0 = -INFINITY, y1 = -INFINITY;  // y: largest score + log2 vs + kPBias
+        float lv[TP], ivs[TP], y[NR][2];  // y: largest score + log2 vs + kPBias
         bool v_bad[TP];
 #pragma unroll
+        for (int nr = 0; nr < NR; ++nr) y[nr][0] = y[nr][1] = -INFINITY;
+#pragma unroll
         for (int u = 0; u < TP; ++u) {
-          const float ks = mt[t + u], lvt = mt[NT + t + u], f0 = fac[0] * ks, f1 = fac[1] * ks;
+          const float ks = mt[t + u], lvt = mt[NT + t + u];
           ivs[u] = mt[2 * NT + t + u];
           v_bad[u] = lvt != lvt;
           lv[u] = v_bad[u] ? kPBias : lvt;
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
+          for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              float z = x[u][nt][e] * (e < 2 ? f0 : f1);
+              float z = x[u][nr][e] * (fac[nr][e & 1] * ks);
               if (p.inv_cap > 0.f) {
                 // cap * tanh(z / cap) = cap * (1 - 2 / (1 + e^(2 z / cap)))
                 const float ez = fast_exp2(z * p.inv_cap);
                 z = p.cap2 * (1.f - __fdividef(2.f, 1.f + ez));
               }
-              x[u][nt][e] = z;
+              if (masked && tok + u * 16 + g + (e & 2) * 4 >= lim[nr][e & 1]) z = -INFINITY;
+              x[u][nr][e] = z;
             }
-          if (masked) {
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (tok + u * 16 + nt * 8 + 2 * t4 + (e & 1) >= lim[e >> 1]) x[u][nt][e] = -INFINITY;
+            for (int k = 0; k < 2; ++k) y[nr][k] = fmaxf(y[nr][k], lv[u] + fmaxf(x[u][nr][k], x[u][nr][k + 2]));
           }
-          y0 = fmaxf(y0, lv[u] + fmaxf(fmaxf(x[u][0][0], x[u][0][1]), fmaxf(x[u][1][0], x[u][1][1])));
-          y1 = fmaxf(y1, lv[u] + fmaxf(fmaxf(x[u][0][2], x[u][0][3]), fmaxf(x[u][1][2], x[u][1][3])));
           if (p.scores && tok + u * 16 < p.score_ld) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
-              if (row_id[half] >= 0) {
-                float* sp = p.scores + ((static_cast<int64_t>(s) * p.c.Hkv + kvh) * p.rows + row_id[half]) * p.score_ld +
-                            tok + u * 16 + 2 * t4;
-                *reinterpret_cast<float2*>(sp) = make_float2(x[u][0][2 * half], x[u][0][2 * half + 1]);
-                *reinterpret_cast<float2*>(sp + 8) = make_float2(x[u][1][2 * half], x[u][1][2 * half + 1]);
+            for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const int row = rc * RT + wm * RW + nr * 8 + 2 * t4 + k;
+                if (row < p.rows) {
+                  float* sp = p.scores + ((static_cast<int64_t>(s) * p.c.Hkv + kvh) * p.rows + row) * p.score_ld + tok + u * 16 + g;
+                  sp[0] = x[u][nr][k];
+                  sp[8] = x[u][nr][k + 2];
+                }
               }
           }
         }
         // ---- running maximum: raised only when a score passes it by 2^kLag ----
-        float mu0 = m[0] == -INFINITY ? 0.f : m[0], mu1 = m[1] == -INFINITY ? 0.f : m[1];
-        const bool up = y0 > m[0] + (kLag + kPBias) || y1 > m[1] + (kLag + kPBias);
-        if (__any_sync(0xffffffffu, up)) {
-          float mx[2] = {y0 - kPBias, y1 - kPBias}, al[2];
+        bool up = false;
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-            mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-            const float mn = fmaxf(m[r], mx[r]), mu = mn == -INFINITY ? 0.f : mn;
-            al[r] = fast_exp2(m[r] - mu);
-            m[r] = mn;
-            l[r] *= al[r];
-            above[r] = 0;
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) up |= y[nr][k] > m[nr][k] + (kLag + kPBias);
+        if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr) {
+            float al[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              float mx = y[nr][k] - kPBias;
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              const float mn = fmaxf(m[nr][k], mx), mu = mn == -INFINITY ? 0.f : mn;
+              al[k] = fast_exp2(m[nr][k] - mu);
+              m[nr][k] = mn;
+              l[nr][k] *= al[k];
+              above[nr][k] = 0;
+            }
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+              o[nr][i][0] *= al[0];
+              o[nr][i][1] *= al[1];
+              o[nr][i][2] *= al[0];
+              o[nr][i][3] *= al[1];
+            }
           }
           many = false;
-          mu0 = m[0] == -INFINITY ? 0.f : m[0];
-          mu1 = m[1] == -INFINITY ? 0.f : m[1];
-#pragma unroll
-          for (int i = 0; i < DP / 8; ++i) {
-            o[i][0] *= al[0];
-            o[i][1] *= al[0];
-            o[i][2] *= al[1];
-            o[i][3] *= al[1];
-          }
         }
-        uint32_t pa[TP][4];
+        uint32_t pb[TP][NR][2];  // P^T fragments
 #pragma unroll
-        for (int u = 0; u < TP; ++u) {
-          const float c0 = lv[u] - mu0, c1 = lv[u] - mu1;
-          float ps[2] = {0.f, 0.f};
+        for (int u = 0; u < TP; ++u)
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
+          for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x[u][nt][e] = fast_exp2(x[u][nt][e] + (e < 2 ? c0 : c1));
-              ps[e >> 1] += x[u][nt][e];
+            for (int k = 0; k < 2; ++k) {
+              const float c0 = lv[u] - (m[nr][k] == -INFINITY ? 0.f : m[nr][k]);
+              x[u][nr][k] = fast_exp2(x[u][nr][k] + c0);
+              x[u][nr][k + 2] = fast_exp2(x[u][nr][k + 2] + c0);
+              l[nr][k] = fmaf(x[u][nr][k] + x[u][nr][k + 2], ivs[u], l[nr][k]);
             }
-          l[0] = fmaf(ps[0], ivs[u], l[0]);
-          l[1] = fmaf(ps[1], ivs[u], l[1]);
-          pa[u][0] = Elem<__half>::pack2(x[u][0][0], x[u][0][1]);
-          pa[u][1] = Elem<__half>::pack2(x[u][0][2], x[u][0][3]);
-          pa[u][2] = Elem<__half>::pack2(x[u][1][0], x[u][1][1]);
-          pa[u][3] = Elem<__half>::pack2(x[u][1][2], x[u][1][3]);
-        }
+          }
         // ---- weights below fp16's normal range (2^-27 of the largest): while a row
         // of the warp has fewer than kFew keys above it, they go through the
         // product apart, times 2^24, so that a column in which those few keys have
@@ -590,82 +618,82 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
         bool apart = false;
         if (!many) {
           float least = 1.f;
-          int n0 = 0, n1 = 0;
+          int fewest = kFew;
 #pragma unroll
-          for (int u = 0; u < TP; ++u)
+          for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float v = x[u][e >> 2][e & 3];
-              least = fminf(least, v);
-              if ((e & 3) < 2) n0 += v >= kHalfMin;
-              else n1 += v >= kHalfMin;
+            for (int k = 0; k < 2; ++k) {
+              int n = 0;
+#pragma unroll
+              for (int u = 0; u < TP; ++u)
+#pragma unroll
+                for (int e = k; e < 4; e += 2) {
+                  least = fminf(least, x[u][nr][e]);
+                  n += x[u][nr][e] >= kHalfMin;
+                }
+              n += __shfl_xor_sync(0xffffffffu, n, 4);
+              n += __shfl_xor_sync(0xffffffffu, n, 8);
+              n += __shfl_xor_sync(0xffffffffu, n, 16);
+              above[nr][k] += n;
+              fewest = min(fewest, above[nr][k]);
             }
-          n0 += __shfl_xor_sync(0xffffffffu, n0, 1);
-          n1 += __shfl_xor_sync(0xffffffffu, n1, 1);
-          above[0] += n0 + __shfl_xor_sync(0xffffffffu, n0, 2);
-          above[1] += n1 + __shfl_xor_sync(0xffffffffu, n1, 2);
-          many = __all_sync(0xffffffffu, min(above[0], above[1]) >= kFew);
+          many = __all_sync(0xffffffffu, fewest >= kFew);
           apart = !many && __any_sync(0xffffffffu, least < kHalfMin);
         }
         if (apart) {
-          uint32_t pb[TP][4];
+          uint32_t pc[TP][NR][2];
           bool some = false;
 #pragma unroll
-          for (int u = 0; u < TP; ++u) {
+          for (int u = 0; u < TP; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {  // pa[.][i] holds keys of n tile i >> 1, row i & 1
-              float f[2], t[2];
+            for (int nr = 0; nr < NR; ++nr) {
+              float f[4];
 #pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const float v = x[u][i >> 1][2 * (i & 1) + k];
+              for (int e = 0; e < 4; ++e) {
+                const float v = x[u][nr][e];
                 const bool small = v < kHalfMin;
-                f[k] = small ? v * 16777216.f : 0.f;
-                t[k] = small ? 0.f : v;
-                some |= f[k] > 0.f;
+                f[e] = small ? v * 16777216.f : 0.f;
+                x[u][nr][e] = small ? 0.f : v;
+                some |= f[e] > 0.f;
               }
-              pb[u][i] = Elem<__half>::pack2(f[0], f[1]);
-              pa[u][i] = Elem<__half>::pack2(t[0], t[1]);
+              pc[u][nr][0] = transpose8x8(Elem<__half>::pack2(f[0], f[1]));
+              pc[u][nr][1] = transpose8x8(Elem<__half>::pack2(f[2], f[3]));
             }
-          }
           if (__any_sync(0xffffffffu, some)) {
-#pragma unroll 1
-            for (int db = 0; db < DP / 32; ++db) {
-              const int piece = 2 * db + (mi >> 1);
-              float a[4][4];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) a[i >> 2][i & 3] = 0.f;
+            for (int db = 0; db < DP / 16; ++db) {
+              float a[NR][4];
+#pragma unroll
+              for (int nr = 0; nr < NR; ++nr) a[nr][0] = a[nr][1] = a[nr][2] = a[nr][3] = 0.f;
 #pragma unroll
               for (int u = 0; u < TP; ++u) {
-                uint32_t r[4];
-                ldsm_x4_t(vbase + (piece >> 3) * CH * C::ROWB + kv8_sw<DP>(r0 + u * 16 + (mi & 1) * 8 + rr, piece & 7), r[0],
-                          r[1], r[2], r[3]);
+                uint32_t r[2], af[4];
+                ldsm_x2_t(vbase + (db >> 3) * CH * C::ROWB + kv8_sw<DP>(r0 + u * 16 + (mi & 1) * 8 + rr, db & 7), r[0], r[1]);
+                codes_to_half<CODE, 1>(r[0], af[0], af[1]);
+                codes_to_half<CODE, 1>(r[1], af[2], af[3]);
 #pragma unroll
-                for (int x2 = 0; x2 < 2; ++x2) {
-                  uint32_t e0, o0, e1, o1;
-                  codes_to_half<CODE, 1>(r[2 * x2], e0, o0);
-                  codes_to_half<CODE, 1>(r[2 * x2 + 1], e1, o1);
-                  Mma<__half>::run(a[2 * x2], pb[u], e0, e1);
-                  Mma<__half>::run(a[2 * x2 + 1], pb[u], o0, o1);
-                }
+                for (int nr = 0; nr < NR; ++nr) Mma<__half>::run(a[nr], af, pc[u][nr][0], pc[u][nr][1]);
               }
 #pragma unroll
-              for (int d2 = 0; d2 < DP / 32; ++d2)  // o stays in registers: a constant index under a uniform test
-                if (d2 == db) {
+              for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) o[4 * d2 + (i >> 2)][i & 3] = fmaf(a[i >> 2][i & 3], 5.9604644775390625e-8f, o[4 * d2 + (i >> 2)][i & 3]);
-                }
+                for (int e = 0; e < 4; ++e) o[nr][db][e] = fmaf(a[nr][e], 5.9604644775390625e-8f, o[nr][db][e]);
             }
           }
         }
 #pragma unroll
-        for (int u = 0; u < TP; ++u) {
-          if (v_bad[u]) {  // a NaN or infinite V scale: NaN for the rows that see a key of the tile
-            pa[u][0] = pa[u][2] = tok + u * 16 < lim[0] ? 0x7fff7fffu : 0u;
-            pa[u][1] = pa[u][3] = tok + u * 16 < lim[1] ? 0x7fff7fffu : 0u;
+        for (int u = 0; u < TP; ++u)
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr) {
+            if (v_bad[u]) {  // a NaN or infinite V scale: NaN for the rows that see a key of the tile
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[u][nr][e] = tok + u * 16 < lim[nr][e & 1] ? __uint_as_float(0x7fffffffu) : 0.f;
+            }
+            pb[u][nr][0] = transpose8x8(Elem<__half>::pack2(x[u][nr][0], x[u][nr][1]));
+            pb[u][nr][1] = transpose8x8(Elem<__half>::pack2(x[u][nr][2], x[u][nr][3]));
           }
-        }
-        // ---- O += P Vc: words transposed by the load pair two keys of columns
-        // 2 g and 2 g + 1, so even and odd columns are two n tiles ----
+        // ---- O^T += Vc^T P^T: words transposed by the load pair two keys of columns
+        // 2 g and 2 g + 1, which become rows g and g + 8 of the MMA ----
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db) {
           const int piece = 2 * db + (mi >> 1);
@@ -675,12 +703,12 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
             ldsm_x4_t(vbase + (piece >> 3) * CH * C::ROWB + kv8_sw<DP>(r0 + u * 16 + (mi & 1) * 8 + rr, piece & 7), r[0], r[1],
                       r[2], r[3]);
 #pragma unroll
-            for (int x2 = 0; x2 < 2; ++x2) {
-              uint32_t e0, o0, e1, o1;
-              codes_to_half<CODE, 1>(r[2 * x2], e0, o0);
-              codes_to_half<CODE, 1>(r[2 * x2 + 1], e1, o1);
-              Mma<__half>::run(o[4 * db + 2 * x2], pa[u], e0, e1);
-              Mma<__half>::run(o[4 * db + 2 * x2 + 1], pa[u], o0, o1);
+            for (int k = 0; k < 2; ++k) {
+              uint32_t af[4];
+              codes_to_half<CODE, 1>(r[2 * k], af[0], af[1]);
+              codes_to_half<CODE, 1>(r[2 * k + 1], af[2], af[3]);
+#pragma unroll
+              for (int nr = 0; nr < NR; ++nr) Mma<__half>::run(o[nr][2 * db + k], af, pb[u][nr][0], pb[u][nr][1]);
             }
           }
         }
@@ -691,46 +719,52 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
 
     // ---- join the warps that shared the rows, then finish or store a part ----
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    }
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        l[nr][k] += __shfl_xor_sync(0xffffffffu, l[nr][k], 4);
+        l[nr][k] += __shfl_xor_sync(0xffffffffu, l[nr][k], 8);
+        l[nr][k] += __shfl_xor_sync(0xffffffffu, l[nr][k], 16);
+      }
     const bool whole = j0 == 0 && j_end == w.n;
     const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (j0 == 0 ? 1 : 0)) * RT;
 #pragma unroll
     for (int dh = 0; dh < DP / C::DH; ++dh) {
       asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");  // the buffer is free again
 #pragma unroll
-      for (int i = 0; i < C::DH / 16; ++i) {
-        const float(*ot)[4] = &o[dh * (C::DH / 8) + 2 * i];
-        float* dst = obuf + (warp * 16 + g) * C::DH + i * 16 + 4 * t4;
-        *reinterpret_cast<float4*>(dst) = make_float4(ot[0][0], ot[1][0], ot[0][1], ot[1][1]);
-        *reinterpret_cast<float4*>(dst + 8 * C::DH) = make_float4(ot[0][2], ot[1][2], ot[0][3], ot[1][3]);
-      }
-      if (dh == 0 && t4 == 0) {
-        mlbuf[(warp * 16 + g) * 2] = m[0];
-        mlbuf[(warp * 16 + g) * 2 + 1] = l[0];
-        mlbuf[(warp * 16 + g + 8) * 2] = m[1];
-        mlbuf[(warp * 16 + g + 8) * 2 + 1] = l[1];
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int i = 0; i < C::DH / 16; ++i) {
+          const float* ot = o[nr][dh * (C::DH / 16) + i];
+          float* dst = obuf + (warp * RW + nr * 8 + 2 * t4) * C::OLD + i * 16 + 2 * g;
+          *reinterpret_cast<float2*>(dst) = make_float2(ot[0], ot[2]);
+          *reinterpret_cast<float2*>(dst + C::OLD) = make_float2(ot[1], ot[3]);
+        }
+      if (dh == 0 && g == 0) {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            *reinterpret_cast<float2*>(mlbuf + (warp * RW + nr * 8 + 2 * t4 + k) * 2) = make_float2(m[nr][k], l[nr][k]);
       }
       asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");
       for (int e = tid; e < RT * (C::DH / 4); e += NW * 32) {
         const int row = e / (C::DH / 4), d = (e - row * (C::DH / 4)) * 4;
         const int grow = rc * RT + row;
         if (grow >= p.rows) continue;
-        const int tile = row >> 4, r16 = row & 15;
+        const int tile = row / RW, rw = row % RW;
         float M = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < WK; ++k) M = fmaxf(M, mlbuf[((k * WM + tile) * 16 + r16) * 2]);
+        for (int k = 0; k < WK; ++k) M = fmaxf(M, mlbuf[((k * WM + tile) * RW + rw) * 2]);
         const float Mu = M == -INFINITY ? 0.f : M;
         float L = 0.f;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < WK; ++k) {
-          const int at = (k * WM + tile) * 16 + r16;
+          const int at = (k * WM + tile) * RW + rw;
           const float f = fast_exp2(mlbuf[at * 2] - Mu);
           L = fmaf(mlbuf[at * 2 + 1], f, L);
-          const float4 v = *reinterpret_cast<const float4*>(obuf + at * C::DH + d);
+          const float4 v = *reinterpret_cast<const float4*>(obuf + at * C::OLD + d);
           a.x = fmaf(v.x, f, a.x);
           a.y = fmaf(v.y, f, a.y);
           a.z = fmaf(v.z, f, a.z);
@@ -896,19 +930,23 @@ static bool tc_ok(const Kv8View& c, const Kv8AttnArgs& a) {
   return true;
 }
 static int tc_dp(const Kv8View& c) { return c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256; }
-// query rows a CTA holds: 16 per warp row, as many warp rows as the rows fill
-static int tc_wm(const Kv8View& c, const Kv8AttnArgs& a) {
+// Rows of a warp (8 NR) and warps across the rows (WM): as many as the query rows
+// of a KV head fill, up to 64.  At 256 columns O allows eight rows a warp.
+struct TcRows { int nr, wm; };
+static TcRows tc_rows(const Kv8View& c, const Kv8AttnArgs& a) {
   const int64_t rows = static_cast<int64_t>(a.H / c.Hkv) * a.Lq;
-  return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  if (rows <= 8) return {1, 1};
+  if (tc_dp(c) == 256) return {1, rows <= 16 ? 2 : rows <= 32 ? 4 : 8};
+  return {2, rows <= 16 ? 1 : rows <= 32 ? 2 : 4};
 }
 struct TcSizes { int N, RT, DP; int64_t bound, ml, o, lse2, scores, total, score_ld; };
 static int64_t up16(int64_t x) { return (x + 255) / 256 * 256; }
 static TcSizes tc_sizes(const Kv8View& c, const Kv8AttnArgs& a) {
   TcSizes z{};
   z.DP = tc_dp(c);
-  const int wm = tc_wm(c, a);
-  z.N = num_sms() * (z.DP >= 256 ? 1 : z.DP == 128 && wm == 4 ? 2 : 3);  // Kv8Cfg::CTAS
-  z.RT = 16 * wm;
+  const TcRows r = tc_rows(c, a);
+  z.N = num_sms() * (z.DP >= 256 ? 1 : z.DP == 128 && r.wm == 4 ? 2 : 3);  // Kv8Cfg::CTAS
+  z.RT = 8 * r.nr * r.wm;
   const int64_t rows = static_cast<int64_t>(a.H / c.Hkv) * a.Lq, all = rows * c.Hkv * c.num_seqs;
   int64_t at = 0;
   z.bound = at; at += up16(static_cast<int64_t>(z.N) * 16);
@@ -959,9 +997,9 @@ static int launch_dependent(K kern, dim3 grid, int threads, cudaStream_t st, A..
   return set_error(3, buf);
 }
 
-template <int CODE, int DP, int WM>
+template <int CODE, int DP, int NR, int WM>
 static int launch_tc(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
-  using C = Kv8Cfg<DP, WM>;
+  using C = Kv8Cfg<DP, NR, WM>;
   const TcSizes z = tc_sizes(c, a);
   Kv8TcParams p{};
   p.c = c;
@@ -992,7 +1030,7 @@ static int launch_tc(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
   CUtensorMap mk, mv;
   if (const int r = encode_codes(&mk, c, 0, C::ROWB, p.box_rows)) return r;
   if (const int r = encode_codes(&mv, c, 1, C::ROWB, p.box_rows)) return r;
-  auto kern = kv8_attention_tc_kernel<CODE, DP, WM>;
+  auto kern = kv8_attention_tc_kernel<CODE, DP, NR, WM>;
   if (const int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::SMEM)) return r;
   kern<<<z.N, (C::NW + 1) * 32, C::SMEM, st>>>(mk, mv, p);
   note_kernel("kv8_attention_tc");
@@ -1006,11 +1044,17 @@ static int launch_tc(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
 }
 
 template <int CODE, int DP>
-static int launch_wm(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
-  switch (tc_wm(c, a)) {
-    case 1: return launch_tc<CODE, DP, 1>(c, a, st);
-    case 2: return launch_tc<CODE, DP, 2>(c, a, st);
-    default: return launch_tc<CODE, DP, 4>(c, a, st);
+static int launch_rows(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
+  constexpr int NR = DP >= 256 ? 1 : 2;
+  const TcRows r = tc_rows(c, a);
+  switch (r.nr * r.wm / NR) {
+    case 0: return launch_tc<CODE, DP, 1, 1>(c, a, st);
+    case 1: return launch_tc<CODE, DP, NR, 1>(c, a, st);
+    case 2: return launch_tc<CODE, DP, NR, 2>(c, a, st);
+    case 4: return launch_tc<CODE, DP, NR, 4>(c, a, st);
+    default:
+      if constexpr (DP >= 256) return launch_tc<CODE, DP, NR, 8>(c, a, st);
+      return set_error(2, "kv8 attention: no kernel for these rows");
   }
 }
 
@@ -1019,9 +1063,9 @@ int kv8_attention_launch(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st
   if (!tc_ok(c, a)) return kv8_attention_generic_launch(c, a, st);
   TAK_BY_CODE(a.code_type, {
     switch (tc_dp(c)) {
-      case 64: return launch_wm<CODE, 64>(c, a, st);
-      case 128: return launch_wm<CODE, 128>(c, a, st);
-      default: return launch_wm<CODE, 256>(c, a, st);
+      case 64: return launch_rows<CODE, 64>(c, a, st);
+      case 128: return launch_rows<CODE, 128>(c, a, st);
+      default: return launch_rows<CODE, 256>(c, a, st);
     }
   });
   return 0;
