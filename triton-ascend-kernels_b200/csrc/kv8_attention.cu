@@ -21,7 +21,7 @@
 //
 // A CTA: one producer warp streams chunks through a ring of TMA loads (K and V
 // codes, page ids from the block table) with the tiles' scales beside them; NW
-// warps consume: WM of them across the query rows (8 or 16 each), NW / WM across
+// warps consume: WM of them across the query rows (8 each), NW / WM across
 // the key tiles.
 #include <cstdio>
 
@@ -45,10 +45,10 @@ struct Kv8TcParams {
   float cap2, inv_cap;  // softcap * log2(e), 2 log2(e) / softcap; 0: no cap
   // workspace
   int4* bound;       // [N] first chunk of each CTA: {sequence, item of it, chunk of the item, chunks of the item}
-  float* part_o;     // [N][2][8 NR WM][DP]
-  float* part_ml;    // [N][2][8 NR WM][2]
+  float* part_o;     // [N][2][8 WM][DP]
+  float* part_ml;    // [N][2][8 WM][2]
   float* lse2;       // [B, Hkv, rows] (weights only)
-  float* scores;     // [B, Hkv, rows, score_ld] (weights only)
+  float* scores;     // [B, Hkv, chunks, 8 WM, score_ld] (weights only)
   int64_t score_ld;
 };
 
@@ -61,15 +61,15 @@ constexpr float kPBias = 13.f;
 constexpr float kLag = 2.f;
 constexpr float kLBias = 10.f;
 constexpr float kLBiasInv = 1.1920928955078125e-7f;  // 2^-(kPBias + kLBias)
+constexpr float kNoMax = -3e38f;             // maximum of a row that has seen no key: finite, so that no difference is inf - inf
 constexpr float kHalfMin = 6.103515625e-5f;  // 2^-14: fp16's smallest normal number
 constexpr int kFew = 8;
 constexpr float kMinVs = 6.162975822039155e-33f;  // 2^-107: the smallest scale that the write makes
 
-// DP: head dim rounded up to 64, 128 or 256.  A warp holds 8 NR query rows, WM
+// DP: head dim rounded up to 64, 128 or 256.  A warp holds eight query rows; WM
 // warps stand across the rows, the rest across the key tiles.
-template <int DP, int NR, int WM> struct Kv8Cfg {
+template <int DP, int WM> struct Kv8Cfg {
   static constexpr int NW = DP >= 256 ? 8 : 4;          // consumer warps
-  static constexpr int RW = 8 * NR;                     // query rows of a warp
   static constexpr int CH = 128;                        // keys of a chunk
   static constexpr int TP = DP >= 256 ? 1 : 2;          // key tiles of a warp's step (two: independent MMA chains)
   static constexpr int NT = CH / 16;                    // key tiles of a chunk
@@ -77,21 +77,14 @@ template <int DP, int NR, int WM> struct Kv8Cfg {
   static constexpr int ROWB = DP >= 128 ? 128 : 64;     // bytes of a row in a column block
   static constexpr int PLANE = CH * DP;                 // bytes of K (or V) in a stage
   static constexpr int STAGE = 2 * PLANE;
-  // With 16 rows a warp Q's fragments live in shared memory ([WM][DP / 16][32
-  // lanes] of 16 bytes) and are loaded per use: in registers they would cost the
-  // third CTA of an SM.  The region is the joining buffer's: an item's Q is dead
-  // when its warps join.
-  static constexpr bool QSMEM = NR == 2 && DP == 128 && WM < 4;
-  static constexpr int CTAS = DP >= 256 ? 1 : DP == 128 && WM == 4 ? 2 : 3;  // per SM
-  static constexpr int NS = DP >= 256 ? 2 : DP == 128 ? (WM == 4 ? 3 : 2) : 4;
-  static constexpr int DH = NR == 2 && (WM < 4 || DP == 64) ? 16 : 32;  // columns joined at a time
+  static constexpr int CTAS = DP >= 256 ? 1 : 3;        // per SM
+  static constexpr int NS = DP == 64 ? 4 : 2;
+  static constexpr int DH = 32;                         // columns joined at a time
   static constexpr int OLD = DH + 8;                    // row stride of the joining buffer (bank spread)
-  static constexpr int MERGE = NW * RW * OLD * 4;
-  static constexpr int QBYTES = QSMEM ? WM * (DP / 16) * 512 : 0;
   static constexpr int META_OFF = NS * STAGE;           // [NS][3][NT] floats: ks, log2 vs + kPBias, 2^-23 / vs
-  static constexpr int OBUF_OFF = META_OFF + NS * 3 * NT * 4;
-  static constexpr int ML_OFF = OBUF_OFF + (MERGE > QBYTES ? MERGE : QBYTES);  // [NW][RW][2]
-  static constexpr int BAR_OFF = ML_OFF + NW * RW * 2 * 4;
+  static constexpr int OBUF_OFF = META_OFF + NS * 3 * NT * 4;  // [NW][8][OLD] floats
+  static constexpr int ML_OFF = OBUF_OFF + NW * 8 * OLD * 4;   // [NW][8][2]
+  static constexpr int BAR_OFF = ML_OFF + NW * 8 * 2 * 4;
   static constexpr int SMEM = BAR_OFF + 2 * NS * 8 + 64 + 1024;
   static_assert((SMEM + 1024) * CTAS <= 228 * 1024, "shared memory");
 };
@@ -185,12 +178,12 @@ template <int CH> struct Kv8Walk {
   __device__ __forceinline__ bool live(const Kv8TcParams& p, int64_t end) const { return at < end && s < p.c.num_seqs; }
 };
 
-template <int CODE, int DP, int NR, int WM>
-__global__ void __launch_bounds__((Kv8Cfg<DP, NR, WM>::NW + 1) * 32, Kv8Cfg<DP, NR, WM>::CTAS)
+template <int CODE, int DP, int WM>
+__global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>::CTAS)
     kv8_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                             const __grid_constant__ Kv8TcParams p) {
-  using C = Kv8Cfg<DP, NR, WM>;
-  constexpr int NW = C::NW, CH = C::CH, NT = C::NT, TP = C::TP, NS = C::NS, WK = NW / WM, RW = C::RW, RT = RW * WM;
+  using C = Kv8Cfg<DP, WM>;
+  constexpr int NW = C::NW, CH = C::CH, NT = C::NT, TP = C::TP, NS = C::NS, WK = NW / WM, RT = 8 * WM;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* meta = reinterpret_cast<float*>(smem + C::META_OFF);
@@ -375,98 +368,81 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, NR, WM>::NW + 1) * 32, Kv8Cfg<DP, 
     // The keys are the M side of both products (S^T = Kc Q^T, O^T = Vc^T P^T), so
     // eight query rows fill an MMA.  k order: thread t4 of a quad holds elements
     // 4 t4 .. 4 t4 + 3 of each 16, the order in which a 32-bit word of codes has them.
-    uint32_t qb[C::QSMEM ? 1 : NR * DP / 16][2];
-    uint4* const qs = reinterpret_cast<uint4*>(smem + C::OBUF_OFF) + wm * (DP / 16) * 32 + lane;
+    uint32_t qb[DP / 16][2];
     auto to_float = [&](uint32_t raw) {
       return p.bf16 ? __uint_as_float(raw << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(raw)));
     };
-    uint2 raw[NR][DP / 16];  // all loads in flight at once
+    uint2 raw[DP / 16];  // all loads in flight at once
+    const int row = rc * RT + wm * 8 + g;
+    const bool real = row < p.rows;
+    const uint16_t* src = kv8_q_row(p, s, kvh, real ? row : 0);
 #pragma unroll
-    for (int nr = 0; nr < NR; ++nr) {
-      const int row = rc * RT + wm * RW + nr * 8 + g;
-      const bool real = row < p.rows;
-      const uint16_t* src = kv8_q_row(p, s, kvh, real ? row : 0);
+    for (int b = 0; b < DP / 16; ++b) {
+      const int d = b * 16 + 4 * t4;
+      uint2 v = make_uint2(0, 0);
+      if (p.q_vec) {
+        if (real && d < p.c.D) v = *reinterpret_cast<const uint2*>(src + d);
+      } else {
+        uint32_t e[4];
 #pragma unroll
-      for (int b = 0; b < DP / 16; ++b) {
-        const int d = b * 16 + 4 * t4;
-        uint2 v = make_uint2(0, 0);
-        if (p.q_vec) {
-          if (real && d < p.c.D) v = *reinterpret_cast<const uint2*>(src + d);
-        } else {
-          uint32_t e[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) e[k] = real && d + k < p.c.D ? src[(d + k) * p.sq[3]] : 0;
-          v = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
-        }
-        raw[nr][b] = v;
+        for (int k = 0; k < 4; ++k) e[k] = real && d + k < p.c.D ? src[(d + k) * p.sq[3]] : 0;
+        v = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
       }
+      raw[b] = v;
     }
     // scores come out with this thread's rows 2 t4 and 2 t4 + 1 (of each eight)
-    float fac[NR][2];
-    int lim[NR][2];  // keys that a row sees
+    float fac[2];
+    int lim[2];  // keys that a row sees
 #pragma unroll
-    for (int nr = 0; nr < NR; ++nr)
+    for (int k = 0; k < 2; ++k) {
+      const int row = rc * RT + wm * 8 + 2 * t4 + k;
+      lim[k] = row < p.rows ? ctx - p.Lq + row / p.G + 1 : ctx;  // rows that pad the tile see every key
+    }
+    float top = 0.f;
+    bool odd = false;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int row = rc * RT + wm * RW + nr * 8 + 2 * t4 + k;
-        lim[nr][k] = row < p.rows ? ctx - p.Lq + row / p.G + 1 : ctx;  // rows that pad the tile see every key
-      }
-    // the last item's joining buffer has been read: Q may take its place
-    if (C::QSMEM) asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");
+    for (int b = 0; b < DP / 16; ++b) {
+      const uint2 v = raw[b];
+      const float f[4] = {to_float(v.x & 0xffff), to_float(v.x >> 16), to_float(v.y & 0xffff), to_float(v.y >> 16)};
 #pragma unroll
-    for (int nr = 0; nr < NR; ++nr) {
-      float top = 0.f;
-      bool odd = false;
-#pragma unroll
-      for (int b = 0; b < DP / 16; ++b) {
-        const uint2 v = raw[nr][b];
-        const float f[4] = {to_float(v.x & 0xffff), to_float(v.x >> 16), to_float(v.y & 0xffff), to_float(v.y >> 16)};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          top = fmaxf(top, fabsf(f[k]));
-          odd |= !(fabsf(f[k]) < INFINITY);
-        }
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      odd |= __shfl_xor_sync(0xffffffffu, odd, 1);
-      odd |= __shfl_xor_sync(0xffffffffu, odd, 2);
-      // 2^e <= top < 2^(e+1); the row's largest comes to [2^8, 2^9)
-      const int e2 = odd || top == 0.f ? 8 : max(-110, static_cast<int>(__float_as_uint(top) >> 23) - 127);
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + 8 - e2) << 23);
-      const float f = p.scale * __uint_as_float(static_cast<uint32_t>(127 - 8 + e2) << 23);
-      fac[nr][0] = __shfl_sync(0xffffffffu, f, 8 * t4);
-      fac[nr][1] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
-#pragma unroll
-      for (int b = 0; b < DP / 16; ++b) {
-        const uint2 v = raw[nr][b];
-        const uint32_t q01 = Elem<__half>::pack2(to_float(v.x & 0xffff) * up, to_float(v.x >> 16) * up);
-        const uint32_t q23 = Elem<__half>::pack2(to_float(v.y & 0xffff) * up, to_float(v.y >> 16) * up);
-        if (!C::QSMEM) {
-          qb[C::QSMEM ? 0 : nr * (DP / 16) + b][0] = q01;
-          qb[C::QSMEM ? 0 : nr * (DP / 16) + b][1] = q23;
-        } else if (wk == 0) {
-          reinterpret_cast<uint2*>(qs + b * 32)[nr] = make_uint2(q01, q23);
-        }
+      for (int k = 0; k < 4; ++k) {
+        top = fmaxf(top, fabsf(f[k]));
+        odd |= !(fabsf(f[k]) < INFINITY);
       }
     }
-    if (C::QSMEM) asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    odd |= __shfl_xor_sync(0xffffffffu, odd, 1);
+    odd |= __shfl_xor_sync(0xffffffffu, odd, 2);
+    // 2^e <= top < 2^(e+1); the row's largest comes to [2^8, 2^9)
+    const int e2 = odd || top == 0.f ? 8 : max(-110, static_cast<int>(__float_as_uint(top) >> 23) - 127);
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + 8 - e2) << 23);
+    const float f = p.scale * __uint_as_float(static_cast<uint32_t>(127 - 8 + e2) << 23);
+    fac[0] = __shfl_sync(0xffffffffu, f, 8 * t4);
+    fac[1] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
+#pragma unroll
+    for (int b = 0; b < DP / 16; ++b) {
+      const uint2 v = raw[b];
+      const uint32_t q01 = Elem<__half>::pack2(to_float(v.x & 0xffff) * up, to_float(v.x >> 16) * up);
+      const uint32_t q23 = Elem<__half>::pack2(to_float(v.y & 0xffff) * up, to_float(v.y >> 16) * up);
+      qb[b][0] = q01;
+      qb[b][1] = q23;
+    }
 
-    float o[NR][DP / 16][4];  // (column 2 g, 2 g + 1 of each 16) x (row 2 t4, 2 t4 + 1): c0 c1 / c2 c3
-    float m[NR][2], l[NR][2];
-    int above[NR][2];   // keys counted in fp16's normal range since the maximum last rose
+    float o[DP / 16][4];  // (column 2 g, 2 g + 1 of each 16) x (row 2 t4, 2 t4 + 1): c0 c1 / c2 c3
+    float m[2], l[2];
+    int above[2];   // keys counted in fp16's normal range since the maximum last rose
     bool many = false;  // every row of the warp has kFew of them
 #pragma unroll
-    for (int nr = 0; nr < NR; ++nr) {
+    for (int i = 0; i < DP / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
-      for (int i = 0; i < DP / 16; ++i) o[nr][i][0] = o[nr][i][1] = o[nr][i][2] = o[nr][i][3] = 0.f;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        m[nr][k] = -INFINITY;
-        l[nr][k] = 0.f;
-        above[nr][k] = 0;
-      }
+    for (int k = 0; k < 2; ++k) {
+      m[k] = kNoMax;
+      l[k] = 0.f;
+      above[k] = 0;
     }
+    // this thread's first row of the stored scores, [item][8 WM rows of each chunk][score_ld]
+    float* const score_row = p.scores + ((static_cast<int64_t>(s) * items + w.r) * RT + wm * 8 + 2 * t4) * p.score_ld;
     const int open = ctx - p.Lq + 1;  // keys below it are seen by every row
 
     for (int j = j0; j < j_end; ++j, ++it) {
@@ -494,11 +470,9 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, NR, WM>::NW + 1) * 32, Kv8Cfg<DP, 
           __syncwarp();
         }
         // ---- S^T = Kc Q^T for TP tiles of 16 keys ----
-        float x[TP][NR][4];  // c0 c1: key g, rows 2 t4, 2 t4 + 1; c2 c3: key g + 8
+        float x[TP][4];  // c0 c1: key g, rows 2 t4, 2 t4 + 1; c2 c3: key g + 8
 #pragma unroll
-        for (int u = 0; u < TP; ++u)
-#pragma unroll
-          for (int nr = 0; nr < NR; ++nr) x[u][nr][0] = x[u][nr][1] = x[u][nr][2] = x[u][nr][3] = 0.f;
+        for (int u = 0; u < TP; ++u) x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.f;
 #pragma unroll
         for (int kb = 0; kb < DP / 32; ++kb) {
           const int piece = 2 * kb + (mi >> 1);
@@ -509,107 +483,101 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, NR, WM>::NW + 1) * 32, Kv8Cfg<DP, 
                     r[u][1], r[u][2], r[u][3]);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {  // k16 step; r[.][2 k]: the first eight keys, r[.][2 k + 1]: the others
-            uint32_t qf[4];
-            if (C::QSMEM) *reinterpret_cast<uint4*>(qf) = qs[(2 * kb + k) * 32];
 #pragma unroll
             for (int u = 0; u < TP; ++u) {
               uint32_t af[4];
               codes_to_half<CODE, 0>(r[u][2 * k], af[0], af[2]);
               codes_to_half<CODE, 0>(r[u][2 * k + 1], af[1], af[3]);
-#pragma unroll
-              for (int nr = 0; nr < NR; ++nr) {
-                const uint32_t* q2 = C::QSMEM ? qf + 2 * nr : qb[C::QSMEM ? 0 : nr * (DP / 16) + 2 * kb + k];
-                Mma<__half>::run(x[u][nr], af, q2[0], q2[1]);
-              }
+              Mma<__half>::run(x[u], af, qb[2 * kb + k][0], qb[2 * kb + k][1]);
             }
           }
         }
         // ---- scores, base 2 ----
         const bool masked = tok + 16 * TP > open;
-        float lv[TP], ivs[TP], y[NR][2];  // y: largest score + log2 vs + kPBias
-        bool v_bad[TP];
-#pragma unroll
-        for (int nr = 0; nr < NR; ++nr) y[nr][0] = y[nr][1] = -INFINITY;
+        float lv[TP], ivs[TP], y[2] = {-INFINITY, -INFINITY};  // y: largest score + log2 vs + kPBias
 #pragma unroll
         for (int u = 0; u < TP; ++u) {
-          const float ks = mt[t + u], lvt = mt[NT + t + u];
+          const float ks = mt[t + u];
+          lv[u] = mt[NT + t + u];
           ivs[u] = mt[2 * NT + t + u];
-          v_bad[u] = lvt != lvt;
-          lv[u] = v_bad[u] ? kPBias : lvt;
+          const float f0 = fac[0] * ks, f1 = fac[1] * ks;
+          x[u][0] *= f0;
+          x[u][1] *= f1;
+          x[u][2] *= f0;
+          x[u][3] *= f1;
+        }
+        bool v_bad = lv[0] != lv[0];  // (the tiles of a NaN or infinite V scale are marked by a NaN)
+        if (TP > 1) v_bad |= lv[TP - 1] != lv[TP - 1];
+        if (v_bad) {
 #pragma unroll
-          for (int nr = 0; nr < NR; ++nr) {
+          for (int u = 0; u < TP; ++u) lv[u] = lv[u] == lv[u] ? lv[u] : kPBias;
+        }
+        if (p.inv_cap > 0.f) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float z = x[u][nr][e] * (fac[nr][e & 1] * ks);
-              if (p.inv_cap > 0.f) {
-                // cap * tanh(z / cap) = cap * (1 - 2 / (1 + e^(2 z / cap)))
-                const float ez = fast_exp2(z * p.inv_cap);
-                z = p.cap2 * (1.f - __fdividef(2.f, 1.f + ez));
-              }
-              if (masked && tok + u * 16 + g + (e & 2) * 4 >= lim[nr][e & 1]) z = -INFINITY;
-              x[u][nr][e] = z;
+          for (int u = 0; u < TP; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)  // cap * tanh(z / cap) = cap * (1 - 2 / (1 + e^(2 z / cap)))
+              x[u][e] = p.cap2 * (1.f - __fdividef(2.f, 1.f + fast_exp2(x[u][e] * p.inv_cap)));
+        }
+        if (masked) {
+#pragma unroll
+          for (int u = 0; u < TP; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (tok + u * 16 + g + (e & 2) * 4 >= lim[e & 1]) x[u][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int u = 0; u < TP; ++u)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) y[k] = fmaxf(y[k], lv[u] + fmaxf(x[u][k], x[u][k + 2]));
+        if (p.scores) {
+#pragma unroll
+          for (int u = 0; u < TP; ++u) {
+            if (tok + u * 16 >= p.score_ld) continue;
+            float* sp = score_row + tok + u * 16 + g;  // (rows that pad the tile have rows of their own there)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              sp[k * p.score_ld] = x[u][k];
+              sp[k * p.score_ld + 8] = x[u][k + 2];
             }
-#pragma unroll
-            for (int k = 0; k < 2; ++k) y[nr][k] = fmaxf(y[nr][k], lv[u] + fmaxf(x[u][nr][k], x[u][nr][k + 2]));
-          }
-          if (p.scores && tok + u * 16 < p.score_ld) {
-#pragma unroll
-            for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const int row = rc * RT + wm * RW + nr * 8 + 2 * t4 + k;
-                if (row < p.rows) {
-                  float* sp = p.scores + ((static_cast<int64_t>(s) * p.c.Hkv + kvh) * p.rows + row) * p.score_ld + tok + u * 16 + g;
-                  sp[0] = x[u][nr][k];
-                  sp[8] = x[u][nr][k + 2];
-                }
-              }
           }
         }
         // ---- running maximum: raised only when a score passes it by 2^kLag ----
         bool up = false;
 #pragma unroll
-        for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) up |= y[nr][k] > m[nr][k] + (kLag + kPBias);
+        for (int k = 0; k < 2; ++k) up |= y[k] > m[k] + (kLag + kPBias);
         if (__any_sync(0xffffffffu, up)) {
+          float al[2];
 #pragma unroll
-          for (int nr = 0; nr < NR; ++nr) {
-            float al[2];
+          for (int k = 0; k < 2; ++k) {
+            float mx = y[k] - kPBias;
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float mn = fmaxf(m[k], mx);
+            al[k] = fast_exp2(m[k] - mn);
+            m[k] = mn;
+            l[k] *= al[k];
+            above[k] = 0;
+          }
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              float mx = y[nr][k] - kPBias;
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              const float mn = fmaxf(m[nr][k], mx), mu = mn == -INFINITY ? 0.f : mn;
-              al[k] = fast_exp2(m[nr][k] - mu);
-              m[nr][k] = mn;
-              l[nr][k] *= al[k];
-              above[nr][k] = 0;
-            }
-#pragma unroll
-            for (int i = 0; i < DP / 16; ++i) {
-              o[nr][i][0] *= al[0];
-              o[nr][i][1] *= al[1];
-              o[nr][i][2] *= al[0];
-              o[nr][i][3] *= al[1];
-            }
+          for (int i = 0; i < DP / 16; ++i) {
+            o[i][0] *= al[0];
+            o[i][1] *= al[1];
+            o[i][2] *= al[0];
+            o[i][3] *= al[1];
           }
           many = false;
         }
-        uint32_t pb[TP][NR][2];  // P^T fragments
+        uint32_t pb[TP][2];  // P^T fragments
 #pragma unroll
         for (int u = 0; u < TP; ++u)
 #pragma unroll
-          for (int nr = 0; nr < NR; ++nr) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float c0 = lv[u] - (m[nr][k] == -INFINITY ? 0.f : m[nr][k]);
-              x[u][nr][k] = fast_exp2(x[u][nr][k] + c0);
-              x[u][nr][k + 2] = fast_exp2(x[u][nr][k + 2] + c0);
-              l[nr][k] = fmaf(x[u][nr][k] + x[u][nr][k + 2], ivs[u], l[nr][k]);
-            }
+          for (int k = 0; k < 2; ++k) {
+            const float c0 = lv[u] - m[k];
+            x[u][k] = fast_exp2(x[u][k] + c0);
+            x[u][k + 2] = fast_exp2(x[u][k + 2] + c0);
+            l[k] = fmaf(x[u][k] + x[u][k + 2], ivs[u], l[k]);
           }
         // ---- weights below fp16's normal range (2^-27 of the largest): while a row
         // of the warp has fewer than kFew keys above it, they go through the
@@ -620,78 +588,71 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, NR, WM>::NW + 1) * 32, Kv8Cfg<DP, 
           float least = 1.f;
           int fewest = kFew;
 #pragma unroll
-          for (int nr = 0; nr < NR; ++nr)
+          for (int k = 0; k < 2; ++k) {
+            int n = 0;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              int n = 0;
+            for (int u = 0; u < TP; ++u)
 #pragma unroll
-              for (int u = 0; u < TP; ++u)
-#pragma unroll
-                for (int e = k; e < 4; e += 2) {
-                  least = fminf(least, x[u][nr][e]);
-                  n += x[u][nr][e] >= kHalfMin;
-                }
-              n += __shfl_xor_sync(0xffffffffu, n, 4);
-              n += __shfl_xor_sync(0xffffffffu, n, 8);
-              n += __shfl_xor_sync(0xffffffffu, n, 16);
-              above[nr][k] += n;
-              fewest = min(fewest, above[nr][k]);
-            }
+              for (int e = k; e < 4; e += 2) {
+                least = fminf(least, x[u][e]);
+                n += x[u][e] >= kHalfMin;
+              }
+            n += __shfl_xor_sync(0xffffffffu, n, 4);
+            n += __shfl_xor_sync(0xffffffffu, n, 8);
+            n += __shfl_xor_sync(0xffffffffu, n, 16);
+            above[k] += n;
+            fewest = min(fewest, above[k]);
+          }
           many = __all_sync(0xffffffffu, fewest >= kFew);
           apart = !many && __any_sync(0xffffffffu, least < kHalfMin);
         }
         if (apart) {
-          uint32_t pc[TP][NR][2];
+          uint32_t pc[TP][2];
           bool some = false;
 #pragma unroll
-          for (int u = 0; u < TP; ++u)
+          for (int u = 0; u < TP; ++u) {
+            float f[4];
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) {
-              float f[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float v = x[u][nr][e];
-                const bool small = v < kHalfMin;
-                f[e] = small ? v * 16777216.f : 0.f;
-                x[u][nr][e] = small ? 0.f : v;
-                some |= f[e] > 0.f;
-              }
-              pc[u][nr][0] = transpose8x8(Elem<__half>::pack2(f[0], f[1]));
-              pc[u][nr][1] = transpose8x8(Elem<__half>::pack2(f[2], f[3]));
+            for (int e = 0; e < 4; ++e) {
+              const float v = x[u][e];
+              const bool small = v < kHalfMin;
+              f[e] = small ? v * 16777216.f : 0.f;
+              x[u][e] = small ? 0.f : v;
+              some |= f[e] > 0.f;
             }
+            pc[u][0] = transpose8x8(Elem<__half>::pack2(f[0], f[1]));
+            pc[u][1] = transpose8x8(Elem<__half>::pack2(f[2], f[3]));
+          }
           if (__any_sync(0xffffffffu, some)) {
 #pragma unroll
             for (int db = 0; db < DP / 16; ++db) {
-              float a[NR][4];
-#pragma unroll
-              for (int nr = 0; nr < NR; ++nr) a[nr][0] = a[nr][1] = a[nr][2] = a[nr][3] = 0.f;
+              float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
               for (int u = 0; u < TP; ++u) {
                 uint32_t r[2], af[4];
                 ldsm_x2_t(vbase + (db >> 3) * CH * C::ROWB + kv8_sw<DP>(r0 + u * 16 + (mi & 1) * 8 + rr, db & 7), r[0], r[1]);
                 codes_to_half<CODE, 1>(r[0], af[0], af[1]);
                 codes_to_half<CODE, 1>(r[1], af[2], af[3]);
-#pragma unroll
-                for (int nr = 0; nr < NR; ++nr) Mma<__half>::run(a[nr], af, pc[u][nr][0], pc[u][nr][1]);
+                Mma<__half>::run(a, af, pc[u][0], pc[u][1]);
               }
 #pragma unroll
-              for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[nr][db][e] = fmaf(a[nr][e], 5.9604644775390625e-8f, o[nr][db][e]);
+              for (int e = 0; e < 4; ++e) o[db][e] = fmaf(a[e], 5.9604644775390625e-8f, o[db][e]);
             }
           }
         }
+        if (v_bad) {  // a NaN or infinite V scale: NaN for the rows that see a key of the tile
 #pragma unroll
         for (int u = 0; u < TP; ++u)
+          if (mt[NT + t + u] != mt[NT + t + u]) {
 #pragma unroll
-          for (int nr = 0; nr < NR; ++nr) {
-            if (v_bad[u]) {  // a NaN or infinite V scale: NaN for the rows that see a key of the tile
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x[u][nr][e] = tok + u * 16 < lim[nr][e & 1] ? __uint_as_float(0x7fffffffu) : 0.f;
+                for (int e = 0; e < 4; ++e) x[u][e] = tok + u * 16 < lim[e & 1] ? __uint_as_float(0x7fffffffu) : 0.f;
             }
-            pb[u][nr][0] = transpose8x8(Elem<__half>::pack2(x[u][nr][0], x[u][nr][1]));
-            pb[u][nr][1] = transpose8x8(Elem<__half>::pack2(x[u][nr][2], x[u][nr][3]));
-          }
+        }
+#pragma unroll
+        for (int u = 0; u < TP; ++u) {
+          pb[u][0] = transpose8x8(Elem<__half>::pack2(x[u][0], x[u][1]));
+          pb[u][1] = transpose8x8(Elem<__half>::pack2(x[u][2], x[u][3]));
+        }
         // ---- O^T += Vc^T P^T: words transposed by the load pair two keys of columns
         // 2 g and 2 g + 1, which become rows g and g + 8 of the MMA ----
 #pragma unroll
@@ -707,8 +668,7 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, NR, WM>::NW + 1) * 32, Kv8Cfg<DP, 
               uint32_t af[4];
               codes_to_half<CODE, 1>(r[2 * k], af[0], af[1]);
               codes_to_half<CODE, 1>(r[2 * k + 1], af[2], af[3]);
-#pragma unroll
-              for (int nr = 0; nr < NR; ++nr) Mma<__half>::run(o[nr][2 * db + k], af, pb[u][nr][0], pb[u][nr][1]);
+              Mma<__half>::run(o[2 * db + k], af, pb[u][0], pb[u][1]);
             }
           }
         }
@@ -719,49 +679,43 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, NR, WM>::NW + 1) * 32, Kv8Cfg<DP, 
 
     // ---- join the warps that shared the rows, then finish or store a part ----
 #pragma unroll
-    for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        l[nr][k] += __shfl_xor_sync(0xffffffffu, l[nr][k], 4);
-        l[nr][k] += __shfl_xor_sync(0xffffffffu, l[nr][k], 8);
-        l[nr][k] += __shfl_xor_sync(0xffffffffu, l[nr][k], 16);
-      }
+    for (int k = 0; k < 2; ++k) {
+      l[k] += __shfl_xor_sync(0xffffffffu, l[k], 4);
+      l[k] += __shfl_xor_sync(0xffffffffu, l[k], 8);
+      l[k] += __shfl_xor_sync(0xffffffffu, l[k], 16);
+    }
     const bool whole = j0 == 0 && j_end == w.n;
     const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (j0 == 0 ? 1 : 0)) * RT;
 #pragma unroll
     for (int dh = 0; dh < DP / C::DH; ++dh) {
       asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");  // the buffer is free again
 #pragma unroll
-      for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-        for (int i = 0; i < C::DH / 16; ++i) {
-          const float* ot = o[nr][dh * (C::DH / 16) + i];
-          float* dst = obuf + (warp * RW + nr * 8 + 2 * t4) * C::OLD + i * 16 + 2 * g;
-          *reinterpret_cast<float2*>(dst) = make_float2(ot[0], ot[2]);
-          *reinterpret_cast<float2*>(dst + C::OLD) = make_float2(ot[1], ot[3]);
-        }
+      for (int i = 0; i < C::DH / 16; ++i) {
+        const float* ot = o[dh * (C::DH / 16) + i];
+        float* dst = obuf + (warp * 8 + 2 * t4) * C::OLD + i * 16 + 2 * g;
+        *reinterpret_cast<float2*>(dst) = make_float2(ot[0], ot[2]);
+        *reinterpret_cast<float2*>(dst + C::OLD) = make_float2(ot[1], ot[3]);
+      }
       if (dh == 0 && g == 0) {
 #pragma unroll
-        for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            *reinterpret_cast<float2*>(mlbuf + (warp * RW + nr * 8 + 2 * t4 + k) * 2) = make_float2(m[nr][k], l[nr][k]);
+        for (int k = 0; k < 2; ++k)
+          *reinterpret_cast<float2*>(mlbuf + (warp * 8 + 2 * t4 + k) * 2) = make_float2(m[k], l[k]);
       }
       asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");
       for (int e = tid; e < RT * (C::DH / 4); e += NW * 32) {
         const int row = e / (C::DH / 4), d = (e - row * (C::DH / 4)) * 4;
         const int grow = rc * RT + row;
         if (grow >= p.rows) continue;
-        const int tile = row / RW, rw = row % RW;
+        const int tile = row >> 3, rw = row & 7;
         float M = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < WK; ++k) M = fmaxf(M, mlbuf[((k * WM + tile) * RW + rw) * 2]);
+        for (int k = 0; k < WK; ++k) M = fmaxf(M, mlbuf[((k * WM + tile) * 8 + rw) * 2]);
         const float Mu = M == -INFINITY ? 0.f : M;
         float L = 0.f;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < WK; ++k) {
-          const int at = (k * WM + tile) * RW + rw;
+          const int at = (k * WM + tile) * 8 + rw;
           const float f = fast_exp2(mlbuf[at * 2] - Mu);
           L = fmaf(mlbuf[at * 2 + 1], f, L);
           const float4 v = *reinterpret_cast<const float4*>(obuf + at * C::OLD + d);
@@ -897,15 +851,15 @@ __global__ void __launch_bounds__(128) kv8_attention_join_kernel(const Kv8TcPara
 
 // Attention weights from the stored scores: each thread owns keys, so every
 // weight is added to once, in the order of the rows.
-__global__ void __launch_bounds__(256) kv8_attention_weights_kernel(const Kv8TcParams p, float* weights, int64_t w0,
-                                                                    int64_t w1, int64_t w2, int64_t width) {
+__global__ void __launch_bounds__(256) kv8_attention_weights_kernel(const Kv8TcParams p, int RT, float* weights,
+                                                                    int64_t w0, int64_t w1, int64_t w2, int64_t width) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int kvh = blockIdx.y, s = blockIdx.z;
   const int64_t n = min(static_cast<int64_t>(kv8_ctx(p, s)), width);
   const int64_t pos = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (pos >= n) return;
   const int64_t item = static_cast<int64_t>(s) * p.c.Hkv + kvh;
-  const float* sc = p.scores + item * p.rows * p.score_ld + pos;
+  const float* sc = p.scores + item * p.chunks * RT * p.score_ld + pos;  // a head's chunks follow one another: row r at r
   const float* ls = p.lse2 + item * p.rows;
   float sum = 0.f;
   for (int r = 0; r < p.rows; ++r) {
@@ -930,23 +884,20 @@ static bool tc_ok(const Kv8View& c, const Kv8AttnArgs& a) {
   return true;
 }
 static int tc_dp(const Kv8View& c) { return c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256; }
-// Rows of a warp (8 NR) and warps across the rows (WM): as many as the query rows
-// of a KV head fill, up to 64.  At 256 columns O allows eight rows a warp.
-struct TcRows { int nr, wm; };
-static TcRows tc_rows(const Kv8View& c, const Kv8AttnArgs& a) {
+// Warps across the query rows (eight each): as many as the rows of a KV head
+// fill.  Sixteen rows a warp (two MMA columns for each converted tile) measured
+// slower, for want of registers: 16 rows of 64 x <= 8192 keys 153 us against 119.
+static int tc_wm(const Kv8View& c, const Kv8AttnArgs& a) {
   const int64_t rows = static_cast<int64_t>(a.H / c.Hkv) * a.Lq;
-  if (rows <= 8) return {1, 1};
-  if (tc_dp(c) == 256) return {1, rows <= 16 ? 2 : rows <= 32 ? 4 : 8};
-  return {2, rows <= 16 ? 1 : rows <= 32 ? 2 : 4};
+  return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 || tc_dp(c) < 256 ? 4 : 8;
 }
 struct TcSizes { int N, RT, DP; int64_t bound, ml, o, lse2, scores, total, score_ld; };
 static int64_t up16(int64_t x) { return (x + 255) / 256 * 256; }
 static TcSizes tc_sizes(const Kv8View& c, const Kv8AttnArgs& a) {
   TcSizes z{};
   z.DP = tc_dp(c);
-  const TcRows r = tc_rows(c, a);
-  z.N = num_sms() * (z.DP >= 256 ? 1 : z.DP == 128 && r.wm == 4 ? 2 : 3);  // Kv8Cfg::CTAS
-  z.RT = 8 * r.nr * r.wm;
+  z.N = num_sms() * (z.DP >= 256 ? 1 : 3);  // Kv8Cfg::CTAS
+  z.RT = 8 * tc_wm(c, a);
   const int64_t rows = static_cast<int64_t>(a.H / c.Hkv) * a.Lq, all = rows * c.Hkv * c.num_seqs;
   int64_t at = 0;
   z.bound = at; at += up16(static_cast<int64_t>(z.N) * 16);
@@ -956,7 +907,8 @@ static TcSizes tc_sizes(const Kv8View& c, const Kv8AttnArgs& a) {
     const int64_t w = a.weights_width < c.max_rows ? a.weights_width : c.max_rows;
     z.score_ld = (w + 15) / 16 * 16;
     z.lse2 = at; at += up16(all * 4);
-    z.scores = at; at += up16(all * z.score_ld * 4);
+    const int64_t padded = (rows + z.RT - 1) / z.RT * z.RT * c.Hkv * c.num_seqs;
+    z.scores = at; at += up16(padded * z.score_ld * 4);
   }
   z.total = at + 256;
   return z;
@@ -997,9 +949,9 @@ static int launch_dependent(K kern, dim3 grid, int threads, cudaStream_t st, A..
   return set_error(3, buf);
 }
 
-template <int CODE, int DP, int NR, int WM>
+template <int CODE, int DP, int WM>
 static int launch_tc(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
-  using C = Kv8Cfg<DP, NR, WM>;
+  using C = Kv8Cfg<DP, WM>;
   const TcSizes z = tc_sizes(c, a);
   Kv8TcParams p{};
   p.c = c;
@@ -1030,7 +982,7 @@ static int launch_tc(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
   CUtensorMap mk, mv;
   if (const int r = encode_codes(&mk, c, 0, C::ROWB, p.box_rows)) return r;
   if (const int r = encode_codes(&mv, c, 1, C::ROWB, p.box_rows)) return r;
-  auto kern = kv8_attention_tc_kernel<CODE, DP, NR, WM>;
+  auto kern = kv8_attention_tc_kernel<CODE, DP, WM>;
   if (const int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::SMEM)) return r;
   kern<<<z.N, (C::NW + 1) * 32, C::SMEM, st>>>(mk, mv, p);
   note_kernel("kv8_attention_tc");
@@ -1038,22 +990,19 @@ static int launch_tc(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
   if (a.weights) {
     const int64_t w = a.weights_width < c.max_rows ? a.weights_width : c.max_rows;
     return launch_dependent(kv8_attention_weights_kernel, dim3(static_cast<unsigned>((w + 255) / 256), c.Hkv, c.num_seqs),
-                            256, st, p, a.weights, a.sw[0], a.sw[1], a.sw[2], w);
+                            256, st, p, z.RT, a.weights, a.sw[0], a.sw[1], a.sw[2], w);
   }
   return 0;
 }
 
 template <int CODE, int DP>
 static int launch_rows(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
-  constexpr int NR = DP >= 256 ? 1 : 2;
-  const TcRows r = tc_rows(c, a);
-  switch (r.nr * r.wm / NR) {
-    case 0: return launch_tc<CODE, DP, 1, 1>(c, a, st);
-    case 1: return launch_tc<CODE, DP, NR, 1>(c, a, st);
-    case 2: return launch_tc<CODE, DP, NR, 2>(c, a, st);
-    case 4: return launch_tc<CODE, DP, NR, 4>(c, a, st);
+  switch (tc_wm(c, a)) {
+    case 1: return launch_tc<CODE, DP, 1>(c, a, st);
+    case 2: return launch_tc<CODE, DP, 2>(c, a, st);
+    case 4: return launch_tc<CODE, DP, 4>(c, a, st);
     default:
-      if constexpr (DP >= 256) return launch_tc<CODE, DP, NR, 8>(c, a, st);
+      if constexpr (DP >= 256) return launch_tc<CODE, DP, 8>(c, a, st);
       return set_error(2, "kv8 attention: no kernel for these rows");
   }
 }
