@@ -89,6 +89,43 @@ __device__ __forceinline__ float kv8_scale_max(float a, float b) {
   return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
 }
 
+// Four codes at once, the same roundings as dec and enc one by one.
+// int8 -> fp32: the byte with its sign bit flipped, as the mantissa's low byte of
+// 2^23, less 2^23 + 128.  fp32 -> int8: adding 1.5 * 2^23 rounds to nearest even
+// and leaves the two's complement in the low byte (|x| < 128 from a finite scale).
+template <int CODE> __device__ __forceinline__ void kv8_dec4(uint32_t q, float* f) {
+  if (CODE == kI8) {
+    const uint32_t x = q ^ 0x80808080u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7540 + k)) - 8388736.f;
+  } else {
+    const float2 a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q & 0xffffu), __NV_E4M3)));
+    const float2 b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q >> 16), __NV_E4M3)));
+    f[0] = a.x;
+    f[1] = a.y;
+    f[2] = b.x;
+    f[3] = b.y;
+  }
+}
+template <int CODE> __device__ __forceinline__ uint32_t kv8_enc4(const float* f) {
+  if (CODE == kI8) {
+    uint32_t u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) u[k] = __float_as_uint(__fadd_rn(fminf(fmaxf(f[k], -127.f), 127.f), 12582912.f));
+    return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+  }
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+template <int CODE> __device__ __forceinline__ uint32_t kv8_rescale4(uint32_t q, float ratio) {
+  float f[4];
+  kv8_dec4<CODE>(q, f);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) f[k] = __fmul_rn(f[k], ratio);
+  return kv8_enc4<CODE>(f);
+}
+
 struct Kv8AttnArgs {
   const void* q; int64_t sq[4];       // [B, Lq, H, D]
   const int32_t* context_lens;

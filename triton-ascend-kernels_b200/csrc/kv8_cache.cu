@@ -1,7 +1,7 @@
 // Writing rows into the 8-bit KV cache and reading them back.
 //
-// Write: rows of sequence s go to positions [start_s, start_s + n_s).  One CTA
-// per (sequence, group of rows, head, K or V): the largest magnitude of the
+// Write: rows of sequence s go to positions [start_s, start_s + n_s).  One work
+// item per (sequence, group of rows, head, K or V): the largest magnitude of the
 // group's new rows gives a scale; where the group already holds rows (its first
 // position lies before start_s) the scale is the larger of that and the stored
 // one, and rows held under a smaller scale are requantised,
@@ -22,60 +22,188 @@ struct Kv8WriteParams {
 // Work items of a sequence: group g of its rows [start, start + n).  Sequence s
 // owns items [cu[s] / group + 2 s, cu[s + 1] / group + 2 (s + 1)), at least as
 // many as the groups that n rows can touch, so the list needs no prefix sums.
+// Without cu each sequence has one row and one item.
 __device__ __forceinline__ int64_t kv8_item_base(const Kv8WriteParams& p, int s) {
-  return (p.cu ? p.cu[s] : s) / p.c.group + 2 * static_cast<int64_t>(s);
+  return p.cu ? p.cu[s] / p.c.group + 2 * static_cast<int64_t>(s) : s;
 }
 
+// What an item writes: rows [r0, r0 + fresh) of sequence s, after `held` rows that
+// the group has.
+struct Kv8WriteItem {
+  int s, held, fresh, in_page;
+  int64_t page, token;
+};
+__device__ __forceinline__ bool kv8_write_item(const Kv8WriteParams& p, int64_t item, Kv8WriteItem& w) {
+  const Kv8View& c = p.c;
+  int lo = 0, hi = c.num_seqs - 1;
+  if (p.cu) {
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (kv8_item_base(p, mid) <= item) lo = mid; else hi = mid - 1;
+    }
+  } else {
+    lo = static_cast<int>(item);
+  }
+  const int64_t tok0 = p.cu ? p.cu[lo] : lo;
+  const int64_t n = p.cu ? p.cu[lo + 1] - tok0 : 1;
+  const int64_t start = p.start_lens[lo];
+  const int64_t first = (start / c.group + (item - kv8_item_base(p, lo))) * c.group;  // the group's first position
+  if (n <= 0 || start < 0 || first >= start + n) return false;
+  w.s = lo;
+  w.page = kv8_page(c, lo, first);
+  if (w.page < 0) return false;
+  const int64_t r0 = max(start, first), r1 = min(start + n, first + c.group);
+  w.in_page = static_cast<int>(first % c.P);
+  w.token = tok0 + (r0 - start);
+  w.held = static_cast<int>(r0 - first);
+  w.fresh = static_cast<int>(r1 - r0);
+  return true;
+}
+
+// Eight elements of a row, as loaded (16-bit types: one 16-byte word)
+template <typename T> struct Eight {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* x) { v = *reinterpret_cast<const uint4*>(x); }
+  __device__ __forceinline__ void get(float* f) const {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 t = Elem<T>::unpack2(u[k]);
+      f[2 * k] = t.x;
+      f[2 * k + 1] = t.y;
+    }
+  }
+};
+template <> struct Eight<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* x) {
+    a = *reinterpret_cast<const float4*>(x);
+    b = *reinterpret_cast<const float4*>(x + 4);
+  }
+  __device__ __forceinline__ void get(float* f) const {
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  }
+};
+
+// One item held in registers: TPI threads (one warp, or a CTA of its own), up to
+// eight pieces of eight elements each, so the rows are read once.
+template <typename T, int CODE, int TPI>
+__global__ void __launch_bounds__(TPI == 32 ? 128 : TPI) kv8_write_vec_kernel(const Kv8WriteParams p, int64_t items) {
+  constexpr int U = 8;
+  const Kv8View& c = p.c;
+  const int lane = threadIdx.x % TPI;
+  // heads and planes of an item are neighbours: they read the same rows
+  int64_t id = TPI == 32 ? static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32 : blockIdx.x;
+  const int which = static_cast<int>(id & 1);
+  id >>= 1;
+  const int h = static_cast<int>(id % c.Hkv);
+  id /= c.Hkv;
+  Kv8WriteItem w;
+  if (id >= items || !kv8_write_item(p, id, w)) return;
+  const Kv8Plane& pl = c.plane[which];
+  const T* x = static_cast<const T*>(p.x[which]) + w.token * p.sx[which][0] + h * p.sx[which][1];
+  const int pr = c.D / 8, n = w.fresh * pr;  // pieces of a row, of the item
+  Eight<T> v[U];
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int e = lane + k * TPI;
+    if (e < n) v[k].load(x + (e / pr) * p.sx[which][0] + (e % pr) * 8);
+  }
+  float* sp = kv8_scale(pl, w.page, h, w.in_page / c.group);
+  const float was = *sp;
+  uint32_t amax = 0;
+#pragma unroll
+  for (int k = 0; k < U; ++k)
+    if (lane + k * TPI < n) {
+      float f[8];
+      v[k].get(f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = max(amax, abs_bits(f[i]));
+    }
+  amax = __reduce_max_sync(0xffffffffu, amax);
+  if (TPI > 32) {
+    __shared__ uint32_t red[TPI / 32];
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+    __syncthreads();  // also: every thread has read the old scale
+#pragma unroll
+    for (int i = 0; i < TPI / 32; ++i) amax = max(amax, red[i]);
+  }
+  const float want = kv8_scale_of<CODE>(amax), now = w.held > 0 ? kv8_scale_max(was, want) : want;
+  if (TPI == 32) __syncwarp();
+  if (lane == 0) *sp = now;
+  uint8_t* const row0 = kv8_row(pl, w.page, h, w.in_page);
+  if (w.held > 0 && was < now) {
+    const float ratio = was / now;
+    for (int e = lane; e < w.held * pr; e += TPI) {
+      uint2* q = reinterpret_cast<uint2*>(row0 + (e / pr) * pl.sc[2] + (e % pr) * 8);
+      uint2 t = *q;
+      t.x = kv8_rescale4<CODE>(t.x, ratio);
+      t.y = kv8_rescale4<CODE>(t.y, ratio);
+      *q = t;
+    }
+  }
+  const float inv = now > 0.f ? 1.0f / now : 0.f;  // 0 for a NaN scale too: its codes are 0
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int e = lane + k * TPI;
+    if (e >= n) continue;
+    float f[8];
+    v[k].get(f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = inv > 0.f ? __fmul_rn(f[i], inv) : 0.f;
+    *reinterpret_cast<uint2*>(row0 + (w.held + e / pr) * pl.sc[2] + (e % pr) * 8) =
+        make_uint2(kv8_enc4<CODE>(f), kv8_enc4<CODE>(f + 4));
+  }
+}
+
+// Any layout and size: one CTA per item, the rows read twice.
 template <typename T, int CODE>
 __global__ void __launch_bounds__(128) kv8_write_kernel(const Kv8WriteParams p) {
   const Kv8View& c = p.c;
-  int lo = 0, hi = c.num_seqs - 1;
-  const int64_t item = blockIdx.x;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (kv8_item_base(p, mid) <= item) lo = mid; else hi = mid - 1;
-  }
-  const int s = lo, h = blockIdx.y;
-  const int64_t tok0 = p.cu ? p.cu[s] : s;
-  const int64_t n = p.cu ? p.cu[s + 1] - tok0 : 1;
-  const int64_t start = p.start_lens[s];
-  const int64_t first = (start / c.group + (item - kv8_item_base(p, s))) * c.group;  // the group's first position
-  if (n <= 0 || start < 0 || first >= start + n) return;
-  const int64_t page = kv8_page(c, s, first);
-  if (page < 0) return;
-  const int64_t r0 = max(start, first), r1 = min(start + n, first + c.group);
-  const int in_page = static_cast<int>(first % c.P);
-  const Kv8Plane& pl = c.plane[blockIdx.z];
-  const T* x = static_cast<const T*>(p.x[blockIdx.z]) + (tok0 + (r0 - start)) * p.sx[blockIdx.z][0] +
-               h * p.sx[blockIdx.z][1];
-  const int64_t st = p.sx[blockIdx.z][0], sd = p.sx[blockIdx.z][2];
-  const int held = static_cast<int>(r0 - first), fresh = static_cast<int>(r1 - r0), D = c.D;
-
+  const int h = blockIdx.y, which = blockIdx.z, D = c.D;
+  Kv8WriteItem w;
+  if (!kv8_write_item(p, blockIdx.x, w)) return;
+  const Kv8Plane& pl = c.plane[which];
+  const T* x = static_cast<const T*>(p.x[which]) + w.token * p.sx[which][0] + h * p.sx[which][1];
+  const int64_t st = p.sx[which][0], sd = p.sx[which][2];
   uint32_t amax = 0;
-  for (int e = threadIdx.x; e < fresh * D; e += 128)
+  for (int e = threadIdx.x; e < w.fresh * D; e += 128)
     amax = max(amax, abs_bits(Elem<T>::to_f(x[(e / D) * st + (e % D) * sd])));
   __shared__ uint32_t red[4];
   amax = __reduce_max_sync(0xffffffffu, amax);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
-  __syncthreads();
-  amax = max(max(red[0], red[1]), max(red[2], red[3]));
-  float* sp = kv8_scale(pl, page, h, in_page / c.group);
-  const float was = *sp, want = kv8_scale_of<CODE>(amax);
-  const float now = held > 0 ? kv8_scale_max(was, want) : want;
+  float* sp = kv8_scale(pl, w.page, h, w.in_page / c.group);
+  const float was = *sp;
   __syncthreads();  // every thread has read the old scale
+  amax = max(max(red[0], red[1]), max(red[2], red[3]));
+  const float want = kv8_scale_of<CODE>(amax), now = w.held > 0 ? kv8_scale_max(was, want) : want;
   if (threadIdx.x == 0) *sp = now;
-  if (held > 0 && was < now) {
+  if (w.held > 0 && was < now) {
     const float ratio = was / now;
-    for (int e = threadIdx.x; e < held * D; e += 128) {
-      uint8_t* q = kv8_row(pl, page, h, in_page + e / D) + (e % D) * pl.sc[3];
+    for (int e = threadIdx.x; e < w.held * D; e += 128) {
+      uint8_t* q = kv8_row(pl, w.page, h, w.in_page + e / D) + (e % D) * pl.sc[3];
       *q = Kv8<CODE>::enc(Kv8<CODE>::dec(*q) * ratio);
     }
   }
-  const float inv = now > 0.f ? 1.0f / now : 0.f;  // 0 for a NaN scale too: its codes are 0
-  for (int e = threadIdx.x; e < fresh * D; e += 128) {
+  const float inv = now > 0.f ? 1.0f / now : 0.f;
+  for (int e = threadIdx.x; e < w.fresh * D; e += 128) {
     const float v = Elem<T>::to_f(x[(e / D) * st + (e % D) * sd]) * inv;
-    kv8_row(pl, page, h, in_page + held + e / D)[(e % D) * pl.sc[3]] = inv > 0.f ? Kv8<CODE>::enc(v) : 0;
+    kv8_row(pl, w.page, h, w.in_page + w.held + e / D)[(e % D) * pl.sc[3]] = inv > 0.f ? Kv8<CODE>::enc(v) : 0;
   }
+}
+
+// rows of codes in whole aligned pieces of n codes
+static bool codes_vec_ok(const Kv8View& c, int n) {
+  if (c.D % n) return false;
+  for (const Kv8Plane& pl : c.plane)
+    if (pl.sc[3] != 1 || (reinterpret_cast<uintptr_t>(pl.code) & (n - 1)) || ((pl.sc[0] | pl.sc[1] | pl.sc[2]) & (n - 1))) return false;
+  return true;
+}
+// rows of T in 16-byte pieces
+static bool rows_vec_ok(const void* x, const int64_t* st, int size) {
+  const int n = 16 / size;
+  return st[2] == 1 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ((st[0] | st[1]) & (n - 1)) == 0;
 }
 
 int kv8_write_launch(const Kv8View& c, int code_type, const void* k, const int64_t* sk, const void* v,
@@ -88,8 +216,22 @@ int kv8_write_launch(const Kv8View& c, int code_type, const void* k, const int64
   p.start_lens = start_lens;
   p.cu = cu;
   p.total = total;
-  const dim3 grid(static_cast<unsigned>(total / c.group + 2 * static_cast<int64_t>(c.num_seqs)), c.Hkv, 2);
+  const int64_t items = cu ? total / c.group + 2 * static_cast<int64_t>(c.num_seqs) : c.num_seqs;
+  const int size = dtype == kF32 ? 4 : 2;
   note_kernel("kv8_write");
+  const int pieces = c.group * (c.D / 8);  // of eight elements; a thread holds up to eight
+  if (codes_vec_ok(c, 8) && rows_vec_ok(k, sk, size) && rows_vec_ok(v, sv, size) && pieces <= 8 * 512 &&
+      items * c.Hkv * 2 < (int64_t{1} << 31)) {
+    const int64_t units = items * c.Hkv * 2;
+    const unsigned warps = static_cast<unsigned>((units + 3) / 4), ctas = static_cast<unsigned>(units);
+    TAK_BY_DTYPE(dtype, TAK_BY_CODE(code_type, {
+      if (pieces <= 8 * 32) kv8_write_vec_kernel<T, CODE, 32><<<warps, 128, 0, st>>>(p, items);
+      else if (pieces <= 8 * 128) kv8_write_vec_kernel<T, CODE, 128><<<ctas, 128, 0, st>>>(p, items);
+      else kv8_write_vec_kernel<T, CODE, 512><<<ctas, 512, 0, st>>>(p, items);
+    }));
+    return 0;
+  }
+  const dim3 grid(static_cast<unsigned>(items), c.Hkv, 2);
   TAK_BY_DTYPE(dtype, TAK_BY_CODE(code_type, kv8_write_kernel<T, CODE><<<grid, 128, 0, st>>>(p)));
   return 0;
 }
@@ -102,23 +244,68 @@ struct Kv8ReadParams {
   int64_t total;
 };
 
-template <typename T, int CODE>
-__global__ void __launch_bounds__(128) kv8_read_kernel(const Kv8ReadParams p) {
+// TB tokens a CTA: their pages are looked up once, then every thread converts
+// pieces of VEC codes (16: one load, 32 bytes of 16-bit values or 64 of fp32 out),
+// in the order of the output.
+template <typename T, int CODE, int VEC>
+__global__ void __launch_bounds__(256) kv8_read_kernel(const __grid_constant__ Kv8ReadParams p, int TB) {
   const Kv8View& c = p.c;
-  const int t = blockIdx.x;
-  if (c.num_seqs == 0) return;
-  const int s = find_slot_seq(p.cu, c.num_seqs, t);
-  const bool in_seq = t >= p.cu[s] && t < p.cu[s + 1];
-  const int64_t pos = in_seq ? t - p.cu[s] + (p.start_lens ? p.start_lens[s] : 0) : -1;
-  const int64_t page = kv8_page(c, s, pos);
-  const int row = page >= 0 ? static_cast<int>(pos % c.P) : 0;
-  for (int e = threadIdx.x; e < 2 * c.Hkv * c.D; e += 128) {
-    const int w = e / (c.Hkv * c.D), h = e / c.D % c.Hkv, d = e % c.D;
+  __shared__ int64_t s_page[16];
+  __shared__ int s_row[16];
+  const int t0 = blockIdx.x * TB, tn = static_cast<int>(min(static_cast<int64_t>(TB), p.total - t0));
+  if (threadIdx.x < tn) {
+    const int t = t0 + threadIdx.x;
+    const int s = find_slot_seq(p.cu, c.num_seqs, t);
+    const bool in_seq = t >= p.cu[s] && t < p.cu[s + 1];
+    const int64_t pos = in_seq ? t - p.cu[s] + (p.start_lens ? p.start_lens[s] : 0) : -1;
+    const int64_t page = kv8_page(c, s, pos);
+    s_page[threadIdx.x] = page;
+    s_row[threadIdx.x] = page >= 0 ? static_cast<int>(pos % c.P) : 0;
+  }
+  __syncthreads();
+  const int pr = c.D / VEC, per_tok = c.Hkv * pr, n = tn * per_tok;
+#pragma unroll 1
+  for (int w = 0; w < 2; ++w) {
     const Kv8Plane& pl = c.plane[w];
-    float v = 0.f;
-    if (page >= 0)
-      v = Kv8<CODE>::dec(kv8_row(pl, page, h, row)[d * pl.sc[3]]) * *kv8_scale(pl, page, h, row / c.group);
-    static_cast<T*>(p.y[w])[t * p.sy[w][0] + h * p.sy[w][1] + d * p.sy[w][2]] = Elem<T>::from_f(v);
+    T* const y = static_cast<T*>(p.y[w]);
+    const int64_t y0 = p.sy[w][0], y1 = p.sy[w][1], y2 = VEC > 1 ? 1 : p.sy[w][2];
+#pragma unroll 4
+    for (int e = threadIdx.x; e < n; e += 256) {
+      const int ti = e / per_tok, e1 = e - ti * per_tok, h = e1 / pr, d = (e1 - h * pr) * VEC;
+      const int64_t page = s_page[ti];
+      const int row = s_row[ti];
+      T* out = y + (t0 + ti) * y0 + h * y1 + d * y2;
+      if (VEC == 16) {
+        uint4 q = make_uint4(0, 0, 0, 0);
+        float sc = 0.f;
+        if (page >= 0) {
+          q = __ldg(reinterpret_cast<const uint4*>(kv8_row(pl, page, h, row) + d));
+          sc = *kv8_scale(pl, page, h, row / c.group);
+        }
+        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+        float f[16];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) kv8_dec4<CODE>(page >= 0 ? u[k] : 0u, f + 4 * k);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) f[k] *= sc;
+        if constexpr (sizeof(T) == 2) {
+          uint32_t o[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o[k] = Elem<T>::pack2(f[2 * k], f[2 * k + 1]);
+          reinterpret_cast<uint4*>(out)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+          reinterpret_cast<uint4*>(out)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            reinterpret_cast<float4*>(out)[k] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+        }
+      } else {
+        float v = 0.f;
+        if (page >= 0)
+          v = Kv8<CODE>::dec(kv8_row(pl, page, h, row)[d * pl.sc[3]]) * *kv8_scale(pl, page, h, row / c.group);
+        *out = Elem<T>::from_f(v);
+      }
+    }
   }
 }
 
@@ -131,8 +318,16 @@ int kv8_read_launch(const Kv8View& c, int code_type, const int32_t* cu, const in
   p.start_lens = start_lens;
   p.cu = cu;
   p.total = total;
+  const int size = dtype == kF32 ? 4 : 2;
+  const bool vec = codes_vec_ok(c, 16) && rows_vec_ok(k, sk, size) && rows_vec_ok(v, sv, size);
+  // tokens of a CTA: fewer where 16 would leave SMs without one
+  const int tb = total >= 16 * 4 * num_sms() ? 16 : total >= 4 * 2 * num_sms() ? 4 : 2;
+  const unsigned grid = static_cast<unsigned>((total + tb - 1) / tb);
   note_kernel("kv8_read");
-  TAK_BY_DTYPE(dtype, TAK_BY_CODE(code_type, kv8_read_kernel<T, CODE><<<static_cast<unsigned>(total), 128, 0, st>>>(p)));
+  TAK_BY_DTYPE(dtype, TAK_BY_CODE(code_type, {
+    if (vec) kv8_read_kernel<T, CODE, 16><<<grid, 256, 0, st>>>(p, tb);
+    else kv8_read_kernel<T, CODE, 1><<<grid, 256, 0, st>>>(p, tb);
+  }));
   return 0;
 }
 

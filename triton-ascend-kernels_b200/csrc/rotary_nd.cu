@@ -33,33 +33,107 @@ __device__ __forceinline__ float2 rotary_cos_sin(const RotaryParams& p, int t, i
   return make_float2(c, p.inverse ? -s : s);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) rotary_nd_kernel(const RotaryParams p) {
-  extern __shared__ float2 table[];  // [rot / 2]
-  const int t = blockIdx.x, half = p.rot / 2, rest = p.D - p.rot;
-  for (int i = threadIdx.x; i < half; i += blockDim.x) table[i] = rotary_cos_sin(p, t, i);
+// A CTA turns TB tokens (and, for few tokens, a share of their heads): the table
+// of TB * rot / 2 cosines and sines is made once and used by every head.  VEC = 16
+// bytes per access where layout allows, else one element.
+template <typename T, int VEC> struct RotVec;
+template <typename T> struct RotVec<T, 1> {
+  T e[1];
+};
+template <typename T> struct alignas(16) RotVec<T, 16 / sizeof(T)> {
+  T e[16 / sizeof(T)];
+};
+
+template <typename T, int VEC, bool IL>
+__global__ void __launch_bounds__(256) rotary_nd_kernel(const __grid_constant__ RotaryParams p, int TB, int heads_per_cta) {
+  using V = RotVec<T, VEC>;
+  extern __shared__ float2 table[];  // [TB][rot / 2]
+  const int t0 = blockIdx.x * TB, tn = min(TB, p.T - t0);
+  const int h0 = blockIdx.y * heads_per_cta, hn = min(heads_per_cta, p.H + p.Hkv - h0);
+  const int half = p.rot / 2;
+  // items of a head: pieces of VEC pairs (half-split: two vectors; interleaved:
+  // VEC / 2 pairs in one vector), then the vectors that pass through
+  const int turn = IL && VEC > 1 ? p.rot / VEC : half / VEC, rest = (p.D - p.rot) / VEC, per_head = turn + rest;
+  const int n = tn * hn * per_head;
+  for (int i = threadIdx.x; i < tn * half; i += 256) table[i] = rotary_cos_sin(p, t0 + i / half, i % half);
   __syncthreads();
-  const int per_head = half + rest;
-  const int n = (p.H + p.Hkv) * per_head;
-  for (int e = threadIdx.x; e < n; e += blockDim.x) {
-    int h = e / per_head;
-    const int i = e - h * per_head;
+  const int per_tok = hn * per_head;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < n; e += 256) {
+    const int ti = e / per_tok, e1 = e - ti * per_tok;
+    const int hi = e1 / per_head, i = e1 - hi * per_head;
+    int h = h0 + hi;
     const int w = h >= p.H;
     if (w) h -= p.H;
+    const int64_t t = t0 + ti;
     const T* x = static_cast<const T*>(p.x[w]) + t * p.sx[w][0] + h * p.sx[w][1];
     T* y = static_cast<T*>(p.y[w]) + t * p.sy[w][0] + h * p.sy[w][1];
-    const int64_t dx = p.sx[w][2], dy = p.sy[w][2];
-    if (i < half) {
-      const int a = p.interleaved ? 2 * i : i, b = p.interleaved ? 2 * i + 1 : i + half;
-      const float u = Elem<T>::to_f(x[a * dx]), v = Elem<T>::to_f(x[b * dx]);
-      const float2 cs = table[i];
-      y[a * dy] = Elem<T>::from_f(u * cs.x - v * cs.y);
-      y[b * dy] = Elem<T>::from_f(u * cs.y + v * cs.x);
+    const int64_t dx = VEC > 1 ? 1 : p.sx[w][2], dy = VEC > 1 ? 1 : p.sy[w][2];
+    const float2* cs = table + ti * half;
+    if (i >= turn) {
+      const int d = p.rot + (i - turn) * VEC;
+      *reinterpret_cast<V*>(y + d * dy) = *reinterpret_cast<const V*>(x + d * dx);
+    } else if (IL && VEC > 1) {
+      V v = *reinterpret_cast<const V*>(x + i * VEC);
+#pragma unroll
+      for (int k = 0; k < VEC / 2; ++k) {
+        const float2 c = cs[i * (VEC / 2) + k];
+        const float a = Elem<T>::to_f(v.e[(2 * k) % VEC]), b = Elem<T>::to_f(v.e[(2 * k + 1) % VEC]);
+        v.e[(2 * k) % VEC] = Elem<T>::from_f(a * c.x - b * c.y);
+        v.e[(2 * k + 1) % VEC] = Elem<T>::from_f(a * c.y + b * c.x);
+      }
+      *reinterpret_cast<V*>(y + i * VEC) = v;
     } else {
-      const int d = p.rot + i - half;
-      y[d * dy] = x[d * dx];
+      const int da = IL ? 2 * i : i * VEC, db = IL ? 2 * i + 1 : i * VEC + half;
+      V a = *reinterpret_cast<const V*>(x + da * dx), b = *reinterpret_cast<const V*>(x + db * dx);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const float2 c = cs[i * VEC + k];
+        const float u = Elem<T>::to_f(a.e[k]), v = Elem<T>::to_f(b.e[k]);
+        a.e[k] = Elem<T>::from_f(u * c.x - v * c.y);
+        b.e[k] = Elem<T>::from_f(u * c.y + v * c.x);
+      }
+      *reinterpret_cast<V*>(y + da * dy) = a;
+      *reinterpret_cast<V*>(y + db * dy) = b;
     }
   }
+}
+
+// 16-byte accesses: unit element strides, rows and base on 16 bytes, and the
+// parts of a head (both halves, or the pairs; what passes through) whole vectors.
+static bool rotary_vec_ok(const RotaryArgs& a, int vec) {
+  const int part = a.interleaved ? a.rot_dim : a.rot_dim / 2;
+  if (part % vec || (a.head_dim - a.rot_dim) % vec) return false;
+  const int64_t* st[] = {a.sq, a.sqo, a.sk, a.sko};
+  const void* base[] = {a.q, a.q_out, a.k, a.k_out};
+  for (int i = 0; i < 4; ++i) {
+    if ((i < 2 ? a.num_q_heads : a.num_kv_heads) == 0) continue;
+    if (st[i][2] != 1 || st[i][0] % vec || st[i][1] % vec || (reinterpret_cast<uintptr_t>(base[i]) & 15)) return false;
+  }
+  return true;
+}
+
+template <typename T>
+static void rotary_launch_t(const RotaryArgs& a, const RotaryParams& p, cudaStream_t st) {
+  constexpr int VEC = 16 / sizeof(T);
+  const bool vec = rotary_vec_ok(a, VEC);
+  const int heads = a.num_q_heads + a.num_kv_heads, half = a.rot_dim / 2;
+  // tokens of a CTA: about one table entry a thread; fewer tokens than that fills
+  // the GPU with CTAs over shares of the heads instead
+  int tb = half > 0 ? (256 + half - 1) / half : 4;
+  if (tb > 8) tb = 8;
+  const int want = 2 * num_sms();
+  while (tb > 1 && (a.total_tokens + tb - 1) / tb < want) tb = (tb + 1) / 2;
+  const int blocks = (a.total_tokens + tb - 1) / tb;
+  int split = blocks < want ? (want + blocks - 1) / blocks : 1;
+  if (split > (heads + 3) / 4) split = (heads + 3) / 4;
+  const int per = (heads + split - 1) / split;
+  const dim3 grid(blocks, (heads + per - 1) / per);
+  const size_t smem = static_cast<size_t>(tb) * half * sizeof(float2);
+  if (vec && a.interleaved) rotary_nd_kernel<T, VEC, true><<<grid, 256, smem, st>>>(p, tb, per);
+  else if (vec) rotary_nd_kernel<T, VEC, false><<<grid, 256, smem, st>>>(p, tb, per);
+  else if (a.interleaved) rotary_nd_kernel<T, 1, true><<<grid, 256, smem, st>>>(p, tb, per);
+  else rotary_nd_kernel<T, 1, false><<<grid, 256, smem, st>>>(p, tb, per);
 }
 
 int rotary_nd_launch(const RotaryArgs& a, cudaStream_t st) {
@@ -74,11 +148,10 @@ int rotary_nd_launch(const RotaryArgs& a, cudaStream_t st) {
   for (int i = 0; i < a.axes; ++i) p.section_end[i] = a.section_end[i];
   p.axes = a.axes; p.T = a.total_tokens; p.H = a.num_q_heads; p.Hkv = a.num_kv_heads;
   p.D = a.head_dim; p.rot = a.rot_dim; p.interleaved = a.interleaved; p.inverse = a.inverse;
-  const size_t smem = static_cast<size_t>(a.rot_dim / 2) * sizeof(float2);
   note_kernel("rotary_nd");
-  if (a.dtype == kBF16) rotary_nd_kernel<__nv_bfloat16><<<a.total_tokens, 256, smem, st>>>(p);
-  else if (a.dtype == kF16) rotary_nd_kernel<__half><<<a.total_tokens, 256, smem, st>>>(p);
-  else rotary_nd_kernel<float><<<a.total_tokens, 256, smem, st>>>(p);
+  if (a.dtype == kBF16) rotary_launch_t<__nv_bfloat16>(a, p, st);
+  else if (a.dtype == kF16) rotary_launch_t<__half>(a, p, st);
+  else rotary_launch_t<float>(a, p, st);
   return 0;
 }
 
