@@ -35,11 +35,16 @@ struct Kv8WriteItem {
 };
 __device__ __forceinline__ bool kv8_write_item(const Kv8WriteParams& p, int64_t item, Kv8WriteItem& w) {
   const Kv8View& c = p.c;
-  int lo = 0, hi = c.num_seqs - 1;
+  int lo = 0;
   if (p.cu) {
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (kv8_item_base(p, mid) <= item) lo = mid; else hi = mid - 1;
+    // last sequence whose items begin at or before `item`, 32 candidates a round
+    // (every lane of the warp looks at the same item)
+    for (int span = c.num_seqs; span > 1;) {
+      const int step = (span + 31) / 32, s = lo + static_cast<int>(threadIdx.x & 31) * step;
+      const unsigned le = __ballot_sync(0xffffffffu, s < c.num_seqs && s < lo + span && kv8_item_base(p, s) <= item);
+      const int at = 31 - __clz(le | 1u);
+      span = min(step, span - at * step);
+      lo += at * step;
     }
   } else {
     lo = static_cast<int>(item);
@@ -93,67 +98,88 @@ __global__ void __launch_bounds__(TPI == 32 ? 128 : TPI) kv8_write_vec_kernel(co
   constexpr int U = 8;
   const Kv8View& c = p.c;
   const int lane = threadIdx.x % TPI;
-  // heads and planes of an item are neighbours: they read the same rows
+  // the heads of an item are neighbours: they read the same rows
   int64_t id = TPI == 32 ? static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32 : blockIdx.x;
-  const int which = static_cast<int>(id & 1);
-  id >>= 1;
   const int h = static_cast<int>(id % c.Hkv);
   id /= c.Hkv;
   Kv8WriteItem w;
   if (id >= items || !kv8_write_item(p, id, w)) return;
-  const Kv8Plane& pl = c.plane[which];
-  const T* x = static_cast<const T*>(p.x[which]) + w.token * p.sx[which][0] + h * p.sx[which][1];
   const int pr = c.D / 8, n = w.fresh * pr;  // pieces of a row, of the item
-  Eight<T> v[U];
+  // piece k of this thread: row and piece of it (one division where the threads
+  // cover whole rows)
+  const int lr = lane / pr, lc = lane - lr * pr, step = TPI / pr;
+  const bool whole = step * pr == TPI;
+  auto place = [&](int k, int& r, int& d) {
+    r = whole ? lr + k * step : (lane + k * TPI) / pr;
+    d = (whole ? lc : (lane + k * TPI) - r * pr) * 8;
+  };
+  Eight<T> v[2][U];
+  float* sp[2];
+  float was[2];
 #pragma unroll
-  for (int k = 0; k < U; ++k) {
-    const int e = lane + k * TPI;
-    if (e < n) v[k].load(x + (e / pr) * p.sx[which][0] + (e % pr) * 8);
-  }
-  float* sp = kv8_scale(pl, w.page, h, w.in_page / c.group);
-  const float was = *sp;
-  uint32_t amax = 0;
+  for (int which = 0; which < 2; ++which) {  // K and V in flight together
+    const T* x = static_cast<const T*>(p.x[which]) + w.token * p.sx[which][0] + h * p.sx[which][1];
+    sp[which] = kv8_scale(c.plane[which], w.page, h, w.in_page / c.group);
+    was[which] = *sp[which];
 #pragma unroll
-  for (int k = 0; k < U; ++k)
-    if (lane + k * TPI < n) {
-      float f[8];
-      v[k].get(f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) amax = max(amax, abs_bits(f[i]));
+    for (int k = 0; k < U; ++k) {
+      int r, d;
+      place(k, r, d);
+      if (lane + k * TPI < n) v[which][k].load(x + r * p.sx[which][0] + d);
     }
-  amax = __reduce_max_sync(0xffffffffu, amax);
+  }
+  uint32_t amax[2] = {0, 0};
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (lane + k * TPI < n) {
+        float f[8];
+        v[which][k].get(f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax[which] = max(amax[which], abs_bits(f[i]));
+      }
+    amax[which] = __reduce_max_sync(0xffffffffu, amax[which]);
+  }
   if (TPI > 32) {
-    __shared__ uint32_t red[TPI / 32];
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
-    __syncthreads();  // also: every thread has read the old scale
+    __shared__ uint2 red[TPI / 32];
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_uint2(amax[0], amax[1]);
+    __syncthreads();  // also: every thread has read the old scales
 #pragma unroll
-    for (int i = 0; i < TPI / 32; ++i) amax = max(amax, red[i]);
-  }
-  const float want = kv8_scale_of<CODE>(amax), now = w.held > 0 ? kv8_scale_max(was, want) : want;
-  if (TPI == 32) __syncwarp();
-  if (lane == 0) *sp = now;
-  uint8_t* const row0 = kv8_row(pl, w.page, h, w.in_page);
-  if (w.held > 0 && was < now) {
-    const float ratio = was / now;
-    for (int e = lane; e < w.held * pr; e += TPI) {
-      uint2* q = reinterpret_cast<uint2*>(row0 + (e / pr) * pl.sc[2] + (e % pr) * 8);
-      uint2 t = *q;
-      t.x = kv8_rescale4<CODE>(t.x, ratio);
-      t.y = kv8_rescale4<CODE>(t.y, ratio);
-      *q = t;
+    for (int i = 0; i < TPI / 32; ++i) {
+      amax[0] = max(amax[0], red[i].x);
+      amax[1] = max(amax[1], red[i].y);
     }
   }
-  const float inv = now > 0.f ? 1.0f / now : 0.f;  // 0 for a NaN scale too: its codes are 0
+  __syncwarp();
 #pragma unroll
-  for (int k = 0; k < U; ++k) {
-    const int e = lane + k * TPI;
-    if (e >= n) continue;
-    float f[8];
-    v[k].get(f);
+  for (int which = 0; which < 2; ++which) {
+    const Kv8Plane& pl = c.plane[which];
+    const float want = kv8_scale_of<CODE>(amax[which]), now = w.held > 0 ? kv8_scale_max(was[which], want) : want;
+    if (lane == 0) *sp[which] = now;
+    uint8_t* const row0 = kv8_row(pl, w.page, h, w.in_page);
+    if (w.held > 0 && was[which] < now) {
+      const float ratio = was[which] / now;
+      for (int e = lane; e < w.held * pr; e += TPI) {
+        uint2* q = reinterpret_cast<uint2*>(row0 + (e / pr) * pl.sc[2] + (e % pr) * 8);
+        uint2 t = *q;
+        t.x = kv8_rescale4<CODE>(t.x, ratio);
+        t.y = kv8_rescale4<CODE>(t.y, ratio);
+        *q = t;
+      }
+    }
+    const float inv = now > 0.f ? 1.0f / now : 0.f;  // 0 for a NaN scale too: its codes are 0
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = inv > 0.f ? __fmul_rn(f[i], inv) : 0.f;
-    *reinterpret_cast<uint2*>(row0 + (w.held + e / pr) * pl.sc[2] + (e % pr) * 8) =
-        make_uint2(kv8_enc4<CODE>(f), kv8_enc4<CODE>(f + 4));
+    for (int k = 0; k < U; ++k) {
+      if (lane + k * TPI >= n) continue;
+      float f[8];
+      v[which][k].get(f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = inv > 0.f ? __fmul_rn(f[i], inv) : 0.f;
+      int r, d;
+      place(k, r, d);
+      *reinterpret_cast<uint2*>(row0 + (w.held + r) * pl.sc[2] + d) = make_uint2(kv8_enc4<CODE>(f), kv8_enc4<CODE>(f + 4));
+    }
   }
 }
 
@@ -221,8 +247,8 @@ int kv8_write_launch(const Kv8View& c, int code_type, const void* k, const int64
   note_kernel("kv8_write");
   const int pieces = c.group * (c.D / 8);  // of eight elements; a thread holds up to eight
   if (codes_vec_ok(c, 8) && rows_vec_ok(k, sk, size) && rows_vec_ok(v, sv, size) && pieces <= 8 * 512 &&
-      items * c.Hkv * 2 < (int64_t{1} << 31)) {
-    const int64_t units = items * c.Hkv * 2;
+      items * c.Hkv < (int64_t{1} << 31)) {
+    const int64_t units = items * c.Hkv;  // K and V together
     const unsigned warps = static_cast<unsigned>((units + 3) / 4), ctas = static_cast<unsigned>(units);
     TAK_BY_DTYPE(dtype, TAK_BY_CODE(code_type, {
       if (pieces <= 8 * 32) kv8_write_vec_kernel<T, CODE, 32><<<warps, 128, 0, st>>>(p, items);
@@ -245,13 +271,12 @@ struct Kv8ReadParams {
 };
 
 // TB tokens a CTA: their pages are looked up once, then every thread converts
-// pieces of VEC codes (16: one load, 32 bytes of 16-bit values or 64 of fp32 out),
-// in the order of the output.
+// pieces of VEC codes (16: one load, 32 bytes of 16-bit values or 64 of fp32 out).
 template <typename T, int CODE, int VEC>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const __grid_constant__ Kv8ReadParams p, int TB) {
   const Kv8View& c = p.c;
   __shared__ int64_t s_page[16];
-  __shared__ int s_row[16];
+  __shared__ int s_row[16], s_group[16];
   const int t0 = blockIdx.x * TB, tn = static_cast<int>(min(static_cast<int64_t>(TB), p.total - t0));
   if (threadIdx.x < tn) {
     const int t = t0 + threadIdx.x;
@@ -261,49 +286,56 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const __grid_constant__ K
     const int64_t page = kv8_page(c, s, pos);
     s_page[threadIdx.x] = page;
     s_row[threadIdx.x] = page >= 0 ? static_cast<int>(pos % c.P) : 0;
+    s_group[threadIdx.x] = s_row[threadIdx.x] / c.group;
   }
   __syncthreads();
-  const int pr = c.D / VEC, per_tok = c.Hkv * pr, n = tn * per_tok;
-#pragma unroll 1
-  for (int w = 0; w < 2; ++w) {
-    const Kv8Plane& pl = c.plane[w];
-    T* const y = static_cast<T*>(p.y[w]);
-    const int64_t y0 = p.sy[w][0], y1 = p.sy[w][1], y2 = VEC > 1 ? 1 : p.sy[w][2];
+  // a thread keeps its piece of a token (head and columns) and walks the tokens
+  const int pr = c.D / VEC, per_tok = c.Hkv * pr;
+  const int px = per_tok < 256 ? per_tok : 256, lanes = 256 / px;
+  const int tl = threadIdx.x / px;
+  if (tl >= lanes) return;
+  for (int e = threadIdx.x - tl * px; e < per_tok; e += px) {
+    const int h = e / pr, d = (e - h * pr) * VEC;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const Kv8Plane& pl = c.plane[w];
+      T* const y = static_cast<T*>(p.y[w]) + h * p.sy[w][1] + d * (VEC > 1 ? 1 : p.sy[w][2]);
+      const uint8_t* const code = pl.code + h * pl.sc[1] + d * (VEC > 1 ? 1 : pl.sc[3]);
+      const float* const scale = pl.scale + h * pl.ss[1];
 #pragma unroll 4
-    for (int e = threadIdx.x; e < n; e += 256) {
-      const int ti = e / per_tok, e1 = e - ti * per_tok, h = e1 / pr, d = (e1 - h * pr) * VEC;
-      const int64_t page = s_page[ti];
-      const int row = s_row[ti];
-      T* out = y + (t0 + ti) * y0 + h * y1 + d * y2;
-      if (VEC == 16) {
-        uint4 q = make_uint4(0, 0, 0, 0);
-        float sc = 0.f;
-        if (page >= 0) {
-          q = __ldg(reinterpret_cast<const uint4*>(kv8_row(pl, page, h, row) + d));
-          sc = *kv8_scale(pl, page, h, row / c.group);
-        }
-        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-        float f[16];
+      for (int ti = tl; ti < tn; ti += lanes) {
+        const int64_t page = s_page[ti];
+        const int row = s_row[ti];
+        T* const out = y + (t0 + ti) * p.sy[w][0];
+        if (VEC == 16) {
+          uint4 q = make_uint4(0, 0, 0, 0);
+          float sc = 0.f;
+          if (page >= 0) {
+            q = *reinterpret_cast<const uint4*>(code + page * pl.sc[0] + row * pl.sc[2]);
+            sc = scale[page * pl.ss[0] + s_group[ti] * pl.ss[2]];
+          }
+          const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+          float f[16];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) kv8_dec4<CODE>(page >= 0 ? u[k] : 0u, f + 4 * k);
+          for (int k = 0; k < 4; ++k) kv8_dec4<CODE>(u[k], f + 4 * k);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) f[k] *= sc;
-        if constexpr (sizeof(T) == 2) {
-          uint32_t o[8];
+          for (int k = 0; k < 16; ++k) f[k] *= sc;
+          if constexpr (sizeof(T) == 2) {
+            uint32_t o[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o[k] = Elem<T>::pack2(f[2 * k], f[2 * k + 1]);
-          reinterpret_cast<uint4*>(out)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-          reinterpret_cast<uint4*>(out)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+            for (int k = 0; k < 8; ++k) o[k] = Elem<T>::pack2(f[2 * k], f[2 * k + 1]);
+            reinterpret_cast<uint4*>(out)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            reinterpret_cast<uint4*>(out)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              reinterpret_cast<float4*>(out)[k] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+          }
         } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            reinterpret_cast<float4*>(out)[k] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+          float v = 0.f;
+          if (page >= 0) v = Kv8<CODE>::dec(code[page * pl.sc[0] + row * pl.sc[2]]) * scale[page * pl.ss[0] + s_group[ti] * pl.ss[2]];
+          *out = Elem<T>::from_f(v);
         }
-      } else {
-        float v = 0.f;
-        if (page >= 0)
-          v = Kv8<CODE>::dec(kv8_row(pl, page, h, row)[d * pl.sc[3]]) * *kv8_scale(pl, page, h, row / c.group);
-        *out = Elem<T>::from_f(v);
       }
     }
   }

@@ -34,8 +34,9 @@ __device__ __forceinline__ float2 rotary_cos_sin(const RotaryParams& p, int t, i
 }
 
 // A CTA turns TB tokens (and, for few tokens, a share of their heads): the table
-// of TB * rot / 2 cosines and sines is made once and used by every head.  VEC = 16
-// bytes per access where layout allows, else one element.
+// of TB * rot / 2 cosines and sines is made once; each thread then keeps the ones
+// of its piece of a head in registers and walks the heads.  VEC = 16 bytes per
+// access where the layout allows, else one element.
 template <typename T, int VEC> struct RotVec;
 template <typename T> struct RotVec<T, 1> {
   T e[1];
@@ -54,47 +55,53 @@ __global__ void __launch_bounds__(256) rotary_nd_kernel(const __grid_constant__ 
   // items of a head: pieces of VEC pairs (half-split: two vectors; interleaved:
   // VEC / 2 pairs in one vector), then the vectors that pass through
   const int turn = IL && VEC > 1 ? p.rot / VEC : half / VEC, rest = (p.D - p.rot) / VEC, per_head = turn + rest;
-  const int n = tn * hn * per_head;
   for (int i = threadIdx.x; i < tn * half; i += 256) table[i] = rotary_cos_sin(p, t0 + i / half, i % half);
   __syncthreads();
-  const int per_tok = hn * per_head;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < n; e += 256) {
-    const int ti = e / per_tok, e1 = e - ti * per_tok;
-    const int hi = e1 / per_head, i = e1 - hi * per_head;
-    int h = h0 + hi;
-    const int w = h >= p.H;
-    if (w) h -= p.H;
+  constexpr int NCS = VEC == 1 ? 1 : IL ? VEC / 2 : VEC;  // pairs of a piece
+  const int px = per_head < 256 ? per_head : 256, lanes = 256 / px;
+  const int hl = threadIdx.x / px;
+  if (hl >= lanes) return;
+  for (int ti = 0; ti < tn; ++ti) {
     const int64_t t = t0 + ti;
-    const T* x = static_cast<const T*>(p.x[w]) + t * p.sx[w][0] + h * p.sx[w][1];
-    T* y = static_cast<T*>(p.y[w]) + t * p.sy[w][0] + h * p.sy[w][1];
-    const int64_t dx = VEC > 1 ? 1 : p.sx[w][2], dy = VEC > 1 ? 1 : p.sy[w][2];
-    const float2* cs = table + ti * half;
-    if (i >= turn) {
-      const int d = p.rot + (i - turn) * VEC;
-      *reinterpret_cast<V*>(y + d * dy) = *reinterpret_cast<const V*>(x + d * dx);
-    } else if (IL && VEC > 1) {
-      V v = *reinterpret_cast<const V*>(x + i * VEC);
+    for (int i = threadIdx.x - hl * px; i < per_head; i += px) {
+      float2 cs[NCS];
+      if (i < turn) {
 #pragma unroll
-      for (int k = 0; k < VEC / 2; ++k) {
-        const float2 c = cs[i * (VEC / 2) + k];
-        const float a = Elem<T>::to_f(v.e[(2 * k) % VEC]), b = Elem<T>::to_f(v.e[(2 * k + 1) % VEC]);
-        v.e[(2 * k) % VEC] = Elem<T>::from_f(a * c.x - b * c.y);
-        v.e[(2 * k + 1) % VEC] = Elem<T>::from_f(a * c.y + b * c.x);
+        for (int k = 0; k < NCS; ++k) cs[k] = table[ti * half + i * NCS + k];
       }
-      *reinterpret_cast<V*>(y + i * VEC) = v;
-    } else {
-      const int da = IL ? 2 * i : i * VEC, db = IL ? 2 * i + 1 : i * VEC + half;
-      V a = *reinterpret_cast<const V*>(x + da * dx), b = *reinterpret_cast<const V*>(x + db * dx);
+      // first element of the piece, and of its partner half
+      const int da = i >= turn ? p.rot + (i - turn) * VEC : IL ? (VEC > 1 ? i * VEC : 2 * i) : i * VEC;
+      const int db = IL ? da + 1 : da + half;
+#pragma unroll 4
+      for (int hi = hl; hi < hn; hi += lanes) {
+        int h = h0 + hi;
+        const int w = h >= p.H;
+        if (w) h -= p.H;
+        const T* x = static_cast<const T*>(p.x[w]) + t * p.sx[w][0] + h * p.sx[w][1];
+        T* y = static_cast<T*>(p.y[w]) + t * p.sy[w][0] + h * p.sy[w][1];
+        const int64_t dx = VEC > 1 ? 1 : p.sx[w][2], dy = VEC > 1 ? 1 : p.sy[w][2];
+        V a = *reinterpret_cast<const V*>(x + da * dx);
+        if (i < turn) {
+          if (IL && VEC > 1) {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const float2 c = cs[i * VEC + k];
-        const float u = Elem<T>::to_f(a.e[k]), v = Elem<T>::to_f(b.e[k]);
-        a.e[k] = Elem<T>::from_f(u * c.x - v * c.y);
-        b.e[k] = Elem<T>::from_f(u * c.y + v * c.x);
+            for (int k = 0; k < VEC / 2; ++k) {
+              const float u = Elem<T>::to_f(a.e[(2 * k) % VEC]), v = Elem<T>::to_f(a.e[(2 * k + 1) % VEC]);
+              a.e[(2 * k) % VEC] = Elem<T>::from_f(u * cs[k % NCS].x - v * cs[k % NCS].y);
+              a.e[(2 * k + 1) % VEC] = Elem<T>::from_f(u * cs[k % NCS].y + v * cs[k % NCS].x);
+            }
+          } else {
+            V b = *reinterpret_cast<const V*>(x + db * dx);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+              const float u = Elem<T>::to_f(a.e[k]), v = Elem<T>::to_f(b.e[k]);
+              a.e[k] = Elem<T>::from_f(u * cs[k % NCS].x - v * cs[k % NCS].y);
+              b.e[k] = Elem<T>::from_f(u * cs[k % NCS].y + v * cs[k % NCS].x);
+            }
+            *reinterpret_cast<V*>(y + db * dy) = b;
+          }
+        }
+        *reinterpret_cast<V*>(y + da * dy) = a;
       }
-      *reinterpret_cast<V*>(y + da * dy) = a;
-      *reinterpret_cast<V*>(y + db * dy) = b;
     }
   }
 }
@@ -121,7 +128,7 @@ static void rotary_launch_t(const RotaryArgs& a, const RotaryParams& p, cudaStre
   // tokens of a CTA: about one table entry a thread; fewer tokens than that fills
   // the GPU with CTAs over shares of the heads instead
   int tb = half > 0 ? (256 + half - 1) / half : 4;
-  if (tb > 8) tb = 8;
+  if (tb > 4) tb = 4;
   const int want = 2 * num_sms();
   while (tb > 1 && (a.total_tokens + tb - 1) / tb < want) tb = (tb + 1) / 2;
   const int blocks = (a.total_tokens + tb - 1) / tb;
