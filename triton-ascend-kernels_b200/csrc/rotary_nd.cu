@@ -46,7 +46,7 @@ template <typename T> struct alignas(16) RotVec<T, 16 / sizeof(T)> {
 };
 
 template <typename T, int VEC, bool IL>
-__global__ void __launch_bounds__(256) rotary_nd_kernel(const __grid_constant__ RotaryParams p, int TB, int heads_per_cta) {
+__global__ void __launch_bounds__(256, 4) rotary_nd_kernel(const __grid_constant__ RotaryParams p, int TB, int heads_per_cta) {
   using V = RotVec<T, VEC>;
   extern __shared__ float2 table[];  // [TB][rot / 2]
   const int t0 = blockIdx.x * TB, tn = min(TB, p.T - t0);
@@ -72,35 +72,51 @@ __global__ void __launch_bounds__(256) rotary_nd_kernel(const __grid_constant__ 
       // first element of the piece, and of its partner half
       const int da = i >= turn ? p.rot + (i - turn) * VEC : IL ? (VEC > 1 ? i * VEC : 2 * i) : i * VEC;
       const int db = IL ? da + 1 : da + half;
-#pragma unroll 4
-      for (int hi = hl; hi < hn; hi += lanes) {
-        int h = h0 + hi;
-        const int w = h >= p.H;
-        if (w) h -= p.H;
-        const T* x = static_cast<const T*>(p.x[w]) + t * p.sx[w][0] + h * p.sx[w][1];
-        T* y = static_cast<T*>(p.y[w]) + t * p.sy[w][0] + h * p.sy[w][1];
+      // q's heads of this CTA, then k's (apart, so that each has fixed strides)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const int lo = w ? max(h0, p.H) : h0, hi = w ? h0 + hn : min(h0 + hn, p.H), off = w ? p.H : 0;
+        const T* const x0 = static_cast<const T*>(p.x[w]) + t * p.sx[w][0];
+        T* const y0 = static_cast<T*>(p.y[w]) + t * p.sy[w][0];
         const int64_t dx = VEC > 1 ? 1 : p.sx[w][2], dy = VEC > 1 ? 1 : p.sy[w][2];
-        V a = *reinterpret_cast<const V*>(x + da * dx);
-        if (i < turn) {
-          if (IL && VEC > 1) {
+        constexpr int MLP = VEC == 1 ? 1 : IL ? 4 : 2;  // heads in flight
+        for (int h = lo + hl; h < hi; h += MLP * lanes) {
+          V a[MLP], b[MLP];
 #pragma unroll
-            for (int k = 0; k < VEC / 2; ++k) {
-              const float u = Elem<T>::to_f(a.e[(2 * k) % VEC]), v = Elem<T>::to_f(a.e[(2 * k + 1) % VEC]);
-              a.e[(2 * k) % VEC] = Elem<T>::from_f(u * cs[k % NCS].x - v * cs[k % NCS].y);
-              a.e[(2 * k + 1) % VEC] = Elem<T>::from_f(u * cs[k % NCS].y + v * cs[k % NCS].x);
+          for (int u = 0; u < MLP; ++u) {
+            const int hh = h + u * lanes;
+            if (hh < hi) {
+              const T* x = x0 + (hh - off) * p.sx[w][1];
+              a[u] = *reinterpret_cast<const V*>(x + da * dx);
+              if ((!IL || VEC == 1) && i < turn) b[u] = *reinterpret_cast<const V*>(x + db * dx);
             }
-          } else {
-            V b = *reinterpret_cast<const V*>(x + db * dx);
+          }
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-              const float u = Elem<T>::to_f(a.e[k]), v = Elem<T>::to_f(b.e[k]);
-              a.e[k] = Elem<T>::from_f(u * cs[k % NCS].x - v * cs[k % NCS].y);
-              b.e[k] = Elem<T>::from_f(u * cs[k % NCS].y + v * cs[k % NCS].x);
+          for (int u = 0; u < MLP; ++u) {
+            const int hh = h + u * lanes;
+            if (hh >= hi) continue;
+            T* y = y0 + (hh - off) * p.sy[w][1];
+            if (i < turn) {
+              if (IL && VEC > 1) {
+#pragma unroll
+                for (int k = 0; k < VEC / 2; ++k) {
+                  const float e = Elem<T>::to_f(a[u].e[(2 * k) % VEC]), f = Elem<T>::to_f(a[u].e[(2 * k + 1) % VEC]);
+                  a[u].e[(2 * k) % VEC] = Elem<T>::from_f(e * cs[k % NCS].x - f * cs[k % NCS].y);
+                  a[u].e[(2 * k + 1) % VEC] = Elem<T>::from_f(e * cs[k % NCS].y + f * cs[k % NCS].x);
+                }
+              } else {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                  const float e = Elem<T>::to_f(a[u].e[k]), f = Elem<T>::to_f(b[u].e[k]);
+                  a[u].e[k] = Elem<T>::from_f(e * cs[k % NCS].x - f * cs[k % NCS].y);
+                  b[u].e[k] = Elem<T>::from_f(e * cs[k % NCS].y + f * cs[k % NCS].x);
+                }
+                *reinterpret_cast<V*>(y + db * dy) = b[u];
+              }
             }
-            *reinterpret_cast<V*>(y + db * dy) = b;
+            *reinterpret_cast<V*>(y + da * dy) = a[u];
           }
         }
-        *reinterpret_cast<V*>(y + da * dy) = a;
       }
     }
   }
