@@ -36,8 +36,8 @@ struct Kv8View {
 // Page holding row r of sequence s, or -1 when the row lies past the
 // sequence's block-table row or the table names a page outside the cache.
 __device__ __forceinline__ int64_t kv8_page(const Kv8View& c, int s, int64_t r) {
-  if (r < 0 || r >= c.max_rows) return -1;
-  const int64_t page = c.block_tables[s * c.sbt[0] + (r / c.P) * c.sbt[1]];
+  if (r < 0 || r >= c.max_rows) return -1;  // max_rows < 2^31: a 32-bit division
+  const int64_t page = c.block_tables[s * c.sbt[0] + static_cast<int64_t>(static_cast<uint32_t>(r) / static_cast<uint32_t>(c.P)) * c.sbt[1]];
   return (page >= 0 && page < c.num_blocks) ? page : -1;
 }
 __device__ __forceinline__ uint8_t* kv8_row(const Kv8Plane& p, int64_t page, int h, int row) {

@@ -52,13 +52,14 @@ __device__ __forceinline__ bool kv8_write_item(const Kv8WriteParams& p, int64_t 
   const int64_t tok0 = p.cu ? p.cu[lo] : lo;
   const int64_t n = p.cu ? p.cu[lo + 1] - tok0 : 1;
   const int64_t start = p.start_lens[lo];
-  const int64_t first = (start / c.group + (item - kv8_item_base(p, lo))) * c.group;  // the group's first position
-  if (n <= 0 || start < 0 || first >= start + n) return false;
+  if (n <= 0 || start < 0) return false;
+  const int64_t first = (static_cast<uint32_t>(start) / static_cast<uint32_t>(c.group) + (item - kv8_item_base(p, lo))) * c.group;  // the group's first position
+  if (first >= start + n) return false;
   w.s = lo;
   w.page = kv8_page(c, lo, first);
   if (w.page < 0) return false;
   const int64_t r0 = max(start, first), r1 = min(start + n, first + c.group);
-  w.in_page = static_cast<int>(first % c.P);
+  w.in_page = static_cast<int>(static_cast<uint32_t>(first) % static_cast<uint32_t>(c.P));  // page >= 0: first < 2^31
   w.token = tok0 + (r0 - start);
   w.held = static_cast<int>(r0 - first);
   w.fresh = static_cast<int>(r1 - r0);
@@ -99,9 +100,9 @@ __global__ void __launch_bounds__(TPI == 32 ? 128 : TPI) kv8_write_vec_kernel(co
   const Kv8View& c = p.c;
   const int lane = threadIdx.x % TPI;
   // the heads of an item are neighbours: they read the same rows
-  int64_t id = TPI == 32 ? static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32 : blockIdx.x;
-  const int h = static_cast<int>(id % c.Hkv);
-  id /= c.Hkv;
+  uint32_t id = TPI == 32 ? blockIdx.x * 4 + threadIdx.x / 32 : blockIdx.x;  // units < 2^31
+  const int h = id % static_cast<uint32_t>(c.Hkv);
+  id /= static_cast<uint32_t>(c.Hkv);
   Kv8WriteItem w;
   if (id >= items || !kv8_write_item(p, id, w)) return;
   const int pr = c.D / 8, n = w.fresh * pr;  // pieces of a row, of the item
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const __grid_constant__ K
     const int64_t pos = in_seq ? t - p.cu[s] + (p.start_lens ? p.start_lens[s] : 0) : -1;
     const int64_t page = kv8_page(c, s, pos);
     s_page[threadIdx.x] = page;
-    s_row[threadIdx.x] = page >= 0 ? static_cast<int>(pos % c.P) : 0;
+    s_row[threadIdx.x] = page >= 0 ? static_cast<int>(static_cast<uint32_t>(pos) % static_cast<uint32_t>(c.P)) : 0;
     s_group[threadIdx.x] = s_row[threadIdx.x] / c.group;
   }
   __syncthreads();

@@ -320,6 +320,10 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
   const int m = p.budget, step = cs * win, first = rank * win;
   const int32_t* kept = p.kept + (static_cast<int64_t>(s) * c.Hkv + h) * p.budget;
   const int steps = (m + step - 1) / step;
+  const int my_g0 = tid / c.group * c.group;  // first row of this thread's group in a window
+  auto step_barrier = [&]() {
+    if (cs > 1) cluster.sync(); else __syncthreads();
+  };
 
   auto position = [&](int w) {  // source position of this thread's row in step w
     const int j = first + w * step + tid;
@@ -330,8 +334,8 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
       sc = nullptr;
       return static_cast<uint8_t*>(nullptr);
     }
-    const int row = i % c.P;
-    sc = kv8_scale(pl, page, h, row / c.group);
+    const int row = static_cast<uint32_t>(i) % static_cast<uint32_t>(c.P);
+    sc = kv8_scale(pl, page, h, static_cast<uint32_t>(row) / static_cast<uint32_t>(c.group));
     return kv8_row(pl, page, h, row);
   };
   auto fetch = [&](int w) {  // the rows of step w, whose addresses are in src[w & 1]
@@ -370,7 +374,7 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
     if (tid < win) src[win + tid] = x;
   }
   cp_async_wait_all();
-  cluster.sync();
+  step_barrier();
   for (int w = 0; w < steps; ++w) {
     const int j0 = first + w * step, rows = max(0, min(win, m - j0));
     // loads for the steps ahead
@@ -384,13 +388,12 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
     if (tid < win) was[tid] = mine ? v0 : 0.f;
     __syncthreads();
     if (mine) {
-      const int g0 = tid / c.group * c.group;
       float big = 0.f;
-      for (int r = g0; r < min(rows, g0 + c.group); ++r) big = kv8_scale_max(big, was[r]);
+      for (int r = my_g0; r < min(rows, my_g0 + c.group); ++r) big = kv8_scale_max(big, was[r]);
       ratio[tid] = v0 < big ? v0 / big : 1.f;
       const float* sc;
       dst[tid] = place(dpage, j0 + tid, sc);
-      if (tid == g0 && sc) *const_cast<float*>(sc) = big;
+      if (tid == my_g0 && sc) *const_cast<float*>(sc) = big;
     }
     __syncthreads();
     // ---- write this step's rows ----
@@ -431,7 +434,7 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
     }
     i2 = i3;
     cp_async_wait_all();
-    cluster.sync();
+    step_barrier();
   }
 }
 
