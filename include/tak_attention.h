@@ -22,7 +22,8 @@
  *   - stream is a cudaStream_t (NULL = legacy default stream).  Calls are
  *     asynchronous; no entry point synchronises the device.
  *   - Return value: 0 on success, nonzero on error (1 = invalid argument,
- *     2 = unsupported shape, 3 = CUDA error); tak_last_error() describes the
+ *     2 = unsupported shape, 3 = CUDA error, 4 = tak_kv8_attention's workspace
+ *     is too small, nothing launched); tak_last_error() describes the
  *     last error of the calling thread.  No entry point aborts the process.
  */
 #ifndef TAK_ATTENTION_H_

@@ -125,7 +125,29 @@ def as_i32(t, device):
     return t.to(device=device, dtype=torch.int32)
 
 
+def i32_on(t, index):
+    """as_i32 for the device with this index; a tensor that already fits is
+    returned as it is, without the cost of a .to() call."""
+    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.is_cuda and t.get_device() == index:
+        return t
+    return as_i32(t, torch.device("cuda", index))
+
+
+def raw_stream(index):
+    """cudaStream_t of the current stream of a device, as an int."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 _ws = {}
+
+
+def workspace_of(index, stream, nbytes=0):
+    """The (device, stream)'s scratch buffer of workspace(), as it is or grown to
+    nbytes, keyed by plain ints."""
+    buf = _ws.get((index, stream))
+    if buf is None or buf.numel() < nbytes:
+        buf = workspace(torch.device("cuda", index), ctypes.c_void_p(stream), nbytes)
+    return buf
 
 
 def workspace(device, stream_handle, nbytes):

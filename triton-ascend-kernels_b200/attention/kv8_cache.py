@@ -14,6 +14,7 @@ import _tak_b200 as _t
 
 _torch = _t.torch
 _CODES = {_torch.int8: 0, _torch.float8_e4m3fn: 1}
+_S3 = struct.Struct("=3q").pack
 _PACK = struct.Struct("=5q5q4q4q3q8q")  # struct tak_kv8_cache: every field 8 bytes
 
 
@@ -30,25 +31,40 @@ def kv8_alloc(num_blocks, num_kv_heads, block_size, head_dim, *, group=16, dtype
 
 
 def describe(k_cache, v_cache, k_scale, v_scale, block_tables):
-    """The C ABI's description of a cache (struct tak_kv8_cache, as bytes) and
-    the int32 block table that it points to."""
+    """The C ABI's description of a cache (struct tak_kv8_cache, as bytes), the
+    int32 block table that it points to, and (device index, num_kv_heads,
+    head_dim, num_seqs)."""
     _t.require_cuda(k_cache, v_cache, k_scale, v_scale)
-    assert k_cache.dtype in _CODES, f"unsupported cache dtype {k_cache.dtype}: expected int8 or float8_e4m3fn"
-    assert k_cache.dim() == 4 and v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype, \
+    dtype = k_cache.dtype
+    code = _CODES.get(dtype)
+    assert code is not None, f"unsupported cache dtype {dtype}: expected int8 or float8_e4m3fn"
+    shape = k_cache.shape
+    assert len(shape) == 4 and v_cache.shape == shape and v_cache.dtype is dtype, \
         "k_cache and v_cache must be [num_blocks, num_kv_heads, block_size, head_dim] of one dtype"
-    nb, hkv, rows, d = k_cache.shape
-    assert k_scale.dim() == 3 and k_scale.shape[:2] == (nb, hkv) and v_scale.shape == k_scale.shape, \
+    nb, hkv, rows, d = shape
+    ss = k_scale.shape
+    assert len(ss) == 3 and ss[0] == nb and ss[1] == hkv and v_scale.shape == ss, \
         "k_scale and v_scale must be [num_blocks, num_kv_heads, block_size / group]"
-    assert k_scale.dtype == _torch.float32 and v_scale.dtype == _torch.float32, "scales must be float32"
-    ng = k_scale.shape[2]
+    assert k_scale.dtype is _torch.float32 and v_scale.dtype is _torch.float32, "scales must be float32"
+    ng = ss[2]
+    index = k_cache.get_device()
+    assert v_cache.get_device() == index and k_scale.get_device() == index and v_scale.get_device() == index, \
+        "the cache's tensors must be on one device"
     assert ng > 0 and rows % ng == 0, f"the number of scales ({ng}) must divide block_size ({rows})"
-    bt = _t.as_i32(block_tables, k_cache.device)
+    bt = _t.i32_on(block_tables, index)
     assert bt.dim() == 2, "block_tables must be [num_seqs, max_blocks]"
+    seqs, width = bt.shape
     return _PACK.pack(
         k_cache.data_ptr(), *k_cache.stride(), v_cache.data_ptr(), *v_cache.stride(),
         k_scale.data_ptr(), *k_scale.stride(), v_scale.data_ptr(), *v_scale.stride(),
-        bt.data_ptr(), *bt.stride(), nb, hkv, rows, d, rows // ng, bt.shape[0], bt.shape[1],
-        _CODES[k_cache.dtype]), bt
+        bt.data_ptr(), *bt.stride(), nb, hkv, rows, d, rows // ng, seqs, width, code), bt, (index, hkv, d, seqs)
+
+
+def _lens(t, index, n, name):
+    """A contiguous int32 [n] tensor on the device."""
+    t = _t.i32_on(t, index)
+    assert t.dim() == 1 and t.shape[0] == n, f"{name} must have {n} elements here"
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def kv8_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, block_tables, start_lens, cu_seqlens=None):
@@ -68,19 +84,19 @@ def kv8_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, block_tables, star
     rows held under a smaller one are rounded again into it.
     """
     _t.require_cuda(k, v)
-    d, bt = describe(k_cache, v_cache, k_scale, v_scale, block_tables)
-    assert k.dim() == 3 and v.shape == k.shape and v.dtype == k.dtype, "K and V must have the same shape and dtype"
-    assert k.shape[1] == k_cache.shape[1] and k.shape[2] == k_cache.shape[3], \
-        "k / v must be [total_tokens, num_kv_heads, head_dim] of the cache"
-    start = _t.as_i32(start_lens, k.device)
-    assert start.dim() == 1 and start.shape[0] == bt.shape[0], "start_lens must be [num_seqs]"
-    cu = None if cu_seqlens is None else _t.as_i32(cu_seqlens, k.device)
-    assert cu is None or (cu.dim() == 1 and cu.shape[0] == bt.shape[0] + 1), "cu_seqlens must be [num_seqs + 1]"
-    assert cu is not None or k.shape[0] == bt.shape[0], "without cu_seqlens k / v hold one row per sequence"
-    start = start.contiguous()
-    cu = None if cu is None else cu.contiguous()
-    _t.check(_t.lib().tak_kv8_write(d, _t.ptr(k), _t.strides(k), _t.ptr(v), _t.strides(v), _t.ptr(start), _t.ptr(cu),
-                                    k.shape[0], _t.dtype_code(k), _t.stream_of(k)))
+    desc, _bt, (index, hkv, d, seqs) = describe(k_cache, v_cache, k_scale, v_scale, block_tables)
+    shape = k.shape
+    assert len(shape) == 3 and v.shape == shape and v.dtype is k.dtype, "K and V must have the same shape and dtype"
+    assert k.get_device() == index and v.get_device() == index, "k / v must be on the cache's device"
+    assert shape[1] == hkv and shape[2] == d, "k / v must be [total_tokens, num_kv_heads, head_dim] of the cache"
+    start = _lens(start_lens, index, seqs, "start_lens")
+    cu = None if cu_seqlens is None else _lens(cu_seqlens, index, seqs + 1, "cu_seqlens")
+    assert cu is not None or shape[0] == seqs, "without cu_seqlens k / v hold one row per sequence"
+    rc = _t.lib().tak_kv8_write(desc, k.data_ptr(), _S3(*k.stride()), v.data_ptr(), _S3(*v.stride()),
+                                start.data_ptr(), None if cu is None else cu.data_ptr(), shape[0], _t.dtype_code(k),
+                                _t.raw_stream(index))
+    if rc:
+        _t.check(rc)
 
 
 def kv8_cache_read(k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens, total_tokens, *,
@@ -89,16 +105,17 @@ def kv8_cache_read(k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens,
     num_kv_heads, head_dim], rows cu_seqlens[s] and on holding positions
     start_lens[s] (None: 0) and on of sequence s.  Rows outside every sequence
     are zeros."""
-    d, bt = describe(k_cache, v_cache, k_scale, v_scale, block_tables)
-    dev = k_cache.device
-    cu = _t.as_i32(cu_seqlens, dev).contiguous()
-    assert cu.dim() == 1 and cu.shape[0] == bt.shape[0] + 1, "cu_seqlens must be [num_seqs + 1]"
-    start = None if start_lens is None else _t.as_i32(start_lens, dev).contiguous()
-    assert start is None or (start.dim() == 1 and start.shape[0] == bt.shape[0]), "start_lens must be [num_seqs]"
-    k = _torch.empty((int(total_tokens), k_cache.shape[1], k_cache.shape[3]), dtype=dtype, device=dev)
-    v = _torch.empty_like(k)
-    _t.check(_t.lib().tak_kv8_read(d, _t.ptr(cu), _t.ptr(start), k.shape[0], _t.ptr(k), _t.strides(k), _t.ptr(v),
-                                   _t.strides(v), _t.dtype_code(k), _t.stream_of(k)))
+    desc, _bt, (index, hkv, d, seqs) = describe(k_cache, v_cache, k_scale, v_scale, block_tables)
+    cu = _lens(cu_seqlens, index, seqs + 1, "cu_seqlens")
+    start = None if start_lens is None else _lens(start_lens, index, seqs, "start_lens")
+    total = int(total_tokens)
+    k = k_scale.new_empty((total, hkv, d), dtype=dtype)
+    v = k_scale.new_empty((total, hkv, d), dtype=dtype)
+    st = _S3(hkv * d, d, 1)
+    rc = _t.lib().tak_kv8_read(desc, cu.data_ptr(), None if start is None else start.data_ptr(), total,
+                               k.data_ptr(), st, v.data_ptr(), st, _t.dtype_code(k), _t.raw_stream(index))
+    if rc:
+        _t.check(rc)
     return k, v
 
 
@@ -120,17 +137,19 @@ def kv8_cache_evict(k_cache, v_cache, k_scale, v_scale, block_tables, context_le
     int32 rows per sequence.  Pages past new_lens are free; sequences must not
     share pages.
     """
-    d, bt = describe(k_cache, v_cache, k_scale, v_scale, block_tables)
-    dev = k_cache.device
-    cl = _t.as_i32(context_lens, dev).contiguous()
-    budget, recent = int(budget), int(recent)
-    assert cl.dim() == 1 and cl.shape[0] == bt.shape[0], "context_lens must be [num_seqs]"
     _t.require_cuda(weights)
-    assert weights.dim() == 3 and weights.shape[:2] == (bt.shape[0], k_cache.shape[1]) \
-        and weights.dtype == _torch.float32, "weights must be float32 [num_seqs, num_kv_heads, max_rows]"
+    desc, _bt, (index, hkv, _d, seqs) = describe(k_cache, v_cache, k_scale, v_scale, block_tables)
+    cl = _lens(context_lens, index, seqs, "context_lens")
+    budget, recent = int(budget), int(recent)
+    ws = weights.shape
+    assert len(ws) == 3 and ws[0] == seqs and ws[1] == hkv and weights.dtype is _torch.float32, \
+        "weights must be float32 [num_seqs, num_kv_heads, max_rows]"
+    assert weights.get_device() == index, "weights must be on the cache's device"
     assert budget >= 1 and 0 <= recent <= budget, "budget must be >= 1 and recent in [0, budget]"
-    kept = _torch.empty((bt.shape[0], k_cache.shape[1], budget), dtype=_torch.int32, device=dev)
-    lens = _torch.empty((bt.shape[0],), dtype=_torch.int32, device=dev)
-    _t.check(_t.lib().tak_kv8_evict(d, _t.ptr(cl), _t.ptr(weights), _t.strides(weights), weights.shape[2], budget,
-                                    recent, _t.ptr(kept), _t.ptr(lens), _t.stream_of(k_cache)))
+    kept = cl.new_empty((seqs, hkv, budget))
+    lens = cl.new_empty((seqs,))
+    rc = _t.lib().tak_kv8_evict(desc, cl.data_ptr(), weights.data_ptr(), _S3(*weights.stride()), ws[2], budget,
+                                recent, kept.data_ptr(), lens.data_ptr(), _t.raw_stream(index))
+    if rc:
+        _t.check(rc)
     return kept, lens

@@ -6,9 +6,12 @@ V are held in 8 bits with a scale for each page, head and group of rows.
 """
 
 import math
+import struct
 
 import _tak_b200 as _t
-from kv8_cache import describe
+from kv8_cache import _lens, describe
+
+_S3, _S4 = struct.Struct("=3q").pack, struct.Struct("=4q").pack
 
 
 def paged_attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, *, softcap=0.0,
@@ -32,35 +35,44 @@ def paged_attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_tables, con
 
     A row that sees no key gives zeros (lse -inf).
     """
-    _t.require_cuda(q)
-    d, bt = describe(k_cache, v_cache, k_scale, v_scale, block_tables)
-    assert q.dim() in (3, 4), "q must be [num_seqs, num_q_heads, head_dim] or [num_seqs, num_queries, ...]"
-    q4 = q if q.dim() == 4 else q.unsqueeze(1)
-    B, Lq, H, D = q4.shape
-    hkv = k_cache.shape[1]
-    assert B == bt.shape[0], "block_tables must have a row per sequence"
-    assert D == k_cache.shape[3], f"head_dim of q ({D}) and of the cache ({k_cache.shape[3]}) differ"
+    _t.require_cuda(q, weights)
+    desc, _bt, (index, hkv, d, seqs) = describe(k_cache, v_cache, k_scale, v_scale, block_tables)
+    shape = q.shape
+    assert len(shape) in (3, 4), "q must be [num_seqs, num_q_heads, head_dim] or [num_seqs, num_queries, ...]"
+    assert q.get_device() == index and (weights is None or weights.get_device() == index), \
+        "q and weights must be on the cache's device"
+    B, H, D = shape[0], shape[-2], shape[-1]
+    Lq = shape[1] if len(shape) == 4 else 1
+    assert B == seqs, "block_tables must have a row per sequence"
+    assert D == d, f"head_dim of q ({D}) and of the cache ({d}) differ"
     assert H % hkv == 0, f"num_q_heads ({H}) must be divisible by num_kv_heads ({hkv})"
     assert softcap >= 0.0, "softcap must be >= 0"
-    cl = _t.as_i32(context_lens, q.device)
-    assert cl.dim() == 1 and cl.shape[0] == B, "context_lens must be [num_seqs]"
-    cl = cl.contiguous()
+    cl = _lens(context_lens, index, seqs, "context_lens")
+    st = q.stride()
+    if len(st) == 3:
+        st = (st[0], 0, st[1], st[2])
+    wp = wst = None
     width = 0
     if weights is not None:
-        _t.require_cuda(weights)
-        assert weights.dim() == 3 and weights.shape[:2] == (B, hkv) and weights.dtype == _t.torch.float32, \
+        ws = weights.shape
+        assert len(ws) == 3 and ws[0] == B and ws[1] == hkv and weights.dtype is _t.torch.float32, \
             "weights must be float32 [num_seqs, num_kv_heads, max_rows]"
-        width = weights.shape[2]
-    out = q.new_empty(q.shape)
-    out4 = out if q.dim() == 4 else out.unsqueeze(1)
-    lse = q.new_empty(q.shape[:-1], dtype=_t.torch.float32) if return_lse else None
+        width = ws[2]
+        wp, wst = weights.data_ptr(), _S3(*weights.stride())
+    out = q.new_empty(shape)
+    lse = q.new_empty(shape[:-1], dtype=_t.torch.float32) if return_lse else None
     L = _t.lib()
-    st = _t.stream_of(q)
+    stream = _t.raw_stream(index)
     code = _t.dtype_code(q)
-    need = L.tak_kv8_attention_workspace_size(d, H, Lq, width, code)
-    ws = _t.workspace(q.device, st, max(need, 0))
-    _t.check(L.tak_kv8_attention(
-        d, _t.ptr(q4), _t.strides(q4), _t.ptr(cl), _t.ptr(out4), _t.strides(out4), _t.ptr(lse), _t.ptr(weights),
-        None if weights is None else _t.strides(weights), width, H, Lq, 1.0 / math.sqrt(D), float(softcap), code,
-        _t.ptr(ws), ws.numel(), st))
+    scratch = _t.workspace_of(index, stream)
+    while True:
+        rc = L.tak_kv8_attention(
+            desc, q.data_ptr(), _S4(*st), cl.data_ptr(), out.data_ptr(), _S4(Lq * H * D, H * D, D, 1),
+            None if lse is None else lse.data_ptr(), wp, wst, width, H, Lq, 1.0 / math.sqrt(D), softcap, code,
+            scratch.data_ptr(), scratch.numel(), stream)
+        if rc != 4:  # 4: the workspace is too small; nothing was launched
+            break
+        scratch = _t.workspace_of(index, stream, L.tak_kv8_attention_workspace_size(desc, H, Lq, width, code))
+    if rc:
+        _t.check(rc)
     return (out, lse) if return_lse else out

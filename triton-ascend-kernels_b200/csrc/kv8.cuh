@@ -92,7 +92,8 @@ __device__ __forceinline__ float kv8_scale_max(float a, float b) {
 // Four codes at once, the same roundings as dec and enc one by one.
 // int8 -> fp32: the byte with its sign bit flipped, as the mantissa's low byte of
 // 2^23, less 2^23 + 128.  fp32 -> int8: adding 1.5 * 2^23 rounds to nearest even
-// and leaves the two's complement in the low byte (|x| < 128 from a finite scale).
+// and leaves the two's complement in the low byte; a group's own scale keeps |f|
+// within 127 (1 + 2^-22), so nothing has to be clamped.
 template <int CODE> __device__ __forceinline__ void kv8_dec4(uint32_t q, float* f) {
   if (CODE == kI8) {
     const uint32_t x = q ^ 0x80808080u;
@@ -111,7 +112,7 @@ template <int CODE> __device__ __forceinline__ uint32_t kv8_enc4(const float* f)
   if (CODE == kI8) {
     uint32_t u[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) u[k] = __float_as_uint(__fadd_rn(fminf(fmaxf(f[k], -127.f), 127.f), 12582912.f));
+    for (int k = 0; k < 4; ++k) u[k] = __float_as_uint(__fadd_rn(f[k], 12582912.f));
     return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
   }
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3);

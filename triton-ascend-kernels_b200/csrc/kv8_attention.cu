@@ -1008,7 +1008,7 @@ static int launch_rows(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) 
 }
 
 int kv8_attention_launch(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
-  if (kv8_attention_ws_bytes(c, a) > a.workspace_bytes) return set_error(2, "kv8 attention: workspace too small");
+  if (kv8_attention_ws_bytes(c, a) > a.workspace_bytes) return set_error(4, "kv8 attention: workspace too small");
   if (!tc_ok(c, a)) return kv8_attention_generic_launch(c, a, st);
   TAK_BY_CODE(a.code_type, {
     switch (tc_dp(c)) {

@@ -66,10 +66,29 @@ __device__ __forceinline__ bool kv8_write_item(const Kv8WriteParams& p, int64_t 
   return true;
 }
 
-// Eight elements of a row, as loaded (16-bit types: one 16-byte word)
+// Eight elements of a row, as loaded (16-bit types: one 16-byte word), and the
+// running maximum of magnitudes over such pieces.  The maxima keep NaN.
+template <typename T> struct Pair;
+template <> struct Pair<__half> { using type = __half2; };
+template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
 template <typename T> struct Eight {
+  using P = typename Pair<T>::type;
   uint4 v;
+  struct Max {
+    uint32_t m = 0;
+    __device__ __forceinline__ uint32_t bits() const {
+      const float2 f = Elem<T>::unpack2(m);
+      return max(abs_bits(f.x), abs_bits(f.y));
+    }
+  };
   __device__ __forceinline__ void load(const T* x) { v = *reinterpret_cast<const uint4*>(x); }
+  __device__ __forceinline__ void into(Max& a) const {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+    P m = *reinterpret_cast<P*>(&a.m);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const P*>(&u[k])));
+    a.m = *reinterpret_cast<uint32_t*>(&m);
+  }
   __device__ __forceinline__ void get(float* f) const {
     const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -82,9 +101,19 @@ template <typename T> struct Eight {
 };
 template <> struct Eight<float> {
   float4 a, b;
+  struct Max {
+    uint32_t m = 0;
+    __device__ __forceinline__ uint32_t bits() const { return m; }
+  };
   __device__ __forceinline__ void load(const float* x) {
     a = *reinterpret_cast<const float4*>(x);
     b = *reinterpret_cast<const float4*>(x + 4);
+  }
+  __device__ __forceinline__ void into(Max& x) const {
+    float f[8];
+    get(f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.m = max(x.m, abs_bits(f[i]));
   }
   __device__ __forceinline__ void get(float* f) const {
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
@@ -129,18 +158,14 @@ __global__ void __launch_bounds__(TPI == 32 ? 128 : TPI) kv8_write_vec_kernel(co
       if (lane + k * TPI < n) v[which][k].load(x + r * p.sx[which][0] + d);
     }
   }
-  uint32_t amax[2] = {0, 0};
+  uint32_t amax[2];
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
+    typename Eight<T>::Max top;
 #pragma unroll
     for (int k = 0; k < U; ++k)
-      if (lane + k * TPI < n) {
-        float f[8];
-        v[which][k].get(f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) amax[which] = max(amax[which], abs_bits(f[i]));
-      }
-    amax[which] = __reduce_max_sync(0xffffffffu, amax[which]);
+      if (lane + k * TPI < n) v[which][k].into(top);
+    amax[which] = __reduce_max_sync(0xffffffffu, top.bits());
   }
   if (TPI > 32) {
     __shared__ uint2 red[TPI / 32];
@@ -169,17 +194,21 @@ __global__ void __launch_bounds__(TPI == 32 ? 128 : TPI) kv8_write_vec_kernel(co
         *q = t;
       }
     }
-    const float inv = now > 0.f ? 1.0f / now : 0.f;  // 0 for a NaN scale too: its codes are 0
+    const float inv = now > 0.f ? 1.0f / now : 0.f;
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       if (lane + k * TPI >= n) continue;
-      float f[8];
-      v[which][k].get(f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = inv > 0.f ? __fmul_rn(f[i], inv) : 0.f;
       int r, d;
       place(k, r, d);
-      *reinterpret_cast<uint2*>(row0 + (w.held + r) * pl.sc[2] + d) = make_uint2(kv8_enc4<CODE>(f), kv8_enc4<CODE>(f + 4));
+      uint2 q = make_uint2(0, 0);
+      if (now > 0.f) {  // else (zeros, or a NaN scale) the codes are 0
+        float f[8];
+        v[which][k].get(f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(f[i], inv);
+        q = make_uint2(kv8_enc4<CODE>(f), kv8_enc4<CODE>(f + 4));
+      }
+      *reinterpret_cast<uint2*>(row0 + (w.held + r) * pl.sc[2] + d) = q;
     }
   }
 }
@@ -276,8 +305,8 @@ struct Kv8ReadParams {
 template <typename T, int CODE, int VEC>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const __grid_constant__ Kv8ReadParams p, int TB) {
   const Kv8View& c = p.c;
-  __shared__ int64_t s_page[16];
-  __shared__ int s_row[16], s_group[16];
+  __shared__ int64_t s_page[64];
+  __shared__ int s_row[64], s_group[64];
   const int t0 = blockIdx.x * TB, tn = static_cast<int>(min(static_cast<int64_t>(TB), p.total - t0));
   if (threadIdx.x < tn) {
     const int t = t0 + threadIdx.x;
@@ -353,8 +382,8 @@ int kv8_read_launch(const Kv8View& c, int code_type, const int32_t* cu, const in
   p.total = total;
   const int size = dtype == kF32 ? 4 : 2;
   const bool vec = codes_vec_ok(c, 16) && rows_vec_ok(k, sk, size) && rows_vec_ok(v, sv, size);
-  // tokens of a CTA: fewer where 16 would leave SMs without one
-  const int tb = total >= 16 * 4 * num_sms() ? 16 : total >= 4 * 2 * num_sms() ? 4 : 2;
+  // tokens of a CTA (one lookup of their pages each): fewer where SMs would be left without one
+  const int tb = total >= 32 * 8 * num_sms() ? 32 : total >= 16 * 4 * num_sms() ? 16 : total >= 4 * 2 * num_sms() ? 4 : 2;
   const unsigned grid = static_cast<unsigned>((total + tb - 1) / tb);
   note_kernel("kv8_read");
   TAK_BY_DTYPE(dtype, TAK_BY_CODE(code_type, {

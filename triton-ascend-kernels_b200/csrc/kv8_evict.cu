@@ -321,6 +321,7 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
   const int32_t* kept = p.kept + (static_cast<int64_t>(s) * c.Hkv + h) * p.budget;
   const int steps = (m + step - 1) / step;
   const int my_g0 = tid / c.group * c.group;  // first row of this thread's group in a window
+  const bool by_shuffle = c.group <= 32 && (c.group & (c.group - 1)) == 0;  // a group lies in one warp
   auto step_barrier = [&]() {
     if (cs > 1) cluster.sync(); else __syncthreads();
   };
@@ -385,11 +386,19 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
     const bool mine = tid < rows;
     const int64_t dpage = mine ? kv8_page(c, s, j0 + tid) : -1;
     // ---- this step's scales: the largest of each destination group ----
-    if (tid < win) was[tid] = mine ? v0 : 0.f;
-    __syncthreads();
+    float v_group = mine ? v0 : 0.f;
+    if (by_shuffle) {
+      for (int o = 1; o < c.group; o <<= 1) v_group = kv8_scale_max(v_group, __shfl_xor_sync(0xffffffffu, v_group, o));
+    } else {
+      if (tid < win) was[tid] = v_group;
+      __syncthreads();
+    }
     if (mine) {
-      float big = 0.f;
-      for (int r = my_g0; r < min(rows, my_g0 + c.group); ++r) big = kv8_scale_max(big, was[r]);
+      float big = v_group;
+      if (!by_shuffle) {
+        big = 0.f;
+        for (int r = my_g0; r < min(rows, my_g0 + c.group); ++r) big = kv8_scale_max(big, was[r]);
+      }
       ratio[tid] = v0 < big ? v0 / big : 1.f;
       const float* sc;
       dst[tid] = place(dpage, j0 + tid, sc);
@@ -461,6 +470,31 @@ static int launch_cluster(K kern, dim3 grid, int threads, size_t smem, int cs, b
   return set_error(3, buf);
 }
 
+// Whether clusters of 16 CTAs of this kernel can run (more than eight is not
+// portable: it has to be allowed, and a GPC has to have the room).
+static bool cluster16_ok(const void* func, int threads, size_t smem) {
+  if (cudaFuncSetAttribute(func, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(16);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 16;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, func, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  return n > 0;
+}
+
 int kv8_evict_launch(const Kv8View& c, int code_type, const int32_t* context_lens, float* weights,
                      const int64_t* sw, int64_t width, int64_t budget, int64_t recent, int32_t* kept,
                      int32_t* new_lens, cudaStream_t st) {
@@ -479,34 +513,39 @@ int kv8_evict_launch(const Kv8View& c, int code_type, const int32_t* context_len
   const int64_t sel = kSelThreads;
   note_kernel("kv8_evict");
   if (rows <= 16 * 8 * sel) {
+    // eight weights a thread let two CTAs fit an SM; past 8 CTAs of that, sixteen
+    // (8 heads of 100000 weights: 28 us; eight a thread in clusters of 16: 56 us)
+    const int kpt = rows <= 4 * sel ? 4 : rows <= 8 * 8 * sel ? 8 : 16;
     int cs = 1;
-    while (rows > 16 * sel * cs) cs *= 2;
+    while (rows > kpt * sel * cs) cs *= 2;
     const dim3 grid(c.Hkv * cs, c.num_seqs);
     int r;
-    if (rows <= 4 * sel) r = launch_cluster(kv8_evict_select_reg_kernel<4>, grid, kSelThreads, 0, cs, false, st, p);
-    else if (rows <= 8 * sel) r = launch_cluster(kv8_evict_select_reg_kernel<8>, grid, kSelThreads, 0, cs, false, st, p);
+    if (kpt == 4) r = launch_cluster(kv8_evict_select_reg_kernel<4>, grid, kSelThreads, 0, cs, false, st, p);
+    else if (kpt == 8) r = launch_cluster(kv8_evict_select_reg_kernel<8>, grid, kSelThreads, 0, cs, false, st, p);
     else r = launch_cluster(kv8_evict_select_reg_kernel<16>, grid, kSelThreads, 0, cs, false, st, p);
     if (r) return r;
   } else {
     kv8_evict_select_kernel<<<dim3(c.Hkv, c.num_seqs), kSelThreads, 0, st>>>(p);
   }
-  // ---- move: windows of about 16 KB of rows, a multiple of the group ----
-  int64_t win = 16384 / c.D / c.group * c.group;
+  // ---- move: windows of about 32 KB of rows, a multiple of the group ----
+  int64_t win = 32768 / c.D / c.group * c.group;
   if (win < c.group) win = c.group;
   if (win > 256) win = 256 / c.group * c.group;
   p.window = static_cast<int>(win);
   const int64_t smem = (2 * win * c.D + 15) / 16 * 16 + 3 * win * 8 + 2 * win * 4;
   if (smem > 200 * 1024) return set_error(2, "kv8 evict: group * head_dim is too large");
-  // a cluster per (sequence, head, K or V) where there are fewer of them than SMs
-  const int64_t units = 2 * static_cast<int64_t>(c.Hkv) * c.num_seqs;
-  int cs = 1;
-  while (cs < 8 && units * cs < 2 * num_sms() && cs * win < budget) cs *= 2;
   bool vec = c.D % 16 == 0;
   for (const Kv8Plane& pl : c.plane)
     vec = vec && pl.sc[3] == 1 && (reinterpret_cast<uintptr_t>(pl.code) & 15) == 0 && ((pl.sc[0] | pl.sc[1] | pl.sc[2]) & 15) == 0;
   TAK_BY_CODE(code_type, {
     auto kern = vec ? kv8_evict_move_kernel<CODE, 16> : kv8_evict_move_kernel<CODE, 1>;
     if (const int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), static_cast<int>(smem))) return r;
+    // a cluster per (sequence, head, K or V), of several CTAs where there are fewer
+    // of them than fill the SMs
+    const int64_t units = 2 * static_cast<int64_t>(c.Hkv) * c.num_seqs;
+    int cs = 1;
+    while (cs < 16 && units * cs < num_sms() && cs * win < budget) cs *= 2;
+    if (cs == 16 && !cluster16_ok(reinterpret_cast<const void*>(kern), 256, static_cast<size_t>(smem))) cs = 8;
     return launch_cluster(kern, dim3(c.Hkv * cs, c.num_seqs, 2), 256, static_cast<size_t>(smem), cs, true, st, p);
   });
   return 0;
