@@ -1,5 +1,6 @@
 // extern "C" entry points declared in include/tak_attention.h: argument
 // validation, error strings, tensor-map encoding, dispatch to the kernels.
+#include <atomic>
 #include <cstdio>
 #include <cstring>
 #include <map>
@@ -36,9 +37,14 @@ int check_launch(const char* what) {
 }
 
 int num_sms() {
+  static std::atomic<int> known[64];  // per device; 0 = not asked yet
   int dev = 0, n = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 148;
+  if (cudaGetDevice(&dev) != cudaSuccess) return n;
+  const bool cached = dev >= 0 && dev < 64;
+  if (cached && known[dev].load(std::memory_order_relaxed) > 0) return known[dev].load(std::memory_order_relaxed);
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  if (cached) known[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 int kernel_path() { return g_kernel_path; }

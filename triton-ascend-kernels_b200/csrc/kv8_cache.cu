@@ -300,74 +300,90 @@ struct Kv8ReadParams {
   int64_t total;
 };
 
-// TB tokens a CTA: their pages are looked up once, then every thread converts
-// pieces of VEC codes (16: one load, 32 bytes of 16-bit values or 64 of fp32 out).
+// A CTA walks blocks of TB tokens: while it converts one, its first warps look up
+// the pages of the next, so only the first block waits for the chain of loads
+// (sequence, block table).  Every thread converts pieces of VEC codes (16: one load,
+// 32 bytes of 16-bit values or 64 of fp32 out).
+constexpr int kReadTokens = 32;
+constexpr int RCT = 4;
+
 template <typename T, int CODE, int VEC>
-__global__ void __launch_bounds__(256) kv8_read_kernel(const __grid_constant__ Kv8ReadParams p, int TB) {
+__global__ void __launch_bounds__(256, RCT) kv8_read_kernel(const __grid_constant__ Kv8ReadParams p, int TB) {
   const Kv8View& c = p.c;
-  __shared__ int64_t s_page[64];
-  __shared__ int s_row[64], s_group[64];
-  const int t0 = blockIdx.x * TB, tn = static_cast<int>(min(static_cast<int64_t>(TB), p.total - t0));
-  if (threadIdx.x < tn) {
-    const int t = t0 + threadIdx.x;
+  __shared__ int64_t sh_page[2][kReadTokens];
+  __shared__ int sh_row[2][kReadTokens], sh_group[2][kReadTokens];
+  auto look_up = [&](int64_t t0, int buf) {
+    const int64_t t = t0 + threadIdx.x;
+    if (threadIdx.x >= TB || t >= p.total) return;
     const int s = find_slot_seq(p.cu, c.num_seqs, t);
-    const bool in_seq = t >= p.cu[s] && t < p.cu[s + 1];
-    const int64_t pos = in_seq ? t - p.cu[s] + (p.start_lens ? p.start_lens[s] : 0) : -1;
+    const int lo = p.cu[s];
+    const bool in_seq = t >= lo && t < p.cu[s + 1];
+    const int64_t pos = in_seq ? t - lo + (p.start_lens ? p.start_lens[s] : 0) : -1;
     const int64_t page = kv8_page(c, s, pos);
-    s_page[threadIdx.x] = page;
-    s_row[threadIdx.x] = page >= 0 ? static_cast<int>(static_cast<uint32_t>(pos) % static_cast<uint32_t>(c.P)) : 0;
-    s_group[threadIdx.x] = s_row[threadIdx.x] / c.group;
-  }
+    const int row = page >= 0 ? static_cast<int>(static_cast<uint32_t>(pos) % static_cast<uint32_t>(c.P)) : 0;
+    sh_page[buf][threadIdx.x] = page;
+    sh_row[buf][threadIdx.x] = row;
+    sh_group[buf][threadIdx.x] = static_cast<uint32_t>(row) / static_cast<uint32_t>(c.group);
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * TB;
+  int64_t t0 = static_cast<int64_t>(blockIdx.x) * TB;
+  look_up(t0, 0);
   __syncthreads();
   // a thread keeps its piece of a token (head and columns) and walks the tokens
   const int pr = c.D / VEC, per_tok = c.Hkv * pr;
   const int px = per_tok < 256 ? per_tok : 256, lanes = 256 / px;
   const int tl = threadIdx.x / px;
-  if (tl >= lanes) return;
-  for (int e = threadIdx.x - tl * px; e < per_tok; e += px) {
-    const int h = e / pr, d = (e - h * pr) * VEC;
+  for (int buf = 0; t0 < p.total; t0 += step, buf ^= 1) {
+    const int tn = static_cast<int>(min(static_cast<int64_t>(TB), p.total - t0));
+    look_up(t0 + step, buf ^ 1);
+    const int64_t* const s_page = sh_page[buf];
+    const int *const s_row = sh_row[buf], *const s_group = sh_group[buf];
+    for (int e = threadIdx.x - tl * px; e < per_tok && tl < lanes; e += px) {
+      const int h = e / pr, d = (e - h * pr) * VEC;
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const Kv8Plane& pl = c.plane[w];
-      T* const y = static_cast<T*>(p.y[w]) + h * p.sy[w][1] + d * (VEC > 1 ? 1 : p.sy[w][2]);
-      const uint8_t* const code = pl.code + h * pl.sc[1] + d * (VEC > 1 ? 1 : pl.sc[3]);
-      const float* const scale = pl.scale + h * pl.ss[1];
+      for (int w = 0; w < 2; ++w) {
+        const Kv8Plane& pl = c.plane[w];
+        T* const y = static_cast<T*>(p.y[w]) + h * p.sy[w][1] + d * (VEC > 1 ? 1 : p.sy[w][2]);
+        const uint8_t* const code = pl.code + h * pl.sc[1] + d * (VEC > 1 ? 1 : pl.sc[3]);
+        const float* const scale = pl.scale + h * pl.ss[1];
 #pragma unroll 4
-      for (int ti = tl; ti < tn; ti += lanes) {
-        const int64_t page = s_page[ti];
-        const int row = s_row[ti];
-        T* const out = y + (t0 + ti) * p.sy[w][0];
-        if (VEC == 16) {
-          uint4 q = make_uint4(0, 0, 0, 0);
-          float sc = 0.f;
-          if (page >= 0) {
-            q = *reinterpret_cast<const uint4*>(code + page * pl.sc[0] + row * pl.sc[2]);
-            sc = scale[page * pl.ss[0] + s_group[ti] * pl.ss[2]];
-          }
-          const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-          float f[16];
+        for (int ti = tl; ti < tn; ti += lanes) {
+          const int64_t page = s_page[ti];
+          const int row = s_row[ti];
+          T* const out = y + (t0 + ti) * p.sy[w][0];
+          if (VEC == 16) {
+            uint4 q = make_uint4(0, 0, 0, 0);
+            float sc = 0.f;
+            if (page >= 0) {
+              q = *reinterpret_cast<const uint4*>(code + page * pl.sc[0] + row * pl.sc[2]);
+              sc = scale[page * pl.ss[0] + s_group[ti] * pl.ss[2]];
+            }
+            const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+            float f[16];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) kv8_dec4<CODE>(u[k], f + 4 * k);
+            for (int k = 0; k < 4; ++k) kv8_dec4<CODE>(u[k], f + 4 * k);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) f[k] *= sc;
-          if constexpr (sizeof(T) == 2) {
-            uint32_t o[8];
+            for (int k = 0; k < 16; ++k) f[k] *= sc;
+            if constexpr (sizeof(T) == 2) {
+              uint32_t o[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) o[k] = Elem<T>::pack2(f[2 * k], f[2 * k + 1]);
-            reinterpret_cast<uint4*>(out)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-            reinterpret_cast<uint4*>(out)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+              for (int k = 0; k < 8; ++k) o[k] = Elem<T>::pack2(f[2 * k], f[2 * k + 1]);
+              reinterpret_cast<uint4*>(out)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+              reinterpret_cast<uint4*>(out)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                reinterpret_cast<float4*>(out)[k] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+            }
           } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              reinterpret_cast<float4*>(out)[k] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+            float v = 0.f;
+            if (page >= 0) v = Kv8<CODE>::dec(code[page * pl.sc[0] + row * pl.sc[2]]) * scale[page * pl.ss[0] + s_group[ti] * pl.ss[2]];
+            *out = Elem<T>::from_f(v);
           }
-        } else {
-          float v = 0.f;
-          if (page >= 0) v = Kv8<CODE>::dec(code[page * pl.sc[0] + row * pl.sc[2]]) * scale[page * pl.ss[0] + s_group[ti] * pl.ss[2]];
-          *out = Elem<T>::from_f(v);
         }
       }
     }
+    __syncthreads();
   }
 }
 
@@ -382,9 +398,11 @@ int kv8_read_launch(const Kv8View& c, int code_type, const int32_t* cu, const in
   p.total = total;
   const int size = dtype == kF32 ? 4 : 2;
   const bool vec = codes_vec_ok(c, 16) && rows_vec_ok(k, sk, size) && rows_vec_ok(v, sv, size);
-  // tokens of a CTA (one lookup of their pages each): fewer where SMs would be left without one
-  const int tb = total >= 32 * 8 * num_sms() ? 32 : total >= 16 * 4 * num_sms() ? 16 : total >= 4 * 2 * num_sms() ? 4 : 2;
-  const unsigned grid = static_cast<unsigned>((total + tb - 1) / tb);
+  // tokens of a block: fewer where the GPU would not be filled
+  const int64_t want = RCT * static_cast<int64_t>(num_sms());
+  const int tb = total >= kReadTokens * want ? kReadTokens : total >= 8 * want ? 8 : total >= 4 * want / 2 ? 4 : 2;
+  const int64_t blocks = (total + tb - 1) / tb;
+  const unsigned grid = static_cast<unsigned>(blocks < want ? blocks : want);
   note_kernel("kv8_read");
   TAK_BY_DTYPE(dtype, TAK_BY_CODE(code_type, {
     if (vec) kv8_read_kernel<T, CODE, 16><<<grid, 256, 0, st>>>(p, tb);
