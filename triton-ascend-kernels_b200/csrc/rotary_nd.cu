@@ -22,20 +22,20 @@ struct RotaryParams {
   int axes, T, H, Hkv, D, rot, interleaved, inverse;
 };
 
-__device__ __forceinline__ float2 rotary_cos_sin(const RotaryParams& p, int position, double freq) {
-  const double turns = static_cast<double>(position) * freq;  // angle / pi
+__device__ __forceinline__ float2 rotary_cos_sin(const RotaryParams& p, int position, float inv_freq) {
+  const double turns = static_cast<double>(position) * static_cast<double>(inv_freq) * 0.31830988618379067154;  // angle / pi
   const float r = static_cast<float>(turns - 2.0 * rint(0.5 * turns));
   float s, c;
   sincospif(r, &s, &c);
   return make_float2(c, p.inverse ? -s : s);
 }
 
-// A CTA walks blocks of TB tokens (and, for few tokens, a share of their heads).
-// A block's TB * rot / 2 cosines and sines are made once, while the block before
-// it is turned (two tables); each thread then keeps the ones of its piece of a head
-// in registers and walks the heads.  VEC = 16 bytes per access where the layout
-// allows, else one element.  Bound by the loads in flight: 16381 tokens x 72 heads
-// of 128 (fp16) take FIGURE.
+// A warp turns one token's heads, or a share of them where there are few tokens: it
+// makes the token's rot / 2 cosines and sines in shared memory of its own (no CTA
+// barrier), each lane keeps the ones of its piece of a head in registers and walks
+// the heads, the next heads' loads in flight while it turns these; the first are
+// issued before the table is made.  VEC = 16 bytes per access where the layout
+// allows, else one element.
 template <typename T, int VEC> struct RotVec;
 template <typename T> struct RotVec<T, 1> {
   T e[1];
@@ -79,108 +79,88 @@ template <typename T> __device__ __forceinline__ void rot_halves(RotVec<T, 1>& a
 }
 
 template <typename T, int VEC, bool IL>
-__global__ void __launch_bounds__(256, 4) rotary_nd_kernel(const __grid_constant__ RotaryParams p, int TB, int heads_per_cta) {
+__global__ void __launch_bounds__(256, 4) rotary_nd_kernel(const __grid_constant__ RotaryParams p, int shares, int per_share) {
   using V = RotVec<T, VEC>;
-  extern __shared__ float2 tables[];  // [2][TB][rot / 2]
-  const int h0 = blockIdx.y * heads_per_cta, hn = min(heads_per_cta, p.H + p.Hkv - h0);
+  extern __shared__ float2 tables[];  // [8 warps][rot / 2]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int half = p.rot / 2;
-  // items of a head: pieces of VEC pairs (half-split: two vectors; interleaved:
-  // VEC / 2 pairs in one vector), then the vectors that pass through
-  const int turn = IL && VEC > 1 ? p.rot / VEC : half / VEC, rest = (p.D - p.rot) / VEC, per_head = turn + rest;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + warp;
+  const int64_t t = unit / shares;
+  if (t >= p.T) return;
+  const int h0 = static_cast<int>(unit - t * shares) * per_share, h1 = min(h0 + per_share, p.H + p.Hkv);
+  // pieces of a head: VEC pairs (half-split: two vectors; interleaved: VEC / 2 pairs
+  // in one vector), then the vectors that pass through
+  const int turn = IL && VEC > 1 ? p.rot / VEC : half / VEC, per_head = turn + (p.D - p.rot) / VEC;
+  const int px = per_head < 32 ? per_head : 32, lanes = 32 / px, hl = lane / px;
   constexpr int NCS = VEC == 1 ? 1 : IL ? VEC / 2 : VEC;  // pairs of a piece
-  const int px = per_head < 256 ? per_head : 256, lanes = 256 / px;
-  const int hl = threadIdx.x / px;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * TB;
+  constexpr bool TWO = !IL || VEC == 1;                   // a piece is two vectors
+  constexpr int MLP = TWO ? 2 : 4;                        // heads in flight
+  float2* const table = tables + warp * half;
+  bool made = false;
 
-  // a thread's table entries have the same pair (and frequency) in every block
-  // when TB * half entries fit the threads; else they are looked up each time
-  const bool one = TB * half <= 256;
-  const int my_t = half > 0 ? threadIdx.x / half : 0, my_i = half > 0 ? threadIdx.x - my_t * half : 0;
-  const bool makes = one && my_t < TB && half > 0;
-  auto axis_of = [&](int i) {
-    int axis = 0;
-    while (axis < p.axes - 1 && i >= p.section_end[axis]) ++axis;
-    return axis;
-  };
-  constexpr double kInvPi = 0.31830988618379067154;
-  const int axis = makes ? axis_of(my_i) : 0;
-  const double freq = makes ? static_cast<double>(p.inv_freq[my_i]) * kInvPi : 0.0;
-  auto position = [&](int64_t t0) {
-    return makes && t0 + my_t < p.T ? p.positions[(t0 + my_t) * p.sp[0] + axis * p.sp[1]] : 0;
-  };
-  auto make_table = [&](int64_t t0, int pos, float2* table) {
-    if (one) {
-      if (makes) table[threadIdx.x] = rotary_cos_sin(p, pos, freq);
-    } else {
-      for (int e = threadIdx.x; e < TB * half; e += 256) {
-        const int ti = e / half, i = e - ti * half;
-        if (t0 + ti < p.T)
-          table[e] = rotary_cos_sin(p, p.positions[(t0 + ti) * p.sp[0] + axis_of(i) * p.sp[1]],
-                                    static_cast<double>(p.inv_freq[i]) * kInvPi);
-      }
-    }
-  };
-
-  int64_t t0 = static_cast<int64_t>(blockIdx.x) * TB;
-  int buf = 0;
-  make_table(t0, position(t0), tables);
-  __syncthreads();
-  for (; t0 < p.T; t0 += step, buf ^= 1) {
-    const float2* const table = tables + buf * TB * half;
-    const int tn = static_cast<int>(min(static_cast<int64_t>(TB), p.T - t0));
-    const bool more = t0 + step < p.T;
-    const int next_pos = more ? position(t0 + step) : 0;
-    for (int ti = 0; ti < tn && hl < lanes; ++ti) {
-      const int64_t t = t0 + ti;
-      for (int i = threadIdx.x - hl * px; i < per_head; i += px) {
-        float2 cs[NCS];
-        if (i < turn) {
+  for (int i0 = 0; i0 < per_head; i0 += px) {
+    const int i = i0 + lane - hl * px;
+    const bool live = hl < lanes && i < per_head;
+    // first element of the piece, and of its partner half
+    const int da = i >= turn ? p.rot + (i - turn) * VEC : IL ? (VEC > 1 ? i * VEC : 2 * i) : i * VEC;
+    const int db = IL ? da + 1 : da + half;
+    float2 cs[NCS];
+    // q's heads of this share, then k's (apart, so that each has fixed strides)
 #pragma unroll
-          for (int k = 0; k < NCS; ++k) cs[k] = table[ti * half + i * NCS + k];
+    for (int w = 0; w < 2; ++w) {
+      const int lo = (w ? max(h0, p.H) - p.H : h0) + hl, hi = w ? h1 - p.H : min(h1, p.H);
+      const int64_t dx = VEC > 1 ? 1 : p.sx[w][2], dy = VEC > 1 ? 1 : p.sy[w][2];
+      const T* x = static_cast<const T*>(p.x[w]) + t * p.sx[w][0] + lo * p.sx[w][1] + da * dx;
+      T* y = static_cast<T*>(p.y[w]) + t * p.sy[w][0] + lo * p.sy[w][1] + da * dy;
+      const int64_t xs = lanes * p.sx[w][1], ys = lanes * p.sy[w][1], xb = (db - da) * dx, yb = (db - da) * dy;
+      V a[MLP], b[MLP];
+      auto load = [&](int h) {
+#pragma unroll
+        for (int u = 0; u < MLP; ++u)
+          if (live && h + u * lanes < hi) {
+            a[u] = *reinterpret_cast<const V*>(x + u * xs);
+            if (TWO && i < turn) b[u] = *reinterpret_cast<const V*>(x + u * xs + xb);
+          }
+        x += MLP * xs;
+      };
+      load(lo);
+      if (!made) {  // the token's table, once, under the first loads
+        for (int e = lane; e < half; e += 32) {
+          int axis = 0;
+          while (axis < p.axes - 1 && e >= p.section_end[axis]) ++axis;
+          table[e] = rotary_cos_sin(p, p.positions[t * p.sp[0] + axis * p.sp[1]], p.inv_freq[e]);
         }
-        // first element of the piece, and of its partner half
-        const int da = i >= turn ? p.rot + (i - turn) * VEC : IL ? (VEC > 1 ? i * VEC : 2 * i) : i * VEC;
-        const int db = IL ? da + 1 : da + half;
-        // q's heads of this CTA, then k's (apart, so that each has fixed strides)
+        __syncwarp();
+        made = true;
+      }
+      if (w == 0 && live && i < turn) {
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int lo = w ? max(h0, p.H) : h0, hi = w ? h0 + hn : min(h0 + hn, p.H), off = w ? p.H : 0;
-          const T* const x0 = static_cast<const T*>(p.x[w]) + t * p.sx[w][0];
-          T* const y0 = static_cast<T*>(p.y[w]) + t * p.sy[w][0];
-          const int64_t dx = VEC > 1 ? 1 : p.sx[w][2], dy = VEC > 1 ? 1 : p.sy[w][2];
-          constexpr int MLP = VEC == 1 ? 1 : IL ? 4 : 2;  // heads in flight
-          for (int h = lo + hl; h < hi; h += MLP * lanes) {
-            V a[MLP], b[MLP];
+        for (int k = 0; k < NCS; ++k) cs[k] = table[i * NCS + k];
+      }
+      for (int h = lo; h < hi; h += MLP * lanes) {
+        V c[MLP], d[MLP];
 #pragma unroll
-            for (int u = 0; u < MLP; ++u) {
-              const int hh = h + u * lanes;
-              if (hh < hi) {
-                const T* x = x0 + (hh - off) * p.sx[w][1];
-                a[u] = *reinterpret_cast<const V*>(x + da * dx);
-                if ((!IL || VEC == 1) && i < turn) b[u] = *reinterpret_cast<const V*>(x + db * dx);
-              }
-            }
+        for (int u = 0; u < MLP; ++u) {
+          c[u] = a[u];
+          if (TWO) d[u] = b[u];
+        }
+        load(h + MLP * lanes);
 #pragma unroll
-            for (int u = 0; u < MLP; ++u) {
-              const int hh = h + u * lanes;
-              if (hh >= hi) continue;
-              T* y = y0 + (hh - off) * p.sy[w][1];
-              if (i < turn) {
-                if constexpr (IL && VEC > 1) {
-                  rot_interleaved<T>(a[u], cs);
-                } else {
-                  rot_halves<T>(a[u], b[u], cs);
-                  *reinterpret_cast<V*>(y + db * dy) = b[u];
-                }
-              }
-              *reinterpret_cast<V*>(y + da * dy) = a[u];
+        for (int u = 0; u < MLP; ++u) {
+          if (!live || h + u * lanes >= hi) continue;
+          if (i < turn) {
+            if constexpr (!TWO) {
+              rot_interleaved<T>(c[u], cs);
+            } else {
+              rot_halves<T>(c[u], d[u], cs);
+              *reinterpret_cast<V*>(y + u * ys + yb) = d[u];
             }
           }
+          *reinterpret_cast<V*>(y + u * ys) = c[u];
         }
+        y += MLP * ys;
       }
     }
-    if (more) make_table(t0 + step, next_pos, tables + (buf ^ 1) * TB * half);
-    __syncthreads();
   }
 }
 
@@ -203,23 +183,19 @@ static void rotary_launch_t(const RotaryArgs& a, const RotaryParams& p, cudaStre
   constexpr int VEC = 16 / sizeof(T);
   const bool vec = rotary_vec_ok(a, VEC);
   const int heads = a.num_q_heads + a.num_kv_heads, half = a.rot_dim / 2;
-  // tokens of a block: about one table entry a thread; fewer tokens than that fills
-  // the GPU with CTAs over shares of the heads instead
-  int tb = half > 0 ? 256 / half : 4;
-  if (tb > 4) tb = 4;
-  if (tb < 1) tb = 1;
-  const int want = 4 * num_sms();
-  while (tb > 1 && (a.total_tokens + tb - 1) / tb < want) tb = (tb + 1) / 2;
-  const int blocks = (a.total_tokens + tb - 1) / tb, ctas = blocks < want ? blocks : want;
-  int split = ctas < want / 2 ? want / 2 / ctas : 1;
-  if (split > (heads + 3) / 4) split = (heads + 3) / 4;
-  const int per = (heads + split - 1) / split;
-  const dim3 grid(ctas, (heads + per - 1) / per);
-  const size_t smem = static_cast<size_t>(2 * tb) * half * sizeof(float2);
-  if (vec && a.interleaved) rotary_nd_kernel<T, VEC, true><<<grid, 256, smem, st>>>(p, tb, per);
-  else if (vec) rotary_nd_kernel<T, VEC, false><<<grid, 256, smem, st>>>(p, tb, per);
-  else if (a.interleaved) rotary_nd_kernel<T, 1, true><<<grid, 256, smem, st>>>(p, tb, per);
-  else rotary_nd_kernel<T, 1, false><<<grid, 256, smem, st>>>(p, tb, per);
+  // a warp per token; with fewer tokens than warps that fill the GPU, a warp per
+  // token and share of its heads (at least four, as each share makes the table)
+  int64_t shares = 16 * static_cast<int64_t>(num_sms()) / a.total_tokens;
+  if (shares > heads / 4) shares = heads / 4;
+  if (shares < 1) shares = 1;
+  const int per = (heads + static_cast<int>(shares) - 1) / static_cast<int>(shares);
+  shares = (heads + per - 1) / per;
+  const unsigned grid = static_cast<unsigned>((a.total_tokens * shares + 7) / 8);
+  const size_t smem = static_cast<size_t>(8) * half * sizeof(float2);
+  if (vec && a.interleaved) rotary_nd_kernel<T, VEC, true><<<grid, 256, smem, st>>>(p, static_cast<int>(shares), per);
+  else if (vec) rotary_nd_kernel<T, VEC, false><<<grid, 256, smem, st>>>(p, static_cast<int>(shares), per);
+  else if (a.interleaved) rotary_nd_kernel<T, 1, true><<<grid, 256, smem, st>>>(p, static_cast<int>(shares), per);
+  else rotary_nd_kernel<T, 1, false><<<grid, 256, smem, st>>>(p, static_cast<int>(shares), per);
 }
 
 int rotary_nd_launch(const RotaryArgs& a, cudaStream_t st) {
