@@ -300,90 +300,103 @@ struct Kv8ReadParams {
   int64_t total;
 };
 
-// A CTA walks blocks of TB tokens: while it converts one, its first warps look up
-// the pages of the next, so only the first block waits for the chain of loads
-// (sequence, block table).  Every thread converts pieces of VEC codes (16: one load,
-// 32 bytes of 16-bit values or 64 of fp32 out).
-constexpr int kReadTokens = 32;
-constexpr int RCT = 4;
+// A warp reads TB (at most 32) consecutive tokens: lane i looks up token i's page,
+// then the warp walks the tokens with each lane on its piece of a head, K and V
+// together, the next token's codes in flight while these are converted.  VEC codes a
+// piece (16: one load, 32 bytes of 16-bit values or 64 of fp32 out).
+template <typename T, int VEC> struct Kv8Piece;
+template <typename T> struct Kv8Piece<T, 16> {
+  uint4 q;
+  __device__ __forceinline__ void load(const uint8_t* x) { q = *reinterpret_cast<const uint4*>(x); }
+  template <int CODE> __device__ __forceinline__ void store(T* out, float sc) const {
+    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+    float f[16];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) kv8_dec4<CODE>(u[k], f + 4 * k);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) f[k] *= sc;
+    if constexpr (sizeof(T) == 2) {
+      uint32_t o[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o[k] = Elem<T>::pack2(f[2 * k], f[2 * k + 1]);
+      reinterpret_cast<uint4*>(out)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+      reinterpret_cast<uint4*>(out)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        reinterpret_cast<float4*>(out)[k] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+    }
+  }
+};
+template <typename T> struct Kv8Piece<T, 1> {
+  uint8_t q;
+  __device__ __forceinline__ void load(const uint8_t* x) { q = *x; }
+  template <int CODE> __device__ __forceinline__ void store(T* out, float sc) const {
+    *out = Elem<T>::from_f(Kv8<CODE>::dec(q) * sc);
+  }
+};
 
 template <typename T, int CODE, int VEC>
-__global__ void __launch_bounds__(256, RCT) kv8_read_kernel(const __grid_constant__ Kv8ReadParams p, int TB) {
+__global__ void __launch_bounds__(256, 4) kv8_read_kernel(const __grid_constant__ Kv8ReadParams p, int TB) {
   const Kv8View& c = p.c;
-  __shared__ int64_t sh_page[2][kReadTokens];
-  __shared__ int sh_row[2][kReadTokens], sh_group[2][kReadTokens];
-  auto look_up = [&](int64_t t0, int buf) {
-    const int64_t t = t0 + threadIdx.x;
-    if (threadIdx.x >= TB || t >= p.total) return;
+  const int lane = threadIdx.x & 31;
+  const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * TB;
+  const int tn = static_cast<int>(min(static_cast<int64_t>(TB), p.total - t0));
+  if (tn <= 0) return;
+  int my_page = -1, my_row = 0;
+  if (lane < tn) {
+    const int64_t t = t0 + lane;
     const int s = find_slot_seq(p.cu, c.num_seqs, t);
     const int lo = p.cu[s];
-    const bool in_seq = t >= lo && t < p.cu[s + 1];
-    const int64_t pos = in_seq ? t - lo + (p.start_lens ? p.start_lens[s] : 0) : -1;
-    const int64_t page = kv8_page(c, s, pos);
-    const int row = page >= 0 ? static_cast<int>(static_cast<uint32_t>(pos) % static_cast<uint32_t>(c.P)) : 0;
-    sh_page[buf][threadIdx.x] = page;
-    sh_row[buf][threadIdx.x] = row;
-    sh_group[buf][threadIdx.x] = static_cast<uint32_t>(row) / static_cast<uint32_t>(c.group);
-  };
-  const int64_t step = static_cast<int64_t>(gridDim.x) * TB;
-  int64_t t0 = static_cast<int64_t>(blockIdx.x) * TB;
-  look_up(t0, 0);
-  __syncthreads();
-  // a thread keeps its piece of a token (head and columns) and walks the tokens
+    if (t >= lo && t < p.cu[s + 1]) {
+      const int64_t pos = t - lo + (p.start_lens ? p.start_lens[s] : 0);
+      my_page = static_cast<int>(kv8_page(c, s, pos));  // num_blocks < 2^31
+      if (my_page >= 0) my_row = static_cast<uint32_t>(pos) % static_cast<uint32_t>(c.P);
+    }
+  }
   const int pr = c.D / VEC, per_tok = c.Hkv * pr;
-  const int px = per_tok < 256 ? per_tok : 256, lanes = 256 / px;
-  const int tl = threadIdx.x / px;
-  for (int buf = 0; t0 < p.total; t0 += step, buf ^= 1) {
-    const int tn = static_cast<int>(min(static_cast<int64_t>(TB), p.total - t0));
-    look_up(t0 + step, buf ^ 1);
-    const int64_t* const s_page = sh_page[buf];
-    const int *const s_row = sh_row[buf], *const s_group = sh_group[buf];
-    for (int e = threadIdx.x - tl * px; e < per_tok && tl < lanes; e += px) {
-      const int h = e / pr, d = (e - h * pr) * VEC;
+  for (int e = lane; e < (per_tok + 31) / 32 * 32; e += 32) {
+    const bool live = e < per_tok;
+    const int h = live ? e / pr : 0, d = live ? (e - h * pr) * VEC : 0;
+    const uint8_t* code[2];
+    const float* scale[2];
+    T* out[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      code[w] = c.plane[w].code + h * c.plane[w].sc[1] + d * (VEC > 1 ? 1 : c.plane[w].sc[3]);
+      scale[w] = c.plane[w].scale + h * c.plane[w].ss[1];
+      out[w] = static_cast<T*>(p.y[w]) + t0 * p.sy[w][0] + h * p.sy[w][1] + d * (VEC > 1 ? 1 : p.sy[w][2]);
+    }
+    Kv8Piece<T, VEC> next[2];
+    float next_sc[2];
+    auto load = [&](int i) {
+      const int page = __shfl_sync(0xffffffffu, my_page, i), row = __shfl_sync(0xffffffffu, my_row, i);
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        const Kv8Plane& pl = c.plane[w];
-        T* const y = static_cast<T*>(p.y[w]) + h * p.sy[w][1] + d * (VEC > 1 ? 1 : p.sy[w][2]);
-        const uint8_t* const code = pl.code + h * pl.sc[1] + d * (VEC > 1 ? 1 : pl.sc[3]);
-        const float* const scale = pl.scale + h * pl.ss[1];
-#pragma unroll 4
-        for (int ti = tl; ti < tn; ti += lanes) {
-          const int64_t page = s_page[ti];
-          const int row = s_row[ti];
-          T* const out = y + (t0 + ti) * p.sy[w][0];
-          if (VEC == 16) {
-            uint4 q = make_uint4(0, 0, 0, 0);
-            float sc = 0.f;
-            if (page >= 0) {
-              q = *reinterpret_cast<const uint4*>(code + page * pl.sc[0] + row * pl.sc[2]);
-              sc = scale[page * pl.ss[0] + s_group[ti] * pl.ss[2]];
-            }
-            const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-            float f[16];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) kv8_dec4<CODE>(u[k], f + 4 * k);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) f[k] *= sc;
-            if constexpr (sizeof(T) == 2) {
-              uint32_t o[8];
-#pragma unroll
-              for (int k = 0; k < 8; ++k) o[k] = Elem<T>::pack2(f[2 * k], f[2 * k + 1]);
-              reinterpret_cast<uint4*>(out)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-              reinterpret_cast<uint4*>(out)[1] = make_uint4(o[4], o[5], o[6], o[7]);
-            } else {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                reinterpret_cast<float4*>(out)[k] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
-            }
-          } else {
-            float v = 0.f;
-            if (page >= 0) v = Kv8<CODE>::dec(code[page * pl.sc[0] + row * pl.sc[2]]) * scale[page * pl.ss[0] + s_group[ti] * pl.ss[2]];
-            *out = Elem<T>::from_f(v);
-          }
+        next[w] = {};
+        next_sc[w] = 0.f;
+        if (page >= 0 && live) {
+          next[w].load(code[w] + page * c.plane[w].sc[0] + row * c.plane[w].sc[2]);
+          next_sc[w] = scale[w][page * c.plane[w].ss[0] + static_cast<uint32_t>(row) / static_cast<uint32_t>(c.group) * c.plane[w].ss[2]];
         }
       }
+    };
+    load(0);
+    for (int i = 0; i < tn; ++i) {
+      Kv8Piece<T, VEC> now[2];
+      float sc[2];
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        now[w] = next[w];
+        sc[w] = next_sc[w];
+      }
+      if (i + 1 < tn) load(i + 1);
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        if (live) now[w].template store<CODE>(out[w], sc[w]);
+        out[w] += p.sy[w][0];
+      }
     }
-    __syncthreads();
   }
 }
 
@@ -398,11 +411,11 @@ int kv8_read_launch(const Kv8View& c, int code_type, const int32_t* cu, const in
   p.total = total;
   const int size = dtype == kF32 ? 4 : 2;
   const bool vec = codes_vec_ok(c, 16) && rows_vec_ok(k, sk, size) && rows_vec_ok(v, sv, size);
-  // tokens of a block: fewer where the GPU would not be filled
-  const int64_t want = RCT * static_cast<int64_t>(num_sms());
-  const int tb = total >= kReadTokens * want ? kReadTokens : total >= 8 * want ? 8 : total >= 4 * want / 2 ? 4 : 2;
-  const int64_t blocks = (total + tb - 1) / tb;
-  const unsigned grid = static_cast<unsigned>(blocks < want ? blocks : want);
+  // tokens of a warp (their pages are looked up in one go): fewer where the GPU
+  // would not be filled
+  const int64_t warps = 32 * static_cast<int64_t>(num_sms());
+  const int tb = total >= 16 * 2 * warps ? 16 : total >= 4 * warps ? 8 : total >= warps ? 2 : 1;
+  const unsigned grid = static_cast<unsigned>((total + 8 * tb - 1) / (8 * tb));
   note_kernel("kv8_read");
   TAK_BY_DTYPE(dtype, TAK_BY_CODE(code_type, {
     if (vec) kv8_read_kernel<T, CODE, 16><<<grid, 256, 0, st>>>(p, tb);
