@@ -21,8 +21,8 @@
 //
 // A CTA: one producer warp streams chunks through a ring of TMA loads (K and V
 // codes, page ids from the block table) with the tiles' scales beside them; NW
-// warps consume: WM of them across the query rows (8 each), NW / WM across
-// the key tiles.
+// warps consume, in one of two ways: up to eight query rows (Kv8Few), or 16 and 32
+// (Kv8Many; more rows are chunks of 32 that share the L2's copy of the cache).
 #include <cstdio>
 
 #include "kv8.cuh"
@@ -45,10 +45,10 @@ struct Kv8TcParams {
   float cap2, inv_cap;  // softcap * log2(e), 2 log2(e) / softcap; 0: no cap
   // workspace
   int4* bound;       // [N] first chunk of each CTA: {sequence, item of it, chunk of the item, chunks of the item}
-  float* part_o;     // [N][2][8 WM][DP]
-  float* part_ml;    // [N][2][8 WM][2]
+  float* part_o;     // [N][2][RT][DP]
+  float* part_ml;    // [N][2][RT][2]
   float* lse2;       // [B, Hkv, rows] (weights only)
-  float* scores;     // [B, Hkv, chunks, 8 WM, score_ld] (weights only)
+  float* scores;     // [B, Hkv, chunks, RT, score_ld] (weights only)
   int64_t score_ld;
 };
 
@@ -66,26 +66,50 @@ constexpr float kHalfMin = 6.103515625e-5f;  // 2^-14: fp16's smallest normal nu
 constexpr int kFew = 8;
 constexpr float kMinVs = 6.162975822039155e-33f;  // 2^-107: the smallest scale that the write makes
 
-// DP: head dim rounded up to 64, 128 or 256.  A warp holds eight query rows; WM
-// warps stand across the rows, the rest across the key tiles.
-template <int DP, int WM> struct Kv8Cfg {
+// DP: head dim rounded up to 64, 128 or 256.
+template <int DP> struct Kv8Base {
   static constexpr int NW = DP >= 256 ? 8 : 4;          // consumer warps
   static constexpr int CH = 128;                        // keys of a chunk
-  static constexpr int TP = DP >= 256 ? 1 : 2;          // key tiles of a warp's step (two: independent MMA chains)
+  static constexpr int TP = CH / 16 / NW;               // key tiles of a warp's step (two: independent MMA chains)
   static constexpr int NT = CH / 16;                    // key tiles of a chunk
   static constexpr int CB = DP >= 256 ? 2 : 1;          // column blocks of a row
   static constexpr int ROWB = DP >= 128 ? 128 : 64;     // bytes of a row in a column block
   static constexpr int PLANE = CH * DP;                 // bytes of K (or V) in a stage
   static constexpr int STAGE = 2 * PLANE;
-  static constexpr int CTAS = DP >= 256 ? 1 : 3;        // per SM
   static constexpr int NS = DP == 64 ? 4 : 2;
+  static constexpr int THREADS = (NW + 1) * 32;
+  static constexpr int META_OFF = NS * STAGE;           // [NS][3][NT] floats: ks, log2 vs + kPBias, 2^-23 / vs
+  static constexpr int BAR_OFF = META_OFF + NS * 3 * NT * 4;
+  static constexpr int OWN_OFF = BAR_OFF + 2 * NS * 8;  // the kernel's own shared memory
+};
+// Up to eight query rows: every warp holds all of O for its key tiles, and the
+// warps join at the end of an item.
+template <int DP> struct Kv8Few : Kv8Base<DP> {
+  using B = Kv8Base<DP>;
+  static constexpr int RT = 8;
+  static constexpr int CTAS = DP >= 256 ? 1 : 3;        // per SM
   static constexpr int DH = 32;                         // columns joined at a time
   static constexpr int OLD = DH + 8;                    // row stride of the joining buffer (bank spread)
-  static constexpr int META_OFF = NS * STAGE;           // [NS][3][NT] floats: ks, log2 vs + kPBias, 2^-23 / vs
-  static constexpr int OBUF_OFF = META_OFF + NS * 3 * NT * 4;  // [NW][8][OLD] floats
-  static constexpr int ML_OFF = OBUF_OFF + NW * 8 * OLD * 4;   // [NW][8][2]
-  static constexpr int BAR_OFF = ML_OFF + NW * 8 * 2 * 4;
-  static constexpr int SMEM = BAR_OFF + 2 * NS * 8 + 64 + 1024;
+  static constexpr int OBUF_OFF = B::OWN_OFF;           // [NW][8][OLD] floats
+  static constexpr int ML_OFF = OBUF_OFF + B::NW * 8 * OLD * 4;  // [NW][8][2]
+  static constexpr int SMEM = ML_OFF + B::NW * 8 * 2 * 4 + 1024;
+  static_assert((SMEM + 1024) * CTAS <= 228 * 1024, "shared memory");
+};
+// 16 or 32 query rows (8 NR): a warp scores its key tiles for all rows, the weights
+// go to the other warps through shared memory, and each warp sums its share of the
+// columns over all keys of the chunk, so that a code is converted once per CTA.
+template <int DP, int NR> struct Kv8Many : Kv8Base<DP> {
+  using B = Kv8Base<DP>;
+  static constexpr int RT = 8 * NR;
+  static constexpr int CTAS = DP >= 256 ? 1 : 2;        // per SM
+  static constexpr int CW = DP / B::NW;                 // columns of a warp
+  static constexpr int MB = CW / 16;
+  static constexpr int Q_OFF = (B::OWN_OFF + 15) / 16 * 16;        // [DP / 16][NR][32 lanes] uint2: Q fragments
+  static constexpr int P_OFF = Q_OFF + DP / 16 * NR * 256;         // [2][NT][NR][32 lanes] uint2: P fragments, and those apart
+  static constexpr int FAC_OFF = P_OFF + 2 * B::NT * NR * 256;     // [RT] floats
+  static constexpr int MAX_OFF = FAC_OFF + RT * 4;                 // [NW][RT] floats
+  static constexpr int FLAG_OFF = MAX_OFF + B::NW * RT * 4;        // [2][NW] ints
+  static constexpr int SMEM = FLAG_OFF + 2 * B::NW * 4 + 1024;
   static_assert((SMEM + 1024) * CTAS <= 228 * 1024, "shared memory");
 };
 
@@ -178,23 +202,14 @@ template <int CH> struct Kv8Walk {
   __device__ __forceinline__ bool live(const Kv8TcParams& p, int64_t end) const { return at < end && s < p.c.num_seqs; }
 };
 
-template <int CODE, int DP, int WM>
-__global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>::CTAS)
-    kv8_attention_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                            const __grid_constant__ Kv8TcParams p) {
-  using C = Kv8Cfg<DP, WM>;
-  constexpr int NW = C::NW, CH = C::CH, NT = C::NT, TP = C::TP, NS = C::NS, WK = NW / WM, RT = 8 * WM;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* meta = reinterpret_cast<float*>(smem + C::META_OFF);
-  float* obuf = reinterpret_cast<float*>(smem + C::OBUF_OFF);
-  float* mlbuf = reinterpret_cast<float*>(smem + C::ML_OFF);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
-  uint64_t* empty = full + NS;
+// Start of both kernels: barriers, the CTA's share [w0.at, u1) of the work list,
+// zeros for sequences without a key.  False: the CTA has no chunk.
+template <class C>
+__device__ __forceinline__ bool kv8_begin(const Kv8TcParams& p, uint64_t* full, uint64_t* empty, Kv8Walk<C::CH>& w0, int64_t& u1) {
+  constexpr int NW = C::NW, CH = C::CH, NS = C::NS, THREADS = C::THREADS;
   __shared__ int64_t sh_sum[NW + 1];
   __shared__ int64_t sh_base;
   __shared__ int sh_seq;
-  constexpr int THREADS = (NW + 1) * 32;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int B = p.c.num_seqs, items = p.c.Hkv * p.chunks;
 
@@ -227,7 +242,8 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
     total += sh_sum[w];
   }
   const int64_t U = total * items;
-  const int64_t u0 = U * blockIdx.x / gridDim.x, u1 = U * (blockIdx.x + 1) / gridDim.x;
+  const int64_t u0 = U * blockIdx.x / gridDim.x;
+  u1 = U * (blockIdx.x + 1) / gridDim.x;
   before += incl - mine;  // places (of one item) before this thread's sequences
   if (u0 < U && mine > 0 && before * items <= u0 && u0 < (before + mine) * items) {
     int s = s_lo;
@@ -254,9 +270,8 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
   }
   if (u0 >= u1) {
     if (tid == 0) p.bound[blockIdx.x] = make_int4(0, 0, 0, 0);
-    return;
+    return false;
   }
-  Kv8Walk<CH> w0;
   w0.s = sh_seq;
   w0.load(p);
   w0.at = u0;
@@ -265,96 +280,126 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
   if (w0.j >= w0.n) w0.next_item(p, items);  // u0 lies on an item's empty places
   const bool any = w0.live(p, u1);
   if (tid == 0) p.bound[blockIdx.x] = any ? make_int4(w0.s, w0.r, w0.j, w0.n) : make_int4(0, 0, 0, 0);
-  if (!any) return;
+  return any;
+}
 
-  if (warp == NW) {
-    // ---------------- producer ----------------
-    // lane t < NT looks after tile t of a chunk: its page and scales are loaded
-    // one and two chunks ahead, so that no chunk waits on them
-    tma_prefetch_desc(&tmK);
-    tma_prefetch_desc(&tmV);
-    const int nbox = CH / p.box_rows, tiles_per_box = p.box_rows / 16;
-    struct Meta { int64_t page; int row, kvh, ctx, tok0; float ks, vs; };
-    auto fetch_page = [&](const Kv8Walk<CH>& w, bool live) {
-      Meta m{};
-      m.page = -1;
-      m.ctx = w.ctx;
-      m.tok0 = w.j * CH;
-      m.kvh = w.r / p.chunks;
-      const int tok = m.tok0 + lane * 16;
-      if (live && lane < NT && tok < w.ctx) {
-        const int lp = tok / p.c.P;
-        m.row = tok - lp * p.c.P;
-        m.page = p.c.block_tables[w.s * p.c.sbt[0] + lp * p.c.sbt[1]];
-      }
-      return m;
-    };
-    auto fetch_scales = [&](Meta& m) {
-      m.ks = m.vs = 0.f;
-      if (m.page >= 0 && m.page < p.c.num_blocks) {
-        const int g = m.row / p.c.group;
-        m.ks = *kv8_scale(p.c.plane[0], m.page, m.kvh, g);
-        m.vs = *kv8_scale(p.c.plane[1], m.page, m.kvh, g);
-      }
-    };
-    Kv8Walk<CH> w = w0;
-    bool more = true, more2;  // chunks one and two ahead
-    Meta cur = fetch_page(w, true);
-    w.next(p, items);
-    more = w.live(p, u1);
-    Meta nxt = fetch_page(w, more);
-    fetch_scales(cur);
-    for (int it = 0;; ++it) {
-      more2 = more;
-      if (more) {
-        w.next(p, items);
-        more2 = w.live(p, u1);
-        if (more2 && w.j == 0) {  // an item begins two chunks ahead: its query rows to L2
-          const int kvh = w.r / p.chunks, row0 = (w.r - kvh * p.chunks) * RT, lines = DP / 64;
-          for (int e = lane; e < RT * lines; e += 32) {
-            const int row = row0 + e / lines, d = e % lines * 64;
-            if (row < p.rows && d < p.c.D)
-              asm volatile("prefetch.global.L2 [%0];" ::"l"(kv8_q_row(p, w.s, kvh, row) + d * p.sq[3]));
-          }
-        }
-      }
-      Meta far = fetch_page(w, more2);
-      fetch_scales(nxt);
-      const int st = it % NS;
-      if (it >= NS && !__all_sync(0xffffffffu, mbar_wait_sleep(&empty[st], ((it / NS) - 1) & 1))) break;
-      if (lane < NT) {
-        float* mt = meta + st * 3 * NT;
-        const bool bad = !(cur.vs < INFINITY);  // NaN or inf
-        const float v = bad ? 1.f : fmaxf(cur.vs, kMinVs);
-        mt[lane] = cur.ks;
-        mt[NT + lane] = bad ? __uint_as_float(0x7fffffffu) : log2f(v) + kPBias;
-        mt[2 * NT + lane] = kLBiasInv / v;
-      }
-      __syncwarp();
-      const int boxes = min(nbox, (cur.ctx - cur.tok0 + p.box_rows - 1) / p.box_rows);
-      if (lane == 0) mbar_arrive_expect_tx(&full[st], boxes * 2 * C::CB * p.box_rows * C::ROWB);
-      __syncwarp();
-      const int src = lane < nbox ? lane * tiles_per_box : 0;
-      const int page = static_cast<int>(__shfl_sync(0xffffffffu, cur.page, src));
-      const int row = __shfl_sync(0xffffffffu, cur.row, src);
-      if (lane < boxes) {
-        uint8_t* k = smem + st * C::STAGE + lane * p.box_rows * C::ROWB;
-#pragma unroll
-        for (int cb = 0; cb < C::CB; ++cb) {
-          tma_load_4d(k + cb * CH * C::ROWB, &tmK, &full[st], cb * 128, row, cur.kvh, page);
-          tma_load_4d(k + C::PLANE + cb * CH * C::ROWB, &tmV, &full[st], cb * 128, row, cur.kvh, page);
-        }
-      }
-      if (!more) break;
-      cur = nxt;
-      nxt = far;
-      more = more2;
+// The producer warp of both kernels.
+template <class C>
+__device__ __forceinline__ void kv8_produce(const Kv8TcParams& p, const CUtensorMap& tmK, const CUtensorMap& tmV, uint8_t* smem,
+                                            uint64_t* full, uint64_t* empty, const Kv8Walk<C::CH>& w0, int64_t u1) {
+  constexpr int CH = C::CH, NT = C::NT, NS = C::NS, RT = C::RT;
+  const int lane = threadIdx.x & 31, items = p.c.Hkv * p.chunks;
+  float* meta = reinterpret_cast<float*>(smem + C::META_OFF);
+  // lane t < NT looks after tile t of a chunk: its page and scales are loaded
+  // one and two chunks ahead, so that no chunk waits on them
+  tma_prefetch_desc(&tmK);
+  tma_prefetch_desc(&tmV);
+  const int nbox = CH / p.box_rows, tiles_per_box = p.box_rows / 16;
+  struct Meta { int64_t page; int row, kvh, ctx, tok0; float ks, vs; };
+  auto fetch_page = [&](const Kv8Walk<CH>& w, bool live) {
+    Meta m{};
+    m.page = -1;
+    m.ctx = w.ctx;
+    m.tok0 = w.j * CH;
+    m.kvh = w.r / p.chunks;
+    const int tok = m.tok0 + lane * 16;
+    if (live && lane < NT && tok < w.ctx) {
+      const int lp = tok / p.c.P;
+      m.row = tok - lp * p.c.P;
+      m.page = p.c.block_tables[w.s * p.c.sbt[0] + lp * p.c.sbt[1]];
     }
+    return m;
+  };
+  auto fetch_scales = [&](Meta& m) {
+    m.ks = m.vs = 0.f;
+    if (m.page >= 0 && m.page < p.c.num_blocks) {
+      const int g = m.row / p.c.group;
+      m.ks = *kv8_scale(p.c.plane[0], m.page, m.kvh, g);
+      m.vs = *kv8_scale(p.c.plane[1], m.page, m.kvh, g);
+    }
+  };
+  Kv8Walk<CH> w = w0;
+  bool more = true, more2;  // chunks one and two ahead
+  Meta cur = fetch_page(w, true);
+  w.next(p, items);
+  more = w.live(p, u1);
+  Meta nxt = fetch_page(w, more);
+  fetch_scales(cur);
+  for (int it = 0;; ++it) {
+    more2 = more;
+    if (more) {
+      w.next(p, items);
+      more2 = w.live(p, u1);
+      if (more2 && w.j == 0) {  // an item begins two chunks ahead: its query rows to L2
+        const int kvh = w.r / p.chunks, row0 = (w.r - kvh * p.chunks) * RT, lines = C::PLANE / CH / 64;
+        for (int e = lane; e < RT * lines; e += 32) {
+          const int row = row0 + e / lines, d = e % lines * 64;
+          if (row < p.rows && d < p.c.D)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(kv8_q_row(p, w.s, kvh, row) + d * p.sq[3]));
+        }
+      }
+    }
+    Meta far = fetch_page(w, more2);
+    fetch_scales(nxt);
+    const int st = it % NS;
+    if (it >= NS && !__all_sync(0xffffffffu, mbar_wait_sleep(&empty[st], ((it / NS) - 1) & 1))) break;
+    if (lane < NT) {
+      float* mt = meta + st * 3 * NT;
+      const bool bad = !(cur.vs < INFINITY);  // NaN or inf
+      const float v = bad ? 1.f : fmaxf(cur.vs, kMinVs);
+      mt[lane] = cur.ks;
+      mt[NT + lane] = bad ? __uint_as_float(0x7fffffffu) : log2f(v) + kPBias;
+      mt[2 * NT + lane] = kLBiasInv / v;
+    }
+    __syncwarp();
+    const int boxes = min(nbox, (cur.ctx - cur.tok0 + p.box_rows - 1) / p.box_rows);
+    if (lane == 0) mbar_arrive_expect_tx(&full[st], boxes * 2 * C::CB * p.box_rows * C::ROWB);
+    __syncwarp();
+    const int src = lane < nbox ? lane * tiles_per_box : 0;
+    const int page = static_cast<int>(__shfl_sync(0xffffffffu, cur.page, src));
+    const int row = __shfl_sync(0xffffffffu, cur.row, src);
+    if (lane < boxes) {
+      uint8_t* k = smem + st * C::STAGE + lane * p.box_rows * C::ROWB;
+#pragma unroll
+      for (int cb = 0; cb < C::CB; ++cb) {
+        tma_load_4d(k + cb * CH * C::ROWB, &tmK, &full[st], cb * 128, row, cur.kvh, page);
+        tma_load_4d(k + C::PLANE + cb * CH * C::ROWB, &tmV, &full[st], cb * 128, row, cur.kvh, page);
+      }
+    }
+    if (!more) break;
+    cur = nxt;
+    nxt = far;
+    more = more2;
+  }
+}
+
+template <int CODE, int DP>
+__global__ void __launch_bounds__(Kv8Few<DP>::THREADS, Kv8Few<DP>::CTAS)
+    kv8_attention_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                             const __grid_constant__ Kv8TcParams p) {
+  using C = Kv8Few<DP>;
+  constexpr int NW = C::NW, CH = C::CH, NT = C::NT, TP = C::TP, NS = C::NS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const float* meta = reinterpret_cast<const float*>(smem + C::META_OFF);
+  float* obuf = reinterpret_cast<float*>(smem + C::OBUF_OFF);
+  float* mlbuf = reinterpret_cast<float*>(smem + C::ML_OFF);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* empty = full + NS;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int items = p.c.Hkv * p.chunks;
+  Kv8Walk<CH> w0;
+  int64_t u1;
+  __shared__ int sh_fail;
+  if (tid == 0) sh_fail = 0;
+  if (!kv8_begin<C>(p, full, empty, w0, u1)) return;
+  if (warp == NW) {
+    kv8_produce<C>(p, tmK, tmV, smem, full, empty, w0, u1);
     return;
   }
 
   // ---------------- consumers ----------------
-  const int wm = warp % WM, wk = warp / WM, g = lane >> 2, t4 = lane & 3, mi = lane >> 3, rr = lane & 7;
+  const int g = lane >> 2, t4 = lane & 3, mi = lane >> 3, rr = lane & 7;
   const uint32_t sbase = smem_u32(smem);
   Kv8Walk<CH> w = w0;
   int it = 0;
@@ -373,7 +418,7 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
       return p.bf16 ? __uint_as_float(raw << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(raw)));
     };
     uint2 raw[DP / 16];  // all loads in flight at once
-    const int row = rc * RT + wm * 8 + g;
+    const int row = rc * 8 + g;
     const bool real = row < p.rows;
     const uint16_t* src = kv8_q_row(p, s, kvh, real ? row : 0);
 #pragma unroll
@@ -395,7 +440,7 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
     int lim[2];  // keys that a row sees
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int row = rc * RT + wm * 8 + 2 * t4 + k;
+      const int row = rc * 8 + 2 * t4 + k;
       lim[k] = row < p.rows ? ctx - p.Lq + row / p.G + 1 : ctx;  // rows that pad the tile see every key
     }
     float top = 0.f;
@@ -441,22 +486,20 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
       l[k] = 0.f;
       above[k] = 0;
     }
-    // this thread's first row of the stored scores, [item][8 WM rows of each chunk][score_ld]
-    float* const score_row = p.scores + ((static_cast<int64_t>(s) * items + w.r) * RT + wm * 8 + 2 * t4) * p.score_ld;
+    // this thread's first row of the stored scores, [item][eight rows of each chunk of rows][score_ld]
+    float* const score_row = p.scores + ((static_cast<int64_t>(s) * items + w.r) * 8 + 2 * t4) * p.score_ld;
     const int open = ctx - p.Lq + 1;  // keys below it are seen by every row
 
     for (int j = j0; j < j_end; ++j, ++it) {
       const int st = it % NS;
       if (!mbar_wait(&full[st], (it / NS) & 1)) {
-        ok = false;
+        sh_fail = 1;  // read by all warps after the next barrier: they leave together
         break;
       }
       const uint32_t kbase = sbase + st * C::STAGE, vbase = kbase + C::PLANE;
       const float* mt = meta + st * 3 * NT;
-#pragma unroll 1
-      for (int t = wk * TP; t < NT; t += WK * TP) {
-        const int tok = j * CH + t * 16, r0 = t * 16;
-        if (tok >= ctx) break;
+      const int t = warp * TP, tok = j * CH + t * 16, r0 = t * 16;
+      if (tok < ctx) {
         if (CODE == kE4M3 && tok + 16 * TP > ctx) {
           // rows past the end may hold NaN codes: zero their V rows (several
           // warps may write the same zeros)
@@ -685,7 +728,7 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
       l[k] += __shfl_xor_sync(0xffffffffu, l[k], 16);
     }
     const bool whole = j0 == 0 && j_end == w.n;
-    const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (j0 == 0 ? 1 : 0)) * RT;
+    const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (j0 == 0 ? 1 : 0)) * 8;
 #pragma unroll
     for (int dh = 0; dh < DP / C::DH; ++dh) {
       asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");  // the buffer is free again
@@ -702,20 +745,19 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
           *reinterpret_cast<float2*>(mlbuf + (warp * 8 + 2 * t4 + k) * 2) = make_float2(m[k], l[k]);
       }
       asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory");
-      for (int e = tid; e < RT * (C::DH / 4); e += NW * 32) {
+      for (int e = tid; e < 8 * (C::DH / 4); e += NW * 32) {
         const int row = e / (C::DH / 4), d = (e - row * (C::DH / 4)) * 4;
-        const int grow = rc * RT + row;
+        const int grow = rc * 8 + row;
         if (grow >= p.rows) continue;
-        const int tile = row >> 3, rw = row & 7;
         float M = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < WK; ++k) M = fmaxf(M, mlbuf[((k * WM + tile) * 8 + rw) * 2]);
+        for (int k = 0; k < NW; ++k) M = fmaxf(M, mlbuf[(k * 8 + row) * 2]);
         const float Mu = M == -INFINITY ? 0.f : M;
         float L = 0.f;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < WK; ++k) {
-          const int at = (k * WM + tile) * 8 + rw;
+        for (int k = 0; k < NW; ++k) {
+          const int at = k * 8 + row;
           const float f = fast_exp2(mlbuf[at * 2] - Mu);
           L = fmaf(mlbuf[at * 2 + 1], f, L);
           const float4 v = *reinterpret_cast<const float4*>(obuf + at * C::OLD + d);
@@ -745,6 +787,472 @@ __global__ void __launch_bounds__((Kv8Cfg<DP, WM>::NW + 1) * 32, Kv8Cfg<DP, WM>:
         }
       }
     }
+    ok = *static_cast<volatile int*>(&sh_fail) == 0;
+    // the next item
+    w.next_item(p, items);
+  }
+}
+
+template <int CODE, int DP, int NR>
+__global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTAS)
+    kv8_attention_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                              const __grid_constant__ Kv8TcParams p) {
+  using C = Kv8Many<DP, NR>;
+  constexpr int NW = C::NW, CH = C::CH, NT = C::NT, TP = C::TP, NS = C::NS, RT = C::RT, MB = C::MB;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const float* meta = reinterpret_cast<const float*>(smem + C::META_OFF);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* empty = full + NS;
+  uint2* const qf = reinterpret_cast<uint2*>(smem + C::Q_OFF);
+  uint2* const pf = reinterpret_cast<uint2*>(smem + C::P_OFF);
+  uint2* const pf2 = pf + NT * NR * 32;
+  float* const sfac = reinterpret_cast<float*>(smem + C::FAC_OFF);
+  float* const smax = reinterpret_cast<float*>(smem + C::MAX_OFF);
+  volatile int* const flag_up = reinterpret_cast<volatile int*>(smem + C::FLAG_OFF);
+  volatile int* const flag_apart = flag_up + NW;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int items = p.c.Hkv * p.chunks;
+  Kv8Walk<CH> w0;
+  int64_t u1;
+  if (!kv8_begin<C>(p, full, empty, w0, u1)) return;
+  if (warp == NW) {
+    kv8_produce<C>(p, tmK, tmV, smem, full, empty, w0, u1);
+    return;
+  }
+
+  // ---------------- consumers ----------------
+  auto bar = [] { asm volatile("bar.sync 1, %0;" ::"n"(NW * 32) : "memory"); };
+  const int g = lane >> 2, t4 = lane & 3, mi = lane >> 3, rr = lane & 7;
+  const uint32_t sbase = smem_u32(smem);
+  Kv8Walk<CH> w = w0;
+  int it = 0;
+  bool ok = true;
+  while (ok && w.live(p, u1)) {
+    const int j0 = w.j, j_end = static_cast<int>(min(static_cast<int64_t>(w.n), w.j + (u1 - w.at))), s = w.s, ctx = w.ctx;
+    const int kvh = w.r / p.chunks, rc = w.r - kvh * p.chunks;
+
+    // ---- query rows to fp16 B fragments in shared memory, as in the other kernel:
+    // warp w makes those of rows 8 w .. 8 w + 7 ----
+    if (warp < NR) {
+      auto to_float = [&](uint32_t raw) {
+        return p.bf16 ? __uint_as_float(raw << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(raw)));
+      };
+      uint2 raw[DP / 16];
+      const int row = rc * RT + warp * 8 + g;
+      const bool real = row < p.rows;
+      const uint16_t* src = kv8_q_row(p, s, kvh, real ? row : 0);
+      float top = 0.f;
+      bool odd = false;
+#pragma unroll
+      for (int b = 0; b < DP / 16; ++b) {
+        const int d = b * 16 + 4 * t4;
+        uint2 v = make_uint2(0, 0);
+        if (p.q_vec) {
+          if (real && d < p.c.D) v = *reinterpret_cast<const uint2*>(src + d);
+        } else {
+          uint32_t e[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) e[k] = real && d + k < p.c.D ? src[(d + k) * p.sq[3]] : 0;
+          v = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
+        }
+        raw[b] = v;
+      }
+#pragma unroll
+      for (int b = 0; b < DP / 16; ++b) {
+        const uint2 v = raw[b];
+        const float f[4] = {to_float(v.x & 0xffff), to_float(v.x >> 16), to_float(v.y & 0xffff), to_float(v.y >> 16)};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          top = fmaxf(top, fabsf(f[k]));
+          odd |= !(fabsf(f[k]) < INFINITY);
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      odd |= __shfl_xor_sync(0xffffffffu, odd, 1);
+      odd |= __shfl_xor_sync(0xffffffffu, odd, 2);
+      const int e2 = odd || top == 0.f ? 8 : max(-110, static_cast<int>(__float_as_uint(top) >> 23) - 127);
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + 8 - e2) << 23);
+      if (t4 == 0) sfac[warp * 8 + g] = p.scale * __uint_as_float(static_cast<uint32_t>(127 - 8 + e2) << 23);
+#pragma unroll
+      for (int b = 0; b < DP / 16; ++b) {
+        const uint2 v = raw[b];
+        qf[(b * NR + warp) * 32 + lane] = make_uint2(Elem<__half>::pack2(to_float(v.x & 0xffff) * up, to_float(v.x >> 16) * up),
+                                                     Elem<__half>::pack2(to_float(v.y & 0xffff) * up, to_float(v.y >> 16) * up));
+      }
+    }
+    bar();
+    // this thread's rows are 2 t4 and 2 t4 + 1 of each eight
+    float fac[NR][2];
+    int lim[NR][2];  // keys that a row sees
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        fac[n][k] = sfac[n * 8 + 2 * t4 + k];
+        const int row = rc * RT + n * 8 + 2 * t4 + k;
+        lim[n][k] = row < p.rows ? ctx - p.Lq + row / p.G + 1 : ctx;  // rows that pad the tile see every key
+      }
+
+    float o[MB][NR][4];  // (column 2 g, 2 g + 1 of each 16 of the warp's) x (row 2 t4, 2 t4 + 1)
+    float m[NR][2], l[NR][2];  // the maximum is the CTA's, the sum this thread's keys'
+    int above[NR][2];
+    bool many = false;
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) o[mb][n][0] = o[mb][n][1] = o[mb][n][2] = o[mb][n][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        m[n][k] = kNoMax;
+        l[n][k] = 0.f;
+        above[n][k] = 0;
+      }
+    }
+    float* const score_row = p.scores + ((static_cast<int64_t>(s) * items + w.r) * RT + 2 * t4) * p.score_ld;
+    const int open = ctx - p.Lq + 1;  // keys below it are seen by every row
+
+    for (int j = j0; j < j_end; ++j, ++it) {
+      const int st = it % NS;
+      const bool arrived = mbar_wait(&full[st], (it / NS) & 1);
+      const uint32_t kbase = sbase + st * C::STAGE, vbase = kbase + C::PLANE;
+      const float* mt = meta + st * 3 * NT;
+      const int t = warp * TP, tok = j * CH + t * 16, r0 = t * 16;
+      float x[TP][NR][4], lv[TP], ivs[TP], y[NR][2];
+      bool v_bad = false;
+#pragma unroll
+      for (int n = 0; n < NR; ++n) y[n][0] = y[n][1] = -INFINITY;
+      if (arrived && tok < ctx) {
+        if (CODE == kE4M3 && tok + 16 * TP > ctx) {
+          // rows past the end may hold NaN codes: zero their V rows
+          uint8_t* vt = smem + st * C::STAGE + C::PLANE;
+          for (int i = lane; i < 16 * TP * C::CB * (C::ROWB / 16); i += 32) {
+            const int r = i / (C::CB * (C::ROWB / 16)), cc = i % (C::CB * (C::ROWB / 16));
+            if (tok + r >= ctx)
+              *reinterpret_cast<uint4*>(vt + (cc / 8) * CH * C::ROWB + kv8_sw<DP>(r0 + r, cc % 8)) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int u = 0; u < TP; ++u)
+#pragma unroll
+          for (int n = 0; n < NR; ++n) x[u][n][0] = x[u][n][1] = x[u][n][2] = x[u][n][3] = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < DP / 32; ++kb) {
+          const int piece = 2 * kb + (mi >> 1);
+          uint32_t r[TP][4];
+#pragma unroll
+          for (int u = 0; u < TP; ++u)
+            ldsm_x4(kbase + (piece >> 3) * CH * C::ROWB + kv8_sw<DP>(r0 + u * 16 + (mi & 1) * 8 + rr, piece & 7), r[u][0],
+                    r[u][1], r[u][2], r[u][3]);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            uint2 q[NR];
+#pragma unroll
+            for (int n = 0; n < NR; ++n) q[n] = qf[((2 * kb + k) * NR + n) * 32 + lane];
+#pragma unroll
+            for (int u = 0; u < TP; ++u) {
+              uint32_t af[4];
+              codes_to_half<CODE, 0>(r[u][2 * k], af[0], af[2]);
+              codes_to_half<CODE, 0>(r[u][2 * k + 1], af[1], af[3]);
+#pragma unroll
+              for (int n = 0; n < NR; ++n) Mma<__half>::run(x[u][n], af, q[n].x, q[n].y);
+            }
+          }
+        }
+        // ---- scores, base 2 ----
+        const bool masked = tok + 16 * TP > open;
+#pragma unroll
+        for (int u = 0; u < TP; ++u) {
+          const float ks = mt[t + u];
+          lv[u] = mt[NT + t + u];
+          ivs[u] = mt[2 * NT + t + u];
+          v_bad |= lv[u] != lv[u];
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[u][n][e] *= fac[n][e & 1] * ks;
+        }
+        if (v_bad) {
+#pragma unroll
+          for (int u = 0; u < TP; ++u) lv[u] = lv[u] == lv[u] ? lv[u] : kPBias;
+        }
+        if (p.inv_cap > 0.f) {
+#pragma unroll
+          for (int u = 0; u < TP; ++u)
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                x[u][n][e] = p.cap2 * (1.f - __fdividef(2.f, 1.f + fast_exp2(x[u][n][e] * p.inv_cap)));
+        }
+        if (masked) {
+#pragma unroll
+          for (int u = 0; u < TP; ++u)
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (tok + u * 16 + g + (e & 2) * 4 >= lim[n][e & 1]) x[u][n][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int u = 0; u < TP; ++u)
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) y[n][k] = fmaxf(y[n][k], lv[u] + fmaxf(x[u][n][k], x[u][n][k + 2]));
+        if (p.scores) {
+#pragma unroll
+          for (int u = 0; u < TP; ++u) {
+            if (tok + u * 16 >= p.score_ld) continue;
+            float* sp = score_row + tok + u * 16 + g;
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                sp[(n * 8 + k) * p.score_ld] = x[u][n][k];
+                sp[(n * 8 + k) * p.score_ld + 8] = x[u][n][k + 2];
+              }
+          }
+        }
+      }
+      // ---- running maximum, common to the warps: raised when a score of any of
+      // them passes it by 2^kLag ----
+      bool up = false;
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) up |= y[n][k] > m[n][k] + (kLag + kPBias);
+      up = __any_sync(0xffffffffu, up);
+      if (lane == 0) flag_up[warp] = (up ? 1 : 0) | (arrived ? 0 : 2);
+      bar();  // also: every warp has read the last chunk's P
+      int any_up = 0;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) any_up |= flag_up[i];
+      if (any_up & 2) {  // a wait ran out: all leave together, no warp waits for one that left
+        ok = false;
+        break;
+      }
+      if (any_up) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float mx = y[n][k] - kPBias;
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            if (g == 0) smax[warp * RT + n * 8 + 2 * t4 + k] = mx;
+          }
+        bar();
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          float al[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float mn = m[n][k];
+#pragma unroll
+            for (int i = 0; i < NW; ++i) mn = fmaxf(mn, smax[i * RT + n * 8 + 2 * t4 + k]);
+            al[k] = fast_exp2(m[n][k] - mn);
+            m[n][k] = mn;
+            l[n][k] *= al[k];
+            above[n][k] = 0;
+          }
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) {
+            o[mb][n][0] *= al[0];
+            o[mb][n][1] *= al[1];
+            o[mb][n][2] *= al[0];
+            o[mb][n][3] *= al[1];
+          }
+        }
+        many = false;
+      }
+      // ---- this warp's weights, as P^T fragments for everyone ----
+      bool apart = false;
+      if (tok < ctx) {
+#pragma unroll
+        for (int u = 0; u < TP; ++u)
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float c0 = lv[u] - m[n][k];
+              x[u][n][k] = fast_exp2(x[u][n][k] + c0);
+              x[u][n][k + 2] = fast_exp2(x[u][n][k + 2] + c0);
+              l[n][k] = fmaf(x[u][n][k] + x[u][n][k + 2], ivs[u], l[n][k]);
+            }
+        if (!many) {  // weights below fp16's normal range go apart, as in the other kernel
+          float least = 1.f;
+          int fewest = kFew;
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              int c = 0;
+#pragma unroll
+              for (int u = 0; u < TP; ++u)
+#pragma unroll
+                for (int e = k; e < 4; e += 2) {
+                  least = fminf(least, x[u][n][e]);
+                  c += x[u][n][e] >= kHalfMin;
+                }
+              c += __shfl_xor_sync(0xffffffffu, c, 4);
+              c += __shfl_xor_sync(0xffffffffu, c, 8);
+              c += __shfl_xor_sync(0xffffffffu, c, 16);
+              above[n][k] += c;
+              fewest = min(fewest, above[n][k]);
+            }
+          many = __all_sync(0xffffffffu, fewest >= kFew);
+          apart = !many && __any_sync(0xffffffffu, least < kHalfMin);
+          if (apart) {
+#pragma unroll
+            for (int u = 0; u < TP; ++u)
+#pragma unroll
+              for (int n = 0; n < NR; ++n) {
+                float f[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float v = x[u][n][e];
+                  const bool small = v < kHalfMin;
+                  f[e] = small ? v * 16777216.f : 0.f;
+                  x[u][n][e] = small ? 0.f : v;
+                }
+                const uint32_t a = transpose8x8(Elem<__half>::pack2(f[0], f[1])), b = transpose8x8(Elem<__half>::pack2(f[2], f[3]));
+                pf2[((t + u) * NR + n) * 32 + lane] = make_uint2(a, b);
+              }
+          }
+        }
+        if (v_bad) {  // a NaN or infinite V scale: NaN for the rows that see a key of the tile
+#pragma unroll
+          for (int u = 0; u < TP; ++u)
+            if (mt[NT + t + u] != mt[NT + t + u]) {
+#pragma unroll
+              for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[u][n][e] = tok + u * 16 < lim[n][e & 1] ? __uint_as_float(0x7fffffffu) : 0.f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < TP; ++u)
+#pragma unroll
+          for (int n = 0; n < NR; ++n) {
+            const uint32_t a = transpose8x8(Elem<__half>::pack2(x[u][n][0], x[u][n][1]));
+            const uint32_t b = transpose8x8(Elem<__half>::pack2(x[u][n][2], x[u][n][3]));
+            pf[((t + u) * NR + n) * 32 + lane] = make_uint2(a, b);
+          }
+      }
+      if (lane == 0) flag_apart[warp] = apart;
+      bar();
+      // ---- O^T += Vc^T P^T over all the chunk's tiles, this warp's columns ----
+      const int tiles = min(NT, (ctx - j * CH + 16 * TP - 1) / (16 * TP) * TP);  // tiles whose P was written
+      const int col0 = warp * (C::CW / 16);  // first 16-byte piece
+      auto product = [&](int tile, const uint2* frag, float (&acc)[MB][NR][4]) {
+        uint2 pr[NR];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) pr[n] = frag[(tile * NR + n) * 32 + lane];
+        uint32_t r[2 * MB];
+        if (MB == 2) {
+          const int piece = col0 + (mi >> 1);
+          ldsm_x4_t(vbase + (piece >> 3) * CH * C::ROWB + kv8_sw<DP>(tile * 16 + (mi & 1) * 8 + rr, piece & 7), r[0], r[1],
+                    r[2 * MB - 2], r[2 * MB - 1]);
+        } else {
+          ldsm_x2_t(vbase + (col0 >> 3) * CH * C::ROWB + kv8_sw<DP>(tile * 16 + (mi & 1) * 8 + rr, col0 & 7), r[0], r[1]);
+        }
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          uint32_t af[4];
+          codes_to_half<CODE, 1>(r[2 * mb], af[0], af[1]);
+          codes_to_half<CODE, 1>(r[2 * mb + 1], af[2], af[3]);
+#pragma unroll
+          for (int n = 0; n < NR; ++n) Mma<__half>::run(acc[mb][n], af, pr[n].x, pr[n].y);
+        }
+      };
+      int any_apart = 0;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) any_apart |= flag_apart[i] << i;
+      if (any_apart) {
+        float a[MB][NR][4];
+#pragma unroll
+        for (int i = 0; i < MB * NR * 4; ++i) a[i / (NR * 4)][i / 4 % NR][i % 4] = 0.f;
+#pragma unroll 1
+        for (int tile = 0; tile < tiles; ++tile)
+          if ((any_apart >> (tile / TP)) & 1) product(tile, pf2, a);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[mb][n][e] = fmaf(a[mb][n][e], 5.9604644775390625e-8f, o[mb][n][e]);
+      }
+      if (tiles == NT) {
+#pragma unroll
+        for (int tile = 0; tile < NT; ++tile) product(tile, pf, o);
+      } else {
+#pragma unroll 1
+        for (int tile = 0; tile < tiles; ++tile) product(tile, pf, o);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+
+    // ---- the warps' sums, then each warp finishes or stores its columns ----
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float v = l[n][k];
+        v += __shfl_xor_sync(0xffffffffu, v, 4);
+        v += __shfl_xor_sync(0xffffffffu, v, 8);
+        v += __shfl_xor_sync(0xffffffffu, v, 16);
+        l[n][k] = v;
+      }
+    bar();  // the last maxima have been read
+    if (g == 0) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) smax[warp * RT + n * 8 + 2 * t4 + k] = l[n][k];
+    }
+    bar();
+    const bool whole = j0 == 0 && j_end == w.n;
+    const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + (j0 == 0 ? 1 : 0)) * RT;
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int row = n * 8 + 2 * t4 + k, grow = rc * RT + row;
+        if (grow >= p.rows) continue;
+        float L = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) L += smax[i * RT + row];
+        const int d0 = warp * C::CW + 2 * g;
+        if (whole) {
+          const int i = grow / p.G, h = kvh * p.G + grow - i * p.G;
+          const float inv = L != 0.f ? kLBiasInv / L : 0.f;
+          uint16_t* out = static_cast<uint16_t*>(p.out) + s * p.so[0] + i * p.so[1] + h * p.so[2];
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int d = d0 + mb * 16 + c;
+              const float f = o[mb][n][2 * c + k] * inv;
+              if (d < p.c.D) out[d * p.so[3]] = p.bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f)) : __half_as_ushort(__float2half_rn(f));
+            }
+          if (warp == 0 && g == 0) {
+            const float v = L != 0.f ? m[n][k] + kLBias + log2f(L) : -INFINITY;
+            if (p.lse) p.lse[(static_cast<int64_t>(s) * p.Lq + i) * p.H + h] = v * kLn2;
+            if (p.lse2) p.lse2[(static_cast<int64_t>(s) * p.c.Hkv + kvh) * p.rows + grow] = v;
+          }
+        } else {
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb)
+            *reinterpret_cast<float2*>(p.part_o + (slot + row) * DP + d0 + mb * 16) = make_float2(o[mb][n][k], o[mb][n][2 + k]);
+          if (warp == 0 && g == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + row) * 2) = make_float2(m[n][k], L);
+        }
+      }
     // the next item
     w.next_item(p, items);
   }
@@ -884,20 +1392,18 @@ static bool tc_ok(const Kv8View& c, const Kv8AttnArgs& a) {
   return true;
 }
 static int tc_dp(const Kv8View& c) { return c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256; }
-// Warps across the query rows (eight each): as many as the rows of a KV head
-// fill.  Sixteen rows a warp (two MMA columns for each converted tile) measured
-// slower, for want of registers: 16 rows of 64 x <= 8192 keys 153 us against 119.
-static int tc_wm(const Kv8View& c, const Kv8AttnArgs& a) {
+// query rows of a CTA: 8 (Kv8Few), 16 or 32 (Kv8Many), as the rows of a KV head fill
+static int tc_rt(const Kv8View& c, const Kv8AttnArgs& a) {
   const int64_t rows = static_cast<int64_t>(a.H / c.Hkv) * a.Lq;
-  return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 || tc_dp(c) < 256 ? 4 : 8;
+  return rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
 }
 struct TcSizes { int N, RT, DP; int64_t bound, ml, o, lse2, scores, total, score_ld; };
 static int64_t up16(int64_t x) { return (x + 255) / 256 * 256; }
 static TcSizes tc_sizes(const Kv8View& c, const Kv8AttnArgs& a) {
   TcSizes z{};
   z.DP = tc_dp(c);
-  z.N = num_sms() * (z.DP >= 256 ? 1 : 3);  // Kv8Cfg::CTAS
-  z.RT = 8 * tc_wm(c, a);
+  z.RT = tc_rt(c, a);
+  z.N = num_sms() * (z.DP >= 256 ? 1 : z.RT == 8 ? 3 : 2);  // CTAS of the kernel
   const int64_t rows = static_cast<int64_t>(a.H / c.Hkv) * a.Lq, all = rows * c.Hkv * c.num_seqs;
   int64_t at = 0;
   z.bound = at; at += up16(static_cast<int64_t>(z.N) * 16);
@@ -949,9 +1455,8 @@ static int launch_dependent(K kern, dim3 grid, int threads, cudaStream_t st, A..
   return set_error(3, buf);
 }
 
-template <int CODE, int DP, int WM>
-static int launch_tc(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
-  using C = Kv8Cfg<DP, WM>;
+template <class C, int DP, typename K>
+static int launch_tc(K kern, const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
   const TcSizes z = tc_sizes(c, a);
   Kv8TcParams p{};
   p.c = c;
@@ -982,9 +1487,8 @@ static int launch_tc(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
   CUtensorMap mk, mv;
   if (const int r = encode_codes(&mk, c, 0, C::ROWB, p.box_rows)) return r;
   if (const int r = encode_codes(&mv, c, 1, C::ROWB, p.box_rows)) return r;
-  auto kern = kv8_attention_tc_kernel<CODE, DP, WM>;
   if (const int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::SMEM)) return r;
-  kern<<<z.N, (C::NW + 1) * 32, C::SMEM, st>>>(mk, mv, p);
+  kern<<<z.N, C::THREADS, C::SMEM, st>>>(mk, mv, p);
   note_kernel("kv8_attention_tc");
   if (const int r = launch_dependent(kv8_attention_join_kernel<DP>, dim3(z.N - 1, z.RT / 4), 128, st, p, z.RT, z.N)) return r;
   if (a.weights) {
@@ -997,13 +1501,10 @@ static int launch_tc(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
 
 template <int CODE, int DP>
 static int launch_rows(const Kv8View& c, const Kv8AttnArgs& a, cudaStream_t st) {
-  switch (tc_wm(c, a)) {
-    case 1: return launch_tc<CODE, DP, 1>(c, a, st);
-    case 2: return launch_tc<CODE, DP, 2>(c, a, st);
-    case 4: return launch_tc<CODE, DP, 4>(c, a, st);
-    default:
-      if constexpr (DP >= 256) return launch_tc<CODE, DP, 8>(c, a, st);
-      return set_error(2, "kv8 attention: no kernel for these rows");
+  switch (tc_rt(c, a)) {
+    case 8: return launch_tc<Kv8Few<DP>, DP>(kv8_attention_few_kernel<CODE, DP>, c, a, st);
+    case 16: return launch_tc<Kv8Many<DP, 2>, DP>(kv8_attention_many_kernel<CODE, DP, 2>, c, a, st);
+    default: return launch_tc<Kv8Many<DP, 4>, DP>(kv8_attention_many_kernel<CODE, DP, 4>, c, a, st);
   }
 }
 
