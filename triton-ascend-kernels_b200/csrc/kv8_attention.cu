@@ -44,6 +44,7 @@ struct Kv8TcParams {
   float scale;       // softmax scale * log2(e); with a cap: softmax scale
   float cap2, inv_cap;  // softcap * log2(e), 2 log2(e) / softcap; 0: no cap
   // workspace
+  int64_t* places;   // U, the length of the work list
   int4* bound;       // [N] first chunk of each CTA: {sequence, item of it, chunk of the item, chunks of the item}
   float* part_o;     // [N][2][RT][DP]
   float* part_ml;    // [N][2][RT][2]
@@ -88,7 +89,7 @@ template <int DP> struct Kv8Few : Kv8Base<DP> {
   using B = Kv8Base<DP>;
   static constexpr int RT = 8;
   static constexpr int CTAS = DP >= 256 ? 1 : 3;        // per SM
-  static constexpr int DH = 32;                         // columns joined at a time
+  static constexpr int DH = 64;                         // columns joined at a time
   static constexpr int OLD = DH + 8;                    // row stride of the joining buffer (bank spread)
   static constexpr int OBUF_OFF = B::OWN_OFF;           // [NW][8][OLD] floats
   static constexpr int ML_OFF = OBUF_OFF + B::NW * 8 * OLD * 4;  // [NW][8][2]
@@ -216,7 +217,7 @@ __device__ __forceinline__ bool kv8_begin(const Kv8TcParams& p, uint64_t* full, 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], 2);  // the copies' transaction, and the tiles' scales
       mbar_init(&empty[i], NW);
     }
     fence_barrier_init();
@@ -242,8 +243,11 @@ __device__ __forceinline__ bool kv8_begin(const Kv8TcParams& p, uint64_t* full, 
     total += sh_sum[w];
   }
   const int64_t U = total * items;
-  const int64_t u0 = U * blockIdx.x / gridDim.x;
-  u1 = U * (blockIdx.x + 1) / gridDim.x;
+  // (no more shares than places, so that an item's parts lie in consecutive CTAs)
+  const int64_t n_cta = min(static_cast<int64_t>(gridDim.x), max(U, int64_t{1}));
+  const int64_t u0 = min(U, U * blockIdx.x / n_cta);
+  u1 = min(U, U * (blockIdx.x + 1) / n_cta);
+  if (tid == 0 && blockIdx.x == 0) *p.places = U;
   before += incl - mine;  // places (of one item) before this thread's sequences
   if (u0 < U && mine > 0 && before * items <= u0 && u0 < (before + mine) * items) {
     int s = s_lo;
@@ -340,18 +344,8 @@ __device__ __forceinline__ void kv8_produce(const Kv8TcParams& p, const CUtensor
       }
     }
     Meta far = fetch_page(w, more2);
-    fetch_scales(nxt);
     const int st = it % NS;
     if (it >= NS && !__all_sync(0xffffffffu, mbar_wait_sleep(&empty[st], ((it / NS) - 1) & 1))) break;
-    if (lane < NT) {
-      float* mt = meta + st * 3 * NT;
-      const bool bad = !(cur.vs < INFINITY);  // NaN or inf
-      const float v = bad ? 1.f : fmaxf(cur.vs, kMinVs);
-      mt[lane] = cur.ks;
-      mt[NT + lane] = bad ? __uint_as_float(0x7fffffffu) : log2f(v) + kPBias;
-      mt[2 * NT + lane] = kLBiasInv / v;
-    }
-    __syncwarp();
     const int boxes = min(nbox, (cur.ctx - cur.tok0 + p.box_rows - 1) / p.box_rows);
     if (lane == 0) mbar_arrive_expect_tx(&full[st], boxes * 2 * C::CB * p.box_rows * C::ROWB);
     __syncwarp();
@@ -366,6 +360,17 @@ __device__ __forceinline__ void kv8_produce(const Kv8TcParams& p, const CUtensor
         tma_load_4d(k + C::PLANE + cb * CH * C::ROWB, &tmV, &full[st], cb * 128, row, cur.kvh, page);
       }
     }
+    fetch_scales(nxt);
+    if (lane < NT) {
+      float* mt = meta + st * 3 * NT;
+      const bool bad = !(cur.vs < INFINITY);  // NaN or inf
+      const float v = bad ? 1.f : fmaxf(cur.vs, kMinVs);
+      mt[lane] = cur.ks;
+      mt[NT + lane] = bad ? __uint_as_float(0x7fffffffu) : log2f(v) + kPBias;
+      mt[2 * NT + lane] = kLBiasInv / v;
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&full[st]);
     if (!more) break;
     cur = nxt;
     nxt = far;
@@ -1259,101 +1264,75 @@ __global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTA
 }
 
 // Joins the parts of the items that the split cut.  CTA (c, y) looks at the
-// boundary before the main grid's CTA c: if it is the first one inside its item,
-// it merges the item's parts, in order, for four query rows.
+// boundary before the main grid's CTA c: if it is the first one inside its item, it
+// merges the item's parts for four query rows, in order.  The parts are those of
+// CTA c - 1 (slot 1: the item begins in it) and of the CTAs from c to the one that
+// holds the item's last chunk (slot 0).  A thread merges four columns of a row and
+// finds the row's maximum and sum for itself, so there are two round trips to
+// memory: the boundaries, then everything else.
 template <int DP>
-__global__ void __launch_bounds__(128) kv8_attention_join_kernel(const Kv8TcParams p, int RT, int N) {
-  constexpr int MAXP = 512;
-  __shared__ float wt[4][MAXP];
-  __shared__ int ids[MAXP];
-  __shared__ int sh_n;
-  __shared__ float sh_inv[4];
+__global__ void __launch_bounds__(DP) kv8_attention_join_kernel(const __grid_constant__ Kv8TcParams p, int RT, int N) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x + 1, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int4 b = p.bound[c];
-  if (b.z == 0) return;  // an item begins here, or the CTA has no chunk
-  // parts: the CTA in which the item begins (slot 1), then the CTAs up to its
-  // end (slot 0); those in between cover it without a gap
-  if (warp == 0) {
-    int prev = c - 1;
-    while (prev > 0 && p.bound[prev].w == 0) --prev;  // CTAs without a chunk
-    const int4 a = p.bound[prev];
-    const bool first = !(a.x == b.x && a.y == b.y && a.z > 0);
-    int n = 0;
-    if (first) {
-      if (lane == 0) ids[0] = prev * 2 + 1;
-      n = 1;
-      for (int k0 = c; k0 < N; k0 += 32) {
-        const int k = k0 + lane;
-        const int4 e = k < N ? p.bound[k] : make_int4(-1, 0, 1, 1);
-        const bool in = e.w > 0 && e.x == b.x && e.y == b.y && e.z > 0;
-        const bool stop = e.w > 0 && !in;
-        const unsigned mi = __ballot_sync(0xffffffffu, in), ms = __ballot_sync(0xffffffffu, stop);
-        if (in && n + __popc(mi & ((1u << lane) - 1)) < MAXP) ids[n + __popc(mi & ((1u << lane) - 1))] = k * 2;
-        n += __popc(mi);
-        if (ms) break;
+  const int c = blockIdx.x + 1;
+  const int4 a = p.bound[c - 1], b = p.bound[c];
+  const int64_t U = *p.places;
+  if (b.w == 0 || b.z == 0) return;                        // no chunk, or an item begins here
+  if (a.x == b.x && a.y == b.y && a.z > 0) return;         // not the item's first cut
+  const int64_t n_cta = min(static_cast<int64_t>(N), U);
+  const int64_t last = U * c / n_cta + (b.w - b.z) - 1;    // place of the item's last chunk
+  const int n = static_cast<int>(((last + 1) * n_cta - 1) / U) - c + 2;  // parts
+  const int s = b.x, kvh = b.y / p.chunks, rc = b.y - kvh * p.chunks;
+  const int r = blockIdx.y * 4 + threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4;
+  const int grow = rc * RT + r;
+  if (grow >= p.rows) return;
+  auto slot = [&](int k) { return (static_cast<int64_t>(c - 1 + k) * 2 + (k == 0 ? 1 : 0)) * RT + r; };
+  float M = kNoMax, L = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = 0; k0 < n; k0 += 8) {
+    float2 ml[8];
+    float4 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      ml[u] = make_float2(kNoMax, 0.f);
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k0 + u < n) {
+        ml[u] = *reinterpret_cast<const float2*>(p.part_ml + slot(k0 + u) * 2);
+        v[u] = *reinterpret_cast<const float4*>(p.part_o + slot(k0 + u) * DP + d);
       }
     }
-    if (lane == 0) sh_n = min(n, MAXP);
-  }
-  __syncthreads();
-  const int n = sh_n;
-  if (n == 0) return;
-  const int s = b.x, kvh = b.y / p.chunks, rc = b.y - kvh * p.chunks, row0 = blockIdx.y * 4;
-  {
-    const int row = row0 + warp;
-    float M = -INFINITY;
-    for (int k = lane; k < n; k += 32) M = fmaxf(M, p.part_ml[(static_cast<int64_t>(ids[k]) * RT + row) * 2]);
-    M = warp_max(M);
-    const float Mu = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-    for (int k = lane; k < n; k += 32) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (static_cast<int64_t>(ids[k]) * RT + row) * 2);
-      const float f = fast_exp2(ml.x - Mu);
-      wt[warp][k] = f;
-      L = fmaf(ml.y, f, L);
-    }
-    L = warp_sum(L);
-    const int grow = rc * RT + row;
-    if (lane == 0) {
-      sh_inv[warp] = L != 0.f ? kLBiasInv / L : 0.f;
-      if (grow < p.rows) {
-        const float v = L != 0.f ? M + kLBias + log2f(L) : -INFINITY;
-        const int i = grow / p.G, h = kvh * p.G + grow - i * p.G;
-        if (p.lse) p.lse[(static_cast<int64_t>(s) * p.Lq + i) * p.H + h] = v * kLn2;
-        if (p.lse2) p.lse2[(static_cast<int64_t>(s) * p.c.Hkv + kvh) * p.rows + grow] = v;
-      }
+    float Mn = M;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) Mn = fmaxf(Mn, ml[u].x);
+    const float f0 = fast_exp2(M - Mn);
+    M = Mn;
+    L *= f0;
+    o.x *= f0;
+    o.y *= f0;
+    o.z *= f0;
+    o.w *= f0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float f = fast_exp2(ml[u].x - M);
+      L = fmaf(ml[u].y, f, L);
+      o.x = fmaf(v[u].x, f, o.x);
+      o.y = fmaf(v[u].y, f, o.y);
+      o.z = fmaf(v[u].z, f, o.z);
+      o.w = fmaf(v[u].w, f, o.w);
     }
   }
-  __syncthreads();
-  for (int e = tid; e < 4 * (DP / 4); e += 128) {
-    const int r = e / (DP / 4), d = (e - r * (DP / 4)) * 4, grow = rc * RT + row0 + r;
-    if (grow >= p.rows) continue;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = 0; k0 < n; k0 += 8) {
-      float4 v[8];
+  const float inv = L != 0.f ? kLBiasInv / L : 0.f;
+  const int i = grow / p.G, h = kvh * p.G + grow - i * p.G;
+  uint16_t* out = static_cast<uint16_t*>(p.out) + s * p.so[0] + i * p.so[1] + h * p.so[2];
+  const float f[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (k0 + u < n) v[u] = *reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(ids[k0 + u]) * RT + row0 + r) * DP + d);
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (k0 + u < n) {
-          const float f = wt[r][k0 + u];
-          a.x = fmaf(v[u].x, f, a.x);
-          a.y = fmaf(v[u].y, f, a.y);
-          a.z = fmaf(v[u].z, f, a.z);
-          a.w = fmaf(v[u].w, f, a.w);
-        }
-    }
-    const float inv = sh_inv[r];
-    const int i = grow / p.G, h = kvh * p.G + grow - i * p.G;
-    uint16_t* out = static_cast<uint16_t*>(p.out) + s * p.so[0] + i * p.so[1] + h * p.so[2];
-    const float f[4] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv};
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (d + k < p.c.D)
-        out[(d + k) * p.so[3]] = p.bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f[k])) : __half_as_ushort(__float2half_rn(f[k]));
+  for (int k = 0; k < 4; ++k)
+    if (d + k < p.c.D)
+      out[(d + k) * p.so[3]] = p.bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f[k])) : __half_as_ushort(__float2half_rn(f[k]));
+  if (d == 0) {
+    const float v = L != 0.f ? M + kLBias + log2f(L) : -INFINITY;
+    if (p.lse) p.lse[(static_cast<int64_t>(s) * p.Lq + i) * p.H + h] = v * kLn2;
+    if (p.lse2) p.lse2[(static_cast<int64_t>(s) * p.c.Hkv + kvh) * p.rows + grow] = v;
   }
 }
 
@@ -1370,10 +1349,17 @@ __global__ void __launch_bounds__(256) kv8_attention_weights_kernel(const Kv8TcP
   const float* sc = p.scores + item * p.chunks * RT * p.score_ld + pos;  // a head's chunks follow one another: row r at r
   const float* ls = p.lse2 + item * p.rows;
   float sum = 0.f;
-  for (int r = 0; r < p.rows; ++r) {
-    const float L = ls[r];
-    const float e = fast_exp2(sc[r * p.score_ld] - L);
-    sum += L == -INFINITY ? 0.f : e;
+  for (int r0 = 0; r0 < p.rows; r0 += 8) {
+    float x[8], L[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int r = min(r0 + u, p.rows - 1);
+      x[u] = sc[r * p.score_ld];
+      L[u] = ls[r];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (r0 + u < p.rows && L[u] != -INFINITY) sum += fast_exp2(x[u] - L[u]);
   }
   weights[s * w0 + kvh * w1 + pos * w2] += sum;
 }
@@ -1397,7 +1383,7 @@ static int tc_rt(const Kv8View& c, const Kv8AttnArgs& a) {
   const int64_t rows = static_cast<int64_t>(a.H / c.Hkv) * a.Lq;
   return rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
 }
-struct TcSizes { int N, RT, DP; int64_t bound, ml, o, lse2, scores, total, score_ld; };
+struct TcSizes { int N, RT, DP; int64_t places, bound, ml, o, lse2, scores, total, score_ld; };
 static int64_t up16(int64_t x) { return (x + 255) / 256 * 256; }
 static TcSizes tc_sizes(const Kv8View& c, const Kv8AttnArgs& a) {
   TcSizes z{};
@@ -1406,6 +1392,7 @@ static TcSizes tc_sizes(const Kv8View& c, const Kv8AttnArgs& a) {
   z.N = num_sms() * (z.DP >= 256 ? 1 : z.RT == 8 ? 3 : 2);  // CTAS of the kernel
   const int64_t rows = static_cast<int64_t>(a.H / c.Hkv) * a.Lq, all = rows * c.Hkv * c.num_seqs;
   int64_t at = 0;
+  z.places = at; at += up16(8);
   z.bound = at; at += up16(static_cast<int64_t>(z.N) * 16);
   z.ml = at; at += up16(static_cast<int64_t>(z.N) * 2 * z.RT * 8);
   z.o = at; at += up16(static_cast<int64_t>(z.N) * 2 * z.RT * z.DP * 4);
@@ -1476,6 +1463,7 @@ static int launch_tc(K kern, const Kv8View& c, const Kv8AttnArgs& a, cudaStream_
   p.cap2 = a.softcap * kLog2e;
   p.inv_cap = a.softcap > 0.f ? 2.f * kLog2e / a.softcap : 0.f;
   uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(a.workspace) + 255) & ~uintptr_t(255));
+  p.places = reinterpret_cast<int64_t*>(ws + z.places);
   p.bound = reinterpret_cast<int4*>(ws + z.bound);
   p.part_ml = reinterpret_cast<float*>(ws + z.ml);
   p.part_o = reinterpret_cast<float*>(ws + z.o);
@@ -1490,7 +1478,7 @@ static int launch_tc(K kern, const Kv8View& c, const Kv8AttnArgs& a, cudaStream_
   if (const int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::SMEM)) return r;
   kern<<<z.N, C::THREADS, C::SMEM, st>>>(mk, mv, p);
   note_kernel("kv8_attention_tc");
-  if (const int r = launch_dependent(kv8_attention_join_kernel<DP>, dim3(z.N - 1, z.RT / 4), 128, st, p, z.RT, z.N)) return r;
+  if (const int r = launch_dependent(kv8_attention_join_kernel<DP>, dim3(z.N - 1, z.RT / 4), DP, st, p, z.RT, z.N)) return r;
   if (a.weights) {
     const int64_t w = a.weights_width < c.max_rows ? a.weights_width : c.max_rows;
     return launch_dependent(kv8_attention_weights_kernel, dim3(static_cast<unsigned>((w + 255) / 256), c.Hkv, c.num_seqs),
