@@ -1336,32 +1336,41 @@ __global__ void __launch_bounds__(DP) kv8_attention_join_kernel(const __grid_con
   }
 }
 
-// Attention weights from the stored scores: each thread owns keys, so every
+// Attention weights from the stored scores: each thread owns four keys, so every
 // weight is added to once, in the order of the rows.
-__global__ void __launch_bounds__(256) kv8_attention_weights_kernel(const Kv8TcParams p, int RT, float* weights,
+__global__ void __launch_bounds__(128) kv8_attention_weights_kernel(const __grid_constant__ Kv8TcParams p, int RT, float* weights,
                                                                     int64_t w0, int64_t w1, int64_t w2, int64_t width) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int kvh = blockIdx.y, s = blockIdx.z;
-  const int64_t n = min(static_cast<int64_t>(kv8_ctx(p, s)), width);
-  const int64_t pos = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int n = static_cast<int>(min(static_cast<int64_t>(kv8_ctx(p, s)), width));
+  const int pos = (blockIdx.x * 128 + threadIdx.x) * 4;
   if (pos >= n) return;
   const int64_t item = static_cast<int64_t>(s) * p.c.Hkv + kvh;
   const float* sc = p.scores + item * p.chunks * RT * p.score_ld + pos;  // a head's chunks follow one another: row r at r
   const float* ls = p.lse2 + item * p.rows;
-  float sum = 0.f;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
   for (int r0 = 0; r0 < p.rows; r0 += 8) {
-    float x[8], L[8];
+    float4 x[8];
+    float L[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int r = min(r0 + u, p.rows - 1);
-      x[u] = sc[r * p.score_ld];
+      x[u] = *reinterpret_cast<const float4*>(sc + r * p.score_ld);
       L[u] = ls[r];
     }
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (r0 + u < p.rows && L[u] != -INFINITY) sum += fast_exp2(x[u] - L[u]);
+    for (int u = 0; u < 8; ++u) {
+      const float l = r0 + u < p.rows && L[u] != -INFINITY ? L[u] : INFINITY;  // rows without a key weigh nothing
+      sum[0] += fast_exp2(x[u].x - l);
+      sum[1] += fast_exp2(x[u].y - l);
+      sum[2] += fast_exp2(x[u].z - l);
+      sum[3] += fast_exp2(x[u].w - l);
+    }
   }
-  weights[s * w0 + kvh * w1 + pos * w2] += sum;
+  float* w = weights + s * w0 + kvh * w1 + pos * w2;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (pos + k < n) w[k * w2] += sum[k];
 }
 
 // ---------------------------------------------------------------------------
@@ -1481,8 +1490,8 @@ static int launch_tc(K kern, const Kv8View& c, const Kv8AttnArgs& a, cudaStream_
   if (const int r = launch_dependent(kv8_attention_join_kernel<DP>, dim3(z.N - 1, z.RT / 4), DP, st, p, z.RT, z.N)) return r;
   if (a.weights) {
     const int64_t w = a.weights_width < c.max_rows ? a.weights_width : c.max_rows;
-    return launch_dependent(kv8_attention_weights_kernel, dim3(static_cast<unsigned>((w + 255) / 256), c.Hkv, c.num_seqs),
-                            256, st, p, z.RT, a.weights, a.sw[0], a.sw[1], a.sw[2], w);
+    return launch_dependent(kv8_attention_weights_kernel, dim3(static_cast<unsigned>((w + 511) / 512), c.Hkv, c.num_seqs),
+                            128, st, p, z.RT, a.weights, a.sw[0], a.sw[1], a.sw[2], w);
   }
   return 0;
 }
