@@ -42,7 +42,7 @@ struct Kv8TcParams {
   int H, Lq, G, rows, chunks;  // rows = G * Lq query rows per KV head, in `chunks` chunks
   int box_rows;      // rows of one TMA box: the largest power of two dividing block_size, at most CH
   float scale;       // softmax scale * log2(e); with a cap: softmax scale
-  float cap2, inv_cap;  // softcap * log2(e), 2 log2(e) / softcap; 0: no cap
+  float cap2, inv_cap;  // softcap * log2(e), 1 / softcap; 0: no cap
   // workspace
   int64_t* places;   // U, the length of the work list
   int4* bound;       // [N] first chunk of each CTA: {sequence, item of it, chunk of the item, chunks of the item}
@@ -151,6 +151,36 @@ __device__ __forceinline__ void codes_to_half(uint32_t r, uint32_t& lo, uint32_t
         "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
         : "=r"(lo), "=r"(hi) : "r"(x));
   }
+}
+
+// Four scores z to cap * tanh(z / cap), in base-2 units (cap2 = cap * log2(e)).
+// Below |z / cap| = 0.6, where ordinary scores lie, tanh is its odd polynomial
+// (fitted to 7e-8 relative); past it, 1 - 2 / (1 + e^(2 z / cap)), whose absolute
+// error of 1e-7 is small there.  A warp leaves the second out when it needs it for
+// no score.
+__device__ __forceinline__ void kv8_cap(float (&x)[4], float inv_cap, float cap2) {
+  float t[4];
+  bool far = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float h = x[e] * inv_cap, u = h * h;
+    float r = fmaf(-0.006276387721300125f, u, 0.021116213873028755f);
+    r = fmaf(r, u, -0.053875137120485306f);
+    r = fmaf(r, u, 0.13332924246788025f);
+    r = fmaf(r, u, -0.3333333134651184f);
+    t[e] = fmaf(h * u, r, h);
+    far |= fabsf(h) > 0.6f;
+  }
+  if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float h = x[e] * inv_cap;
+      const float big = 1.f - __fdividef(2.f, 1.f + fast_exp2(h * (2.f * kLog2e)));
+      t[e] = fabsf(h) > 0.6f ? big : t[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = t[e] * cap2;
 }
 
 __device__ __forceinline__ int kv8_ctx(const Kv8TcParams& p, int s) {
@@ -562,10 +592,7 @@ __global__ void __launch_bounds__(Kv8Few<DP>::THREADS, Kv8Few<DP>::CTAS)
         }
         if (p.inv_cap > 0.f) {
 #pragma unroll
-          for (int u = 0; u < TP; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)  // cap * tanh(z / cap) = cap * (1 - 2 / (1 + e^(2 z / cap)))
-              x[u][e] = p.cap2 * (1.f - __fdividef(2.f, 1.f + fast_exp2(x[u][e] * p.inv_cap)));
+          for (int u = 0; u < TP; ++u) kv8_cap(x[u], p.inv_cap, p.cap2);
         }
         if (masked) {
 #pragma unroll
@@ -988,10 +1015,7 @@ __global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTA
 #pragma unroll
           for (int u = 0; u < TP; ++u)
 #pragma unroll
-            for (int n = 0; n < NR; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                x[u][n][e] = p.cap2 * (1.f - __fdividef(2.f, 1.f + fast_exp2(x[u][n][e] * p.inv_cap)));
+            for (int n = 0; n < NR; ++n) kv8_cap(x[u][n], p.inv_cap, p.cap2);
         }
         if (masked) {
 #pragma unroll
@@ -1470,7 +1494,7 @@ static int launch_tc(K kern, const Kv8View& c, const Kv8AttnArgs& a, cudaStream_
   if (p.box_rows > C::CH) p.box_rows = C::CH;
   p.scale = a.softcap > 0.f ? a.scale : a.scale * kLog2e;
   p.cap2 = a.softcap * kLog2e;
-  p.inv_cap = a.softcap > 0.f ? 2.f * kLog2e / a.softcap : 0.f;
+  p.inv_cap = a.softcap > 0.f ? 1.f / a.softcap : 0.f;
   uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(a.workspace) + 255) & ~uintptr_t(255));
   p.places = reinterpret_cast<int64_t*>(ws + z.places);
   p.bound = reinterpret_cast<int4*>(ws + z.bound);
