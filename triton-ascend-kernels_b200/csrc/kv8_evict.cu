@@ -11,6 +11,9 @@
 #include <cooperative_groups.h>
 
 #include <cstdio>
+#include <map>
+#include <mutex>
+#include <tuple>
 
 #include "kv8.cuh"
 
@@ -179,6 +182,10 @@ __global__ void __launch_bounds__(kSelThreads, KPT <= 8 ? 2 : 1) kv8_evict_selec
   __shared__ uint32_t sh_digit, sh_left;
   __shared__ uint2 cta_total;                 // kept, tied keys of the CTA
 
+  auto everyone = [&]() {
+    if (cs > 1) cluster.sync(); else __syncthreads();
+  };
+
   float val[KPT];
 #pragma unroll
   for (int k = 0; k < KPT; ++k) {
@@ -201,16 +208,19 @@ __global__ void __launch_bounds__(kSelThreads, KPT <= 8 ? 2 : 1) kv8_evict_selec
       if (i < cand && (d == 0 || (key >> (d == 1 ? 21 : 10)) == (T >> (d == 1 ? 21 : 10))))
         atomicAdd(&hist[d][(key >> shift) & (bins - 1)], 1u);
     }
-    cluster.sync();
+    everyone();
     // bins from the top: thread t has bins - 1 - 2 t and the one below
     uint32_t c0 = 0, c1 = 0;
     const int top = static_cast<int>(bins) - 1 - 2 * tid;
-    if (top > 0)
-      for (int r = 0; r < cs; ++r) {
+    if (top > 0) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {  // at most 8 CTAs: all the reads in flight at once
+        if (r >= cs) break;
         const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(&hist[d][top - 1], r));
         c0 += v.y;
         c1 += v.x;
       }
+    }
     uint32_t x = c0 + c1;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -270,9 +280,11 @@ __global__ void __launch_bounds__(kSelThreads, KPT <= 8 ? 2 : 1) kv8_evict_selec
     if (tid == kSelThreads - 1) cta_total = make_uint2((before + x) & 0xffffu, (before + x) >> 16);
   }
   __syncthreads();
-  cluster.sync();  // totals are there; and every weight of the cluster is in registers
+  everyone();  // totals are there; and every weight of the cluster is in registers
   uint32_t gt0 = 0, eq0 = 0;
-  for (int r = 0; r < rank; ++r) {
+#pragma unroll
+  for (int r = 0; r < 7; ++r) {
+    if (r >= rank) break;
     const uint2 t = *cluster.map_shared_rank(&cta_total, r);
     gt0 += t.x;
     eq0 += t.y;
@@ -292,7 +304,7 @@ __global__ void __launch_bounds__(kSelThreads, KPT <= 8 ? 2 : 1) kv8_evict_selec
     }
   }
   for (int i = m + at; i < n; i += all) w[i * ws] = 0.f;
-  cluster.sync();  // no CTA leaves while another reads its totals
+  everyone();  // no CTA leaves while another reads its totals
 }
 
 // Moves the kept rows of one (sequence, head, K or V).  A cluster moves `cs`
@@ -471,27 +483,33 @@ static int launch_cluster(K kern, dim3 grid, int threads, size_t smem, int cs, b
 }
 
 // Whether clusters of 16 CTAs of this kernel can run (more than eight is not
-// portable: it has to be allowed, and a GPC has to have the room).
+// portable: it has to be allowed, and a GPC has to have the room).  Asked once per
+// device, kernel and shared-memory size.
 static bool cluster16_ok(const void* func, int threads, size_t smem) {
-  if (cudaFuncSetAttribute(func, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-    cudaGetLastError();
-    return false;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(16);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 16;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, size_t>, bool> known;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(mu);
+  const auto key = std::make_tuple(func, dev, smem);
+  const auto it = known.find(key);
+  if (it != known.end()) return it->second;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, func, &cfg) != cudaSuccess) {
-    cudaGetLastError();
-    return false;
+  if (cudaFuncSetAttribute(func, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 16;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, func, &cfg) != cudaSuccess) n = 0;
   }
+  if (n == 0) cudaGetLastError();  // not an error of the caller's
+  known[key] = n > 0;
   return n > 0;
 }
 
