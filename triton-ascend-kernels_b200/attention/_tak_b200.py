@@ -128,14 +128,20 @@ def as_i32(t, device):
 def i32_on(t, index):
     """as_i32 for the device with this index; a tensor that already fits is
     returned as it is, without the cost of a .to() call."""
-    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.is_cuda and t.get_device() == index:
+    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == index:
         return t
     return as_i32(t, torch.device("cuda", index))
 
 
-def raw_stream(index):
-    """cudaStream_t of the current stream of a device, as an int."""
-    return torch._C._cuda_getCurrentRawStream(index)
+# cudaStream_t of the current stream of a device (by index), as an int
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def like(t):
+    """An uninitialised contiguous tensor of t's shape and type (empty_like is the
+    cheaper call, and contiguous where t is)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 _ws = {}

@@ -34,7 +34,9 @@ def describe(k_cache, v_cache, k_scale, v_scale, block_tables):
     """The C ABI's description of a cache (struct tak_kv8_cache, as bytes), the
     int32 block table that it points to, and (device index, num_kv_heads,
     head_dim, num_seqs)."""
-    _t.require_cuda(k_cache, v_cache, k_scale, v_scale)
+    index = k_cache.get_device()
+    assert index >= 0 and v_cache.get_device() == index and k_scale.get_device() == index \
+        and v_scale.get_device() == index, "The cache's tensors must be on a CUDA device, all on the same"
     dtype = k_cache.dtype
     code = _CODES.get(dtype)
     assert code is not None, f"unsupported cache dtype {dtype}: expected int8 or float8_e4m3fn"
@@ -47,9 +49,6 @@ def describe(k_cache, v_cache, k_scale, v_scale, block_tables):
         "k_scale and v_scale must be [num_blocks, num_kv_heads, block_size / group]"
     assert k_scale.dtype is _torch.float32 and v_scale.dtype is _torch.float32, "scales must be float32"
     ng = ss[2]
-    index = k_cache.get_device()
-    assert v_cache.get_device() == index and k_scale.get_device() == index and v_scale.get_device() == index, \
-        "the cache's tensors must be on one device"
     assert ng > 0 and rows % ng == 0, f"the number of scales ({ng}) must divide block_size ({rows})"
     bt = _t.i32_on(block_tables, index)
     assert bt.dim() == 2, "block_tables must be [num_seqs, max_blocks]"
@@ -83,11 +82,10 @@ def kv8_cache_write(k, v, k_cache, v_cache, k_scale, v_scale, block_tables, star
     Appending to a group that holds rows keeps the larger of the two scales;
     rows held under a smaller one are rounded again into it.
     """
-    _t.require_cuda(k, v)
     desc, _bt, (index, hkv, d, seqs) = describe(k_cache, v_cache, k_scale, v_scale, block_tables)
     shape = k.shape
     assert len(shape) == 3 and v.shape == shape and v.dtype is k.dtype, "K and V must have the same shape and dtype"
-    assert k.get_device() == index and v.get_device() == index, "k / v must be on the cache's device"
+    assert k.get_device() == index and v.get_device() == index, "k / v must be on the cache's CUDA device"
     assert shape[1] == hkv and shape[2] == d, "k / v must be [total_tokens, num_kv_heads, head_dim] of the cache"
     start = _lens(start_lens, index, seqs, "start_lens")
     cu = None if cu_seqlens is None else _lens(cu_seqlens, index, seqs + 1, "cu_seqlens")
@@ -109,8 +107,8 @@ def kv8_cache_read(k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens,
     cu = _lens(cu_seqlens, index, seqs + 1, "cu_seqlens")
     start = None if start_lens is None else _lens(start_lens, index, seqs, "start_lens")
     total = int(total_tokens)
-    k = k_scale.new_empty((total, hkv, d), dtype=dtype)
-    v = k_scale.new_empty((total, hkv, d), dtype=dtype)
+    k = _torch.empty_strided((total, hkv, d), (hkv * d, d, 1), dtype=dtype, device=k_cache.device)
+    v = _torch.empty_like(k)
     st = _S3(hkv * d, d, 1)
     rc = _t.lib().tak_kv8_read(desc, cu.data_ptr(), None if start is None else start.data_ptr(), total,
                                k.data_ptr(), st, v.data_ptr(), st, _t.dtype_code(k), _t.raw_stream(index))
@@ -137,14 +135,13 @@ def kv8_cache_evict(k_cache, v_cache, k_scale, v_scale, block_tables, context_le
     int32 rows per sequence.  Pages past new_lens are free; sequences must not
     share pages.
     """
-    _t.require_cuda(weights)
     desc, _bt, (index, hkv, _d, seqs) = describe(k_cache, v_cache, k_scale, v_scale, block_tables)
     cl = _lens(context_lens, index, seqs, "context_lens")
     budget, recent = int(budget), int(recent)
     ws = weights.shape
     assert len(ws) == 3 and ws[0] == seqs and ws[1] == hkv and weights.dtype is _torch.float32, \
         "weights must be float32 [num_seqs, num_kv_heads, max_rows]"
-    assert weights.get_device() == index, "weights must be on the cache's device"
+    assert weights.get_device() == index, "weights must be on the cache's CUDA device"
     assert budget >= 1 and 0 <= recent <= budget, "budget must be >= 1 and recent in [0, budget]"
     kept = cl.new_empty((seqs, hkv, budget))
     lens = cl.new_empty((seqs,))

@@ -35,12 +35,11 @@ def paged_attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_tables, con
 
     A row that sees no key gives zeros (lse -inf).
     """
-    _t.require_cuda(q, weights)
     desc, _bt, (index, hkv, d, seqs) = describe(k_cache, v_cache, k_scale, v_scale, block_tables)
     shape = q.shape
     assert len(shape) in (3, 4), "q must be [num_seqs, num_q_heads, head_dim] or [num_seqs, num_queries, ...]"
     assert q.get_device() == index and (weights is None or weights.get_device() == index), \
-        "q and weights must be on the cache's device"
+        "q and weights must be on the cache's CUDA device"
     B, H, D = shape[0], shape[-2], shape[-1]
     Lq = shape[1] if len(shape) == 4 else 1
     assert B == seqs, "block_tables must have a row per sequence"
@@ -59,8 +58,9 @@ def paged_attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_tables, con
             "weights must be float32 [num_seqs, num_kv_heads, max_rows]"
         width = ws[2]
         wp, wst = weights.data_ptr(), _S3(*weights.stride())
-    out = q.new_empty(shape)
-    lse = q.new_empty(shape[:-1], dtype=_t.torch.float32) if return_lse else None
+    out = _t.like(q)
+    lse = _t.torch.empty_strided(shape[:-1], (H, 1) if len(shape) == 3 else (Lq * H, H, 1), dtype=_t.torch.float32,
+                                 device=q.device) if return_lse else None
     L = _t.lib()
     stream = _t.raw_stream(index)
     code = _t.dtype_code(q)

@@ -33,15 +33,13 @@ def rotary_nd(q, k, positions, inv_freq, sections, *, interleaved=False, inverse
     Returns ``(q_out, k_out)`` (k_out None without k).  Elements of a head past
     rot_dim are copied.
     """
-    _t.require_cuda(q, k, positions, inv_freq)
-    assert q.dim() == 3, "q must be [total_tokens, num_heads, head_dim]"
-    T, H, D = q.shape
+    index = q.get_device()
+    assert index >= 0 and positions.get_device() == index and inv_freq.get_device() == index, \
+        "Tensors must be on a CUDA device, all on the same"
+    shape = q.shape
+    assert len(shape) == 3, "q must be [total_tokens, num_heads, head_dim]"
+    T, H, D = shape
     dtype = q.dtype
-    Hk = 0
-    if k is not None:
-        assert k.dim() == 3, "k must be [total_tokens, num_heads, head_dim]"
-        Tk, Hk, Dk = k.shape
-        assert Tk == T and Dk == D and k.dtype is dtype, "k must have q's number of tokens, head_dim and dtype"
     pos = positions if positions.dim() == 2 else positions[:, None]
     axes, pairs = len(sections), sum(sections)
     assert pos.shape == (T, axes), "positions must be [total_tokens, len(sections)]"
@@ -50,21 +48,29 @@ def rotary_nd(q, k, positions, inv_freq, sections, *, interleaved=False, inverse
     assert 2 * pairs <= D, f"rot_dim ({2 * pairs}) exceeds head_dim ({D})"
     if pos.dtype is not _torch.int32:
         pos = pos.to(_torch.int32)
-    inv_freq = inv_freq.contiguous()
-    if out is None:
-        qo = q.new_empty((T, H, D))
-        ko = None if k is None else k.new_empty((T, Hk, D))
-    else:
-        qo, ko = out
+    if not inv_freq.is_contiguous():
+        inv_freq = inv_freq.contiguous()
+    qo, ko = (_t.like(q), None) if out is None else out
+    Hk, kp, ks, kop, kos = 0, None, None, None, None
+    if k is not None:
+        kshape = k.shape
+        assert len(kshape) == 3 and kshape[0] == T and kshape[2] == D and k.dtype is dtype, \
+            "k must have q's number of tokens, head_dim and dtype"
+        assert k.get_device() == index, "k must be on q's device (CUDA)"
+        Hk = kshape[1]
+        if out is None:
+            ko = _t.like(k)
+        kp, ks, kop, kos = k.data_ptr(), _S3(*k.stride()), ko.data_ptr(), _S3(*ko.stride())
+    if out is not None:
         for x, y in ((q, qo), (k, ko)):
             if x is not None:
-                assert y is not None and y.is_cuda and y.shape == x.shape and y.dtype is dtype, \
+                assert y is not None and y.get_device() == index and y.shape == x.shape and y.dtype is dtype, \
                     "out must match q and k"
-    kp, ks, kop, kos = (None,) * 4 if k is None else (k.data_ptr(), _S3(*k.stride()), ko.data_ptr(), _S3(*ko.stride()))
     rc = _t.lib().tak_rotary_nd(
         q.data_ptr(), _S3(*q.stride()), kp, ks, pos.data_ptr(), _S2(*pos.stride()), inv_freq.data_ptr(),
-        (_SECTIONS[axes] if axes < 9 else struct.Struct(f"={axes}i").pack)(*sections), axes, qo.data_ptr(), _S3(*qo.stride()), kop, kos, T, H, Hk, D, 2 * pairs,
-        1 if interleaved else 0, 1 if inverse else 0, _t.dtype_code(q), _t.raw_stream(q.get_device()))
+        (_SECTIONS[axes] if axes < 9 else struct.Struct(f"={axes}i").pack)(*sections), axes, qo.data_ptr(),
+        _S3(*qo.stride()), kop, kos, T, H, Hk, D, 2 * pairs, 1 if interleaved else 0, 1 if inverse else 0,
+        _t.dtype_code(q), _t.raw_stream(index))
     if rc:
         _t.check(rc)
     return qo, ko
