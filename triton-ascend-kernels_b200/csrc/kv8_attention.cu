@@ -196,8 +196,9 @@ __device__ __forceinline__ const uint16_t* kv8_q_row(const Kv8TcParams& p, int s
 
 // Positions in the work list: an item of n chunks takes n + kItemCost places, the
 // last kItemCost of them empty.  They stand for what an item costs besides its
-// chunks (query rows, joining the warps, the output), so that CTAs with many
-// short items get fewer chunks.
+// chunks (query rows, joining the warps, the output), so that CTAs with many short
+// items get fewer chunks.  (64 x <= 8192 keys, 4 rows a head: 98 to 101 us from 1 to
+// 4; 32 rows: 244 us without, 221, 202, 190, 190 us from 1 to 4.)
 constexpr int kItemCost = 3;
 template <int CH> __device__ __forceinline__ int64_t kv8_places(int ctx) {
   return ctx > 0 ? (ctx + CH - 1) / CH + kItemCost : 0;
@@ -915,21 +916,15 @@ __global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTA
       }
     }
     bar();
-    // this thread's rows are 2 t4 and 2 t4 + 1 of each eight
-    float fac[NR][2];
-    int lim[NR][2];  // keys that a row sees
-#pragma unroll
-    for (int n = 0; n < NR; ++n)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        fac[n][k] = sfac[n * 8 + 2 * t4 + k];
-        const int row = rc * RT + n * 8 + 2 * t4 + k;
-        lim[n][k] = row < p.rows ? ctx - p.Lq + row / p.G + 1 : ctx;  // rows that pad the tile see every key
-      }
-
+    // this thread's rows are 2 t4 and 2 t4 + 1 of each eight.  (What is needed once a
+    // chunk or less is looked up or worked out again: held, it would spill.)
+    auto limit = [&](int n, int k) {  // keys that a row sees; rows that pad the tile see every key
+      const int row = rc * RT + n * 8 + 2 * t4 + k;
+      return row < p.rows ? ctx - p.Lq + row / p.G + 1 : ctx;
+    };
     float o[MB][NR][4];  // (column 2 g, 2 g + 1 of each 16 of the warp's) x (row 2 t4, 2 t4 + 1)
     float m[NR][2], l[NR][2];  // the maximum is the CTA's, the sum this thread's keys'
-    int above[NR][2];
+    uint32_t above[NR] = {};  // two counts of keys in fp16's normal range since the maximum last rose, 16 bits each
     bool many = false;
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
@@ -939,7 +934,6 @@ __global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTA
       for (int k = 0; k < 2; ++k) {
         m[n][k] = kNoMax;
         l[n][k] = 0.f;
-        above[n][k] = 0;
       }
     }
     float* const score_row = p.scores + ((static_cast<int64_t>(s) * items + w.r) * RT + 2 * t4) * p.score_ld;
@@ -1003,9 +997,14 @@ __global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTA
           ivs[u] = mt[2 * NT + t + u];
           v_bad |= lv[u] != lv[u];
 #pragma unroll
-          for (int n = 0; n < NR; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[u][n][e] *= fac[n][e & 1] * ks;
+          for (int n = 0; n < NR; ++n) {
+            const float2 f = *reinterpret_cast<const float2*>(sfac + n * 8 + 2 * t4);
+            const float f0 = f.x * ks, f1 = f.y * ks;
+            x[u][n][0] *= f0;
+            x[u][n][1] *= f1;
+            x[u][n][2] *= f0;
+            x[u][n][3] *= f1;
+          }
         }
         if (v_bad) {
 #pragma unroll
@@ -1019,12 +1018,16 @@ __global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTA
         }
         if (masked) {
 #pragma unroll
-          for (int u = 0; u < TP; ++u)
+          for (int n = 0; n < NR; ++n)
 #pragma unroll
-            for (int n = 0; n < NR; ++n)
+            for (int k = 0; k < 2; ++k) {
+              const int lim = limit(n, k);
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (tok + u * 16 + g + (e & 2) * 4 >= lim[n][e & 1]) x[u][n][e] = -INFINITY;
+              for (int u = 0; u < TP; ++u) {
+                if (tok + u * 16 + g >= lim) x[u][n][k] = -INFINITY;
+                if (tok + u * 16 + g + 8 >= lim) x[u][n][k + 2] = -INFINITY;
+              }
+            }
         }
 #pragma unroll
         for (int u = 0; u < TP; ++u)
@@ -1087,8 +1090,8 @@ __global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTA
             al[k] = fast_exp2(m[n][k] - mn);
             m[n][k] = mn;
             l[n][k] *= al[k];
-            above[n][k] = 0;
           }
+          above[n] = 0;
 #pragma unroll
           for (int mb = 0; mb < MB; ++mb) {
             o[mb][n][0] *= al[0];
@@ -1131,8 +1134,8 @@ __global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTA
               c += __shfl_xor_sync(0xffffffffu, c, 4);
               c += __shfl_xor_sync(0xffffffffu, c, 8);
               c += __shfl_xor_sync(0xffffffffu, c, 16);
-              above[n][k] += c;
-              fewest = min(fewest, above[n][k]);
+              if ((above[n] >> (16 * k) & 0xffffu) < kFew) above[n] += static_cast<uint32_t>(c) << (16 * k);
+              fewest = min(fewest, static_cast<int>(above[n] >> (16 * k) & 0xffffu));
             }
           many = __all_sync(0xffffffffu, fewest >= kFew);
           apart = !many && __any_sync(0xffffffffu, least < kHalfMin);
@@ -1161,7 +1164,7 @@ __global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTA
 #pragma unroll
               for (int n = 0; n < NR; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[u][n][e] = tok + u * 16 < lim[n][e & 1] ? __uint_as_float(0x7fffffffu) : 0.f;
+                for (int e = 0; e < 4; ++e) x[u][n][e] = tok + u * 16 < limit(n, e & 1) ? __uint_as_float(0x7fffffffu) : 0.f;
             }
         }
 #pragma unroll
