@@ -54,13 +54,14 @@ int tak_read_device_error(void* stream);
  * Process-wide; returns the previous value. */
 int tak_set_kernel_path(int path);
 
-/* Name of the main kernel that the calling thread's last attention or
- * pooling call launched: "prefill_tc", "prefill_generic", "sparse_tc",
+/* Name of the main kernel that the calling thread's last attention, pooling,
+ * rotary or cache call launched: "prefill_tc", "prefill_generic", "sparse_tc",
  * "sparse_generic", "paged_decode_tc", "paged_decode_generic",
  * "compress_bulk", "compress_dual", "compress_csa_hca", "compress_stream",
- * "compress_split" or "compress_rows"; "" when the call launched nothing (an
- * empty problem, an error).  Lets a caller see whether a shape took the
- * tensor-core kernels or fell back to the CUDA-core ones. */
+ * "compress_split", "compress_rows", "rotary_nd", "kv8_write", "kv8_read",
+ * "kv8_attention_tc", "kv8_attention_generic" or "kv8_evict"; "" when the call
+ * launched nothing (an empty problem, an error).  Lets a caller see whether a
+ * shape took the tensor-core kernels or fell back to the CUDA-core ones. */
 const char* tak_last_kernel(void);
 
 /*

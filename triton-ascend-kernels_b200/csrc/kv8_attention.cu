@@ -355,6 +355,7 @@ __device__ __forceinline__ void kv8_produce(const Kv8TcParams& p, const CUtensor
   };
   Kv8Walk<CH> w = w0;
   bool more = true, more2;  // chunks one and two ahead
+  int issued = 0;           // chunks whose copies were started
   Meta cur = fetch_page(w, true);
   w.next(p, items);
   more = w.live(p, u1);
@@ -402,13 +403,25 @@ __device__ __forceinline__ void kv8_produce(const Kv8TcParams& p, const CUtensor
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&full[st]);
+    issued = it + 1;
     if (!more) break;
     cur = nxt;
     nxt = far;
     more = more2;
   }
+  // the CTA's shared memory outlives the copies into it, also where a wait ran out
+  for (int it = max(0, issued - NS); it < issued; ++it) mbar_wait_sleep(&full[it % NS], (it / NS) & 1);
 }
 
+// Up to eight query rows a KV head (a decode step with up to eight query heads for
+// each).  Bound by memory: 64 x <= 8192 keys of 8 heads x 128 (e4m3) in 100 us with
+// the join, 5.45 TB/s, 83 % of the measured copy rate; 3 x <= 131071 keys (int8, 8
+// rows, capped scores) in 102, 80 %.  What is missing is the first data's way (4 us)
+// and the end, where the CTAs finish within 10 % of each other.  Steps on the way,
+// both cases: rows on the MMA's M side, 4 or 8 of its 16 real, 139 and 148 us; with
+// three CTAs an SM, Q in shared memory, 120 and 133; keys on the M side 99 and 100
+// without the join.  One request of 777 keys takes 9.8 us: two launches and the chain
+// of context, page, codes, join.
 template <int CODE, int DP>
 __global__ void __launch_bounds__(Kv8Few<DP>::THREADS, Kv8Few<DP>::CTAS)
     kv8_attention_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -826,6 +839,12 @@ __global__ void __launch_bounds__(Kv8Few<DP>::THREADS, Kv8Few<DP>::CTAS)
   }
 }
 
+// 16 and 32 query rows.  Bound by the issue slots and latencies of the conversions and
+// MMAs (two consumer warps a scheduler): 64 x <= 8192 keys of 8 heads, 32 rows, in 190
+// us, 16 rows in 127; 24 x <= 6000 keys of 4 heads, 32 rows (int8), in 47, 61 with the
+// weights.  Where each warp held eight rows and walked all keys, every code was
+// converted once for each warp (57 and 69 us).  Chunks of 64 keys with three CTAs an SM
+// took 251 us for the first, 61 without weights for the last.
 template <int CODE, int DP, int NR>
 __global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTAS)
     kv8_attention_many_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -1364,7 +1383,9 @@ __global__ void __launch_bounds__(DP) kv8_attention_join_kernel(const __grid_con
 }
 
 // Attention weights from the stored scores: each thread owns four keys, so every
-// weight is added to once, in the order of the rows.
+// weight is added to once, in the order of the rows.  Stored and read back, a key's
+// scores cost 8 bytes a row; recomputing them would read K and multiply again.  24 x
+// <= 6000 keys, 4 heads of 32 rows: 12 us (one key a thread, 18).
 __global__ void __launch_bounds__(128) kv8_attention_weights_kernel(const __grid_constant__ Kv8TcParams p, int RT, float* weights,
                                                                     int64_t w0, int64_t w1, int64_t w2, int64_t width) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1406,6 +1427,7 @@ __global__ void __launch_bounds__(128) kv8_attention_weights_kernel(const __grid
 static bool tc_ok(const Kv8View& c, const Kv8AttnArgs& a) {
   if (a.force_generic || a.dtype == kF32 || c.D > 256 || c.P % 16 || c.group % 16) return false;
   if (c.num_blocks == 0 || c.max_blocks == 0) return false;
+  if (static_cast<int64_t>(a.Lq) * a.H * c.D >= (int64_t{1} << 31)) return false;  // a sequence's query rows are counted in 32 bits
   for (const Kv8Plane& pl : c.plane) {
     if (pl.sc[3] != 1 || (reinterpret_cast<uintptr_t>(pl.code) & 15)) return false;
     for (int i = 0; i < 3; ++i)

