@@ -156,3 +156,28 @@ def test_rotary_sizes(dtype, il, tokens, heads, kv, dim, rot, axes):
     check_rot(qo, q, pos, inv, sec, il, False)
     if kv:
         check_rot(ko, k, pos, inv, sec, il, False)
+
+
+def test_graph_keeps_its_scratch():
+    """A captured call replays right after calls on its stream that needed more
+    scratch, and after the memory that they gave back was overwritten."""
+    c = KC.make("graph", 4, 2, 64, 16, 128, "int8", 900)
+    d = KC.to_device(c)
+    q = torch.randn(4, 8, 128, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16).to("cuda")
+    ctx = torch.tensor([900, 1, 450, 899], dtype=torch.int32, device="cuda")
+    many = torch.randn(4, 600, 8, 128, device="cuda").to(torch.bfloat16)
+    weights = torch.zeros(4, 2, 960, device="cuda")
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        want = paged_attention_kv8(q, *d, ctx)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            got = paged_attention_kv8(q, *d, ctx)
+        paged_attention_kv8(many, *d, ctx, weights=weights)
+        keep = [torch.full((1 << 20,), 255, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        got.zero_()
+        g.replay()
+    st.synchronize()
+    assert torch.equal(want, got)
+    assert all(bool((x == 255).all()) for x in keep)

@@ -141,3 +141,11 @@ def test_c_entry_points_refuse():
     refused(rotary(q=None), "null q")
     refused(rotary(T_=-1), "total_tokens")
     refused(rotary((ctypes.c_int32 * 2)(-1, 33)), "negative")
+
+
+def test_another_current_device_is_refused(monkeypatch):
+    monkeypatch.setattr(T, "_current_device", lambda: 1)
+    monkeypatch.setattr(T, "_raw_stream", lambda index: 40 + index)
+    assert T.raw_stream(1) == 41
+    with pytest.raises(AssertionError, match="current device"):
+        T.raw_stream(0)

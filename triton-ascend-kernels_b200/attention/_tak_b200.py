@@ -133,9 +133,24 @@ def i32_on(t, index):
     return as_i32(t, torch.device("cuda", index))
 
 
-# cudaStream_t of the current stream of a device (by index), as an int
-raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
+
+
+def raw_stream(index):
+    """cudaStream_t of the current stream of a device (by index), as an int.  The
+    launches below go to the current device, so it must be that one."""
+    current = _current_device()
+    assert current == index, \
+        f"Tensors are on cuda:{index}, the current device is cuda:{current}: enter torch.cuda.device({index}) first"
+    return _raw_stream(index)
+
+
+def capturing():
+    """Whether the current stream is being captured into a CUDA graph."""
+    return _capturing()
 
 
 def like(t):

@@ -64,7 +64,13 @@ def paged_attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_tables, con
     L = _t.lib()
     stream = _t.raw_stream(index)
     code = _t.dtype_code(q)
-    scratch = _t.workspace_of(index, stream)
+    if _t.capturing():
+        # a graph's scratch is its own: the stream's may be replaced before a replay, or be
+        # in use beside it
+        scratch = _t.torch.empty(L.tak_kv8_attention_workspace_size(desc, H, Lq, width, code),
+                                 dtype=_t.torch.uint8, device=q.device)
+    else:
+        scratch = _t.workspace_of(index, stream)
     while True:
         rc = L.tak_kv8_attention(
             desc, q.data_ptr(), _S4(*st), cl.data_ptr(), out.data_ptr(), _S4(Lq * H * D, H * D, D, 1),

@@ -24,20 +24,35 @@ struct Kv8Plane {
   int64_t ss[3];
 };
 
+// Division of x < 2^31 by an invariant divisor (Granlund and Montgomery, 1994): with
+// 2^l the least power of two that is at least d and mul = floor(2^(31 + l) / d) + 1,
+// the quotient is x * mul >> (31 + l).  mul 0 stands for d = 1.
+struct Kv8Div {
+  uint32_t mul, shift;
+  __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return mul ? __umulhi(x, mul) >> shift : x; }
+};
+inline Kv8Div kv8_div_by(uint32_t d) {
+  if (d <= 1) return {0, 0};
+  uint32_t l = 1;
+  while ((uint64_t{1} << l) < d) ++l;
+  return {static_cast<uint32_t>((uint64_t{1} << (31 + l)) / d + 1), l - 1};
+}
+
 struct Kv8View {
   Kv8Plane plane[2];  // K, V
   const int32_t* block_tables;
   int64_t sbt[2];
   int Hkv, P, D, group, num_seqs, max_blocks;
   int64_t num_blocks;
-  int64_t max_rows;  // max_blocks * P
+  int64_t max_rows;  // max_blocks * P, below 2^31
+  Kv8Div by_P, by_group;
 };
 
 // Page holding row r of sequence s, or -1 when the row lies past the
 // sequence's block-table row or the table names a page outside the cache.
 __device__ __forceinline__ int64_t kv8_page(const Kv8View& c, int s, int64_t r) {
-  if (r < 0 || r >= c.max_rows) return -1;  // max_rows < 2^31: a 32-bit division
-  const int64_t page = c.block_tables[s * c.sbt[0] + static_cast<int64_t>(static_cast<uint32_t>(r) / static_cast<uint32_t>(c.P)) * c.sbt[1]];
+  if (r < 0 || r >= c.max_rows) return -1;
+  const int64_t page = c.block_tables[s * c.sbt[0] + static_cast<int64_t>(c.by_P(static_cast<uint32_t>(r))) * c.sbt[1]];
   return (page >= 0 && page < c.num_blocks) ? page : -1;
 }
 __device__ __forceinline__ uint8_t* kv8_row(const Kv8Plane& p, int64_t page, int h, int row) {
@@ -94,11 +109,24 @@ __device__ __forceinline__ float kv8_scale_max(float a, float b) {
 // 2^23, less 2^23 + 128.  fp32 -> int8: adding 1.5 * 2^23 rounds to nearest even
 // and leaves the two's complement in the low byte; a group's own scale keeps |f|
 // within 127 (1 + 2^-22), so nothing has to be clamped.
+// (Two fp32 operations at a time where both halves take the same one.)
+__device__ __forceinline__ void add2(float& a, float& b, float c) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(c));
+}
+__device__ __forceinline__ void mul2(float& a, float& b, float c) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(c));
+}
 template <int CODE> __device__ __forceinline__ void kv8_dec4(uint32_t q, float* f) {
   if (CODE == kI8) {
     const uint32_t x = q ^ 0x80808080u;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) f[k] = __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7540 + k)) - 8388736.f;
+    for (int k = 0; k < 4; ++k) f[k] = __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7540 + k));
+    add2(f[0], f[1], -8388736.f);
+    add2(f[2], f[3], -8388736.f);
   } else {
     const float2 a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q & 0xffffu), __NV_E4M3)));
     const float2 b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q >> 16), __NV_E4M3)));
@@ -110,9 +138,10 @@ template <int CODE> __device__ __forceinline__ void kv8_dec4(uint32_t q, float* 
 }
 template <int CODE> __device__ __forceinline__ uint32_t kv8_enc4(const float* f) {
   if (CODE == kI8) {
-    uint32_t u[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) u[k] = __float_as_uint(__fadd_rn(f[k], 12582912.f));
+    float g[4] = {f[0], f[1], f[2], f[3]};
+    add2(g[0], g[1], 12582912.f);
+    add2(g[2], g[3], 12582912.f);
+    const uint32_t u[4] = {__float_as_uint(g[0]), __float_as_uint(g[1]), __float_as_uint(g[2]), __float_as_uint(g[3])};
     return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
   }
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3);
@@ -122,8 +151,13 @@ template <int CODE> __device__ __forceinline__ uint32_t kv8_enc4(const float* f)
 template <int CODE> __device__ __forceinline__ uint32_t kv8_rescale4(uint32_t q, float ratio) {
   float f[4];
   kv8_dec4<CODE>(q, f);
+  if (CODE == kI8) {  // one by one: a packed product before the packed sum is fused with it, and rounds once
 #pragma unroll
-  for (int k = 0; k < 4; ++k) f[k] = __fmul_rn(f[k], ratio);
+    for (int k = 0; k < 4; ++k) f[k] = __fmul_rn(f[k], ratio);
+  } else {
+    mul2(f[0], f[1], ratio);
+    mul2(f[2], f[3], ratio);
+  }
   return kv8_enc4<CODE>(f);
 }
 

@@ -53,13 +53,13 @@ __device__ __forceinline__ bool kv8_write_item(const Kv8WriteParams& p, int64_t 
   const int64_t n = p.cu ? p.cu[lo + 1] - tok0 : 1;
   const int64_t start = p.start_lens[lo];
   if (n <= 0 || start < 0) return false;
-  const int64_t first = (static_cast<uint32_t>(start) / static_cast<uint32_t>(c.group) + (item - kv8_item_base(p, lo))) * c.group;  // the group's first position
+  const int64_t first = (static_cast<int64_t>(c.by_group(static_cast<uint32_t>(start))) + (item - kv8_item_base(p, lo))) * c.group;  // the group's first position
   if (first >= start + n) return false;
   w.s = lo;
   w.page = kv8_page(c, lo, first);
   if (w.page < 0) return false;
   const int64_t r0 = max(start, first), r1 = min(start + n, first + c.group);
-  w.in_page = static_cast<int>(static_cast<uint32_t>(first) % static_cast<uint32_t>(c.P));  // page >= 0: first < 2^31
+  w.in_page = static_cast<int>(first - static_cast<int64_t>(c.by_P(static_cast<uint32_t>(first))) * c.P);  // page >= 0: first < 2^31
   w.token = tok0 + (r0 - start);
   w.held = static_cast<int>(r0 - first);
   w.fresh = static_cast<int>(r1 - r0);
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(256, 4) kv8_read_kernel(const __grid_constant_
     if (t >= lo && t < p.cu[s + 1]) {
       const int64_t pos = t - lo + (p.start_lens ? p.start_lens[s] : 0);
       my_page = static_cast<int>(kv8_page(c, s, pos));  // num_blocks < 2^31
-      if (my_page >= 0) my_row = static_cast<uint32_t>(pos) % static_cast<uint32_t>(c.P);
+      if (my_page >= 0) my_row = static_cast<int>(pos - static_cast<int64_t>(c.by_P(static_cast<uint32_t>(pos))) * c.P);
     }
   }
   const int pr = c.D / VEC, per_tok = c.Hkv * pr;
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(256, 4) kv8_read_kernel(const __grid_constant_
         next_sc[w] = 0.f;
         if (page >= 0 && live) {
           next[w].load(code[w] + page * c.plane[w].sc[0] + row * c.plane[w].sc[2]);
-          next_sc[w] = scale[w][page * c.plane[w].ss[0] + static_cast<uint32_t>(row) / static_cast<uint32_t>(c.group) * c.plane[w].ss[2]];
+          next_sc[w] = scale[w][page * c.plane[w].ss[0] + static_cast<int64_t>(c.by_group(row)) * c.plane[w].ss[2]];
         }
       }
     };

@@ -37,6 +37,8 @@ static int make_view(Kv8View* out, const tak_kv8_cache* c) {
   v.max_blocks = static_cast<int>(c->max_blocks);
   v.num_blocks = c->num_blocks;
   v.max_rows = c->max_blocks * c->block_size;
+  v.by_P = kv8_div_by(static_cast<uint32_t>(v.P));
+  v.by_group = kv8_div_by(static_cast<uint32_t>(v.group));
   if (v.num_blocks > 0) TAK_REQUIRE(c->k_cache && c->v_cache && c->k_scale && c->v_scale, "kv8: null cache pointer");
   if (v.num_seqs > 0 && v.max_blocks > 0) TAK_REQUIRE(c->block_tables, "kv8: null block table");
   v.plane[0].code = static_cast<uint8_t*>(c->k_cache);

@@ -333,9 +333,9 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
   const Kv8Plane pl = blockIdx.z ? c.plane[1] : c.plane[0];
   const int win = p.window;
   const uint8_t** src = reinterpret_cast<const uint8_t**>(stage + (2 * static_cast<size_t>(win) * D + 15) / 16 * 16);  // [2][win]
-  uint8_t** dst = const_cast<uint8_t**>(src + 2 * win);                                              // [win]
+  struct alignas(16) Dst { uint8_t* row; float ratio; };
+  Dst* dst = reinterpret_cast<Dst*>(const_cast<uint8_t**>(src + 2 * win));                           // [win]
   float* was = reinterpret_cast<float*>(dst + win);                                                  // [win] scales
-  float* ratio = was + win;                                                                          // [win]
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the selection
   const int n = kv8_evict_rows(p, s);
   if (n <= p.budget) return;
@@ -352,14 +352,22 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
     const int j = first + w * step + tid;
     return tid < win && w < steps && j < m ? kept[j] : -1;
   };
-  auto place = [&](int64_t page, int i, const float*& sc) {  // row and scale addresses
-    if (page < 0) {
-      sc = nullptr;
-      return static_cast<uint8_t*>(nullptr);
-    }
-    const int row = static_cast<uint32_t>(i) % static_cast<uint32_t>(c.P);
-    sc = kv8_scale(pl, page, h, static_cast<uint32_t>(row) / static_cast<uint32_t>(c.group));
-    return kv8_row(pl, page, h, row);
+  // page (-1: none) and row in it of a position
+  const int32_t* const table = c.block_tables + s * c.sbt[0];
+  const int num_blocks = static_cast<int>(c.num_blocks), max_rows = static_cast<int>(c.max_rows);
+  auto page_of = [&](int i, int& row) {
+    row = 0;
+    if (i < 0 || i >= max_rows) return -1;
+    const uint32_t lp = c.by_P(i);
+    row = i - static_cast<int>(lp) * c.P;
+    const int page = table[lp * c.sbt[1]];
+    return page < num_blocks ? page : -1;
+  };
+  uint8_t* const codes = pl.code + h * pl.sc[1];
+  float* const scales = pl.scale + h * pl.ss[1];
+  auto place = [&](int page, int row, float*& sc) {  // row and scale addresses
+    sc = page < 0 ? nullptr : scales + page * pl.ss[0] + c.by_group(row) * pl.ss[2];
+    return page < 0 ? nullptr : codes + page * pl.sc[0] + row * pl.sc[2];
   };
   auto fetch = [&](int w) {  // the rows of step w, whose addresses are in src[w & 1]
     const int rows = max(0, min(win, m - (first + w * step)));
@@ -382,18 +390,19 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
     }
   };
 
-  const float *sc0, *sc1;
-  int i1 = position(1), i2 = position(2);
+  float *sc0, *sc1;
+  int i1 = position(1), i2 = position(2), row;
   {
-    const int i0 = position(0);
-    uint8_t* x = place(kv8_page(c, s, i0), i0, sc0);
+    const int page = page_of(position(0), row);
+    uint8_t* x = place(page, row, sc0);
     if (tid < win) src[tid] = x;
   }
   float v0 = sc0 ? *sc0 : 0.f;
   __syncthreads();
   fetch(0);
   {
-    uint8_t* x = place(kv8_page(c, s, i1), i1, sc1);
+    const int page = page_of(i1, row);
+    uint8_t* x = place(page, row, sc1);
     if (tid < win) src[win + tid] = x;
   }
   cp_async_wait_all();
@@ -403,10 +412,11 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
     // loads for the steps ahead
     const float v1 = sc1 ? *sc1 : 0.f;
     if (w + 1 < steps) fetch(w + 1);
-    const int64_t page2 = kv8_page(c, s, i2);
+    int row2, drow;
+    const int page2 = page_of(i2, row2);
     const int i3 = position(w + 3);
     const bool mine = tid < rows;
-    const int64_t dpage = mine ? kv8_page(c, s, j0 + tid) : -1;
+    const int dpage = page_of(mine ? j0 + tid : -1, drow);
     // ---- this step's scales: the largest of each destination group ----
     float v_group = mine ? v0 : 0.f;
     if (by_shuffle) {
@@ -421,17 +431,17 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
         big = 0.f;
         for (int r = my_g0; r < min(rows, my_g0 + c.group); ++r) big = kv8_scale_max(big, was[r]);
       }
-      ratio[tid] = v0 < big ? v0 / big : 1.f;
-      const float* sc;
-      dst[tid] = place(dpage, j0 + tid, sc);
-      if (tid == my_g0 && sc) *const_cast<float*>(sc) = big;
+      float* sc;
+      uint8_t* y = place(dpage, drow, sc);
+      dst[tid] = {y, v0 < big ? v0 / big : 1.f};
+      if (tid == my_g0 && sc) *sc = big;
     }
     __syncthreads();
     // ---- write this step's rows ----
     const uint8_t* from = stage + static_cast<size_t>(w & 1) * win * D;
     auto store16 = [&](int r, int d) {
-      uint8_t* y = dst[r];
-      const float f = ratio[r];
+      uint8_t* y = dst[r].row;
+      const float f = dst[r].ratio;
       uint4 q = *reinterpret_cast<const uint4*>(from + r * D + d);
       if (f < 1.f) {
         q.x = kv8_rescale4<CODE>(q.x, f);
@@ -450,17 +460,17 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
         const int r = e / pieces, d = (e - r * pieces) * VEC;
         if (VEC == 16) {
           store16(r, d);
-        } else if (dst[r]) {
+        } else if (dst[r].row) {
           uint8_t q = from[r * D + d];
-          if (ratio[r] < 1.f) q = Kv8<CODE>::enc(Kv8<CODE>::dec(q) * ratio[r]);
-          dst[r][d * pl.sc[3]] = q;
+          if (dst[r].ratio < 1.f) q = Kv8<CODE>::enc(Kv8<CODE>::dec(q) * dst[r].ratio);
+          dst[r].row[d * pl.sc[3]] = q;
         }
       }
     }
     // ---- addresses two steps ahead (their slot's last reader was the fetch of step w) ----
     v0 = v1;
     {
-      uint8_t* x = place(page2, i2, sc1);
+      uint8_t* x = place(page2, row2, sc1);
       if (tid < win) src[(w & 1) * win + tid] = x;
     }
     i2 = i3;
@@ -560,7 +570,7 @@ int kv8_evict_launch(const Kv8View& c, int code_type, const int32_t* context_len
   if (win < c.group) win = c.group;
   if (win > 256) win = 256 / c.group * c.group;
   p.window = static_cast<int>(win);
-  const int64_t smem = (2 * win * c.D + 15) / 16 * 16 + 3 * win * 8 + 2 * win * 4;
+  const int64_t smem = (2 * win * c.D + 15) / 16 * 16 + 2 * win * 8 + win * 16 + win * 4;
   if (smem > 200 * 1024) return set_error(2, "kv8 evict: group * head_dim is too large");
   bool vec = c.D % 16 == 0;
   for (const Kv8Plane& pl : c.plane)
