@@ -158,6 +158,19 @@ def test_rotary_sizes(dtype, il, tokens, heads, kv, dim, rot, axes):
         check_rot(ko, k, pos, inv, sec, il, False)
 
 
+@pytest.mark.parametrize("dim", [64, 72])
+def test_write_ends_with_its_rows(dim):
+    """A cu_seqlens that runs past the rows of k and v writes those that there are."""
+    c = KC.make("past", 2, 2, 32, 16, dim, "int8", 120)
+    d = KC.to_device(c)
+    g = torch.Generator().manual_seed(2)
+    k, v = (torch.randn(60, 2, dim, generator=g).to(BF) for _ in range(2))
+    C8.kv8_cache_write(k.to(DEV), v.to(DEV), *d, dev32([3, 5]), dev32([0, 41, 90]))
+    for w, x in enumerate((k, v)):
+        c.write(w, x.float().numpy(), [3, 5], [0, 41, 60])
+    KC.same(c, d)
+
+
 def test_graph_keeps_its_scratch():
     """A captured call replays right after calls on its stream that needed more
     scratch, and after the memory that they gave back was overwritten."""

@@ -55,7 +55,9 @@ struct Kv8TcParams {
 
 // P is held times 2^kPBias: with the running maximum allowed to lag by kLag it
 // reaches 2^15 (fp16 ends at 2^16), and weights down to 2^-27 of the largest
-// keep fp16's full precision.  l holds sums of P / vs * 2^-kLBias, where P is
+// keep fp16's full precision.  Smaller ones, down to 2^-61, are summed apart while a
+// row has fewer than kFew larger ones; below that a weight adds nothing to O (it
+// still does to l).  l holds sums of P / vs * 2^-kLBias, where P is
 // unbiased: that keeps it in range for V scales down to kMinVs over long
 // contexts.
 constexpr float kPBias = 13.f;

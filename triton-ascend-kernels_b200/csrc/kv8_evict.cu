@@ -320,9 +320,11 @@ __global__ void __launch_bounds__(kSelThreads, KPT <= 8 ? 2 : 1) kv8_evict_selec
 // after row r of the windows: its position is read three steps ahead, its page two,
 // its scale one, so that no step waits for a chain of loads.
 //
-// Bound by the issue slots of the requantisation, then by memory: 36 x 8 heads x 2048
-// rows of 128, K and V, in 75 us (302 MB moved, 4.0 TB/s, 61 % of the measured copy
-// rate); one sequence's 8 heads x 16384 rows, over clusters of 16, in 30.
+// Bound by the issue slots of the requantisation and the row lookups (58 % issue),
+// then by memory: 36 x 8 heads x 2048 rows of 128, K and V, in 71 us (302 MB moved,
+// 4.3 TB/s, 65 % of the measured copy rate); one sequence's 8 heads x 16384 rows, over
+// clusters of 16, in 29.  Windows of 16 KB took 14 % longer.  Pieces held in registers
+// so that four CTAs fit an SM: 10 % less where that saves a wave, 25 % more elsewhere.
 template <int CODE, int VEC>
 __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_constant__ Kv8EvictParams p) {
   extern __shared__ __align__(16) uint8_t stage[];  // [2][window][D] codes, then per row:
