@@ -194,3 +194,19 @@ def test_graph_keeps_its_scratch():
     st.synchronize()
     assert torch.equal(want, got)
     assert all(bool((x == 255).all()) for x in keep)
+
+
+def test_large_scratch_is_not_kept(monkeypatch):
+    """Scratch above the limit is taken from the allocator for the call alone, with the same results."""
+    import paged_attention_kv8 as A
+    c = KC.make("scratch", 3, 2, 32, 16, 128, "int8", 700)
+    d = KC.to_device(c)
+    q = torch.randn(3, 40, 16, 128, generator=torch.Generator().manual_seed(5)).to(BF).to(DEV)
+    ctx = dev32([700, 44, 333])
+    w1, w2 = (torch.zeros(3, 2, 704, device=DEV) for _ in range(2))
+    a = paged_attention_kv8(q, *d, ctx, weights=w1)
+    monkeypatch.setattr(A, "_KEEP", 1 << 16)
+    monkeypatch.setattr(T, "_ws", {})
+    b = paged_attention_kv8(q, *d, ctx, weights=w2)
+    assert torch.equal(a, b) and torch.equal(w1, w2)
+    assert all(x.numel() <= 1 << 20 for x in T._ws.values())

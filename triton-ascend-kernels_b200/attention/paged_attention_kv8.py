@@ -11,6 +11,7 @@ import struct
 import _tak_b200 as _t
 from kv8_cache import _lens, describe
 
+_KEEP = 256 << 20  # bytes of scratch that a stream keeps at most
 _S3, _S4 = struct.Struct("=3q").pack, struct.Struct("=4q").pack
 
 
@@ -78,7 +79,10 @@ def paged_attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_tables, con
             scratch.data_ptr(), scratch.numel(), stream)
         if rc != 4:  # 4: the workspace is too small; nothing was launched
             break
-        scratch = _t.workspace_of(index, stream, L.tak_kv8_attention_workspace_size(desc, H, Lq, width, code))
+        need = L.tak_kv8_attention_workspace_size(desc, H, Lq, width, code)
+        # the scores of a long call with weights go back to the allocator after it
+        scratch = _t.workspace_of(index, stream, need) if need <= _KEEP else \
+            _t.torch.empty(need, dtype=_t.torch.uint8, device=q.device)
     if rc:
         _t.check(rc)
     return (out, lse) if return_lse else out
