@@ -1,0 +1,79 @@
+"""Attention over the 8-bit cache where V's scales lie at the ends of their range (GPU).
+
+Tolerances, derived before the first run (E32 = 2^-24).  Beside what
+kv8_cases.py derives, a tensor-core weight is 2^(s + log2 vs + 13 - M): sums of
+magnitudes up to 2 A each, A the largest |log2 vs| + 13 + |s| in base-2 units,
+so four roundings put 8 A E32 on the exponent, and M + 10 + log2 l puts three
+more, 6 A E32, on the log-sum-exp.  dv = 16 A E32 bounds both; outputs get 2 dv
+of the row's mass.  2^-133 is a bf16 subnormal's spacing.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+import _tak_b200 as T
+import kv8_cases as KC
+from paged_attention_kv8 import paged_attention_kv8
+from test_gpu_kv8 import dev32
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF = torch.bfloat16
+LEAST = {"int8": 2.0 ** -100 / 127, "e4m3": 2.0 ** -100 / 448}  # the smallest scales that a write makes
+
+SHAPES = [  # seqs, q heads, kv heads, dim, block, group, contexts, queries
+    (2, 4, 1, 128, 32, 16, [300, 33], 1),
+    (1, 8, 2, 64, 16, 16, [700], 1),
+    (2, 16, 1, 128, 64, 32, [257, 16], 1),
+    (1, 8, 1, 64, 16, 16, [500], 4),
+    (1, 10, 2, 256, 32, 16, [200], 1),
+    (1, 12, 1, 256, 32, 16, [200], 3),
+    (64, 16, 8, 64, 16, 16, [200 - i for i in range(64)], 1),  # items of two chunks inside one CTA
+    (64, 96, 8, 64, 16, 16, [200 - i for i in range(64)], 1),
+]
+
+
+def cache_of(key, i, code):
+    """A cache without a code of 0, so that every column of a row has the mass of its heaviest keys."""
+    seqs, _, hkv, dim, block, group, ctx, _ = SHAPES[i]
+    c = KC.make((key, i), seqs, hkv, block, group, dim, code, max(ctx))
+    for x in c.codes:
+        x[x == 0] = 1
+    return c
+
+
+def check(c, i, path):
+    seqs, H, hkv, dim, block, group, ctx, Lq = SHAPES[i]
+    q = torch.randn(seqs, Lq, H, dim, generator=torch.Generator().manual_seed(i)).to(BF)
+    d = KC.to_device(c)
+    weights = torch.zeros(seqs, hkv, c.table.shape[1] * block, device=DEV)
+    old = T.set_kernel_path(path)
+    try:
+        out, lse = paged_attention_kv8(q.to(DEV), *d, dev32(ctx), weights=weights, return_lse=True)
+    finally:
+        T.set_kernel_path(old)
+    assert T.last_kernel() == ("kv8_attention_generic" if path else "kv8_attention_tc")
+    ref, rlse, rw, size, mass = c.attend(q.double().numpy(), ctx)
+    out, lse, got_w = KC.numbers(out).astype(np.float64), lse.cpu().double().numpy(), weights.cpu().double().numpy()
+    ds = (dim + 64) * KC.E32 * size + 16 * KC.E32 + 16 * (135 + 1.5 * size) * KC.E32
+    fin = np.isfinite(rlse)
+    assert np.array_equal(np.isfinite(lse), fin)
+    assert (np.abs(lse[fin] - rlse[fin]) <= (ds + 8 * KC.E32 * (1 + np.abs(np.where(fin, rlse, 0))))[fin]).all(), \
+        np.abs(lse[fin] - rlse[fin]).max()
+    tol = (2 * ds.max() + 2.0 ** -20) * np.abs(rw) + 1e-12
+    assert (np.abs(got_w - rw) <= tol).all(), np.abs(got_w - rw).max()
+    tol = KC.ULP[BF] * 1.001 * np.abs(ref) + (2 * ds + 2.0 ** -11)[..., None] * mass + 2.0 ** -133
+    bad = ~(np.abs(out - ref) <= tol)
+    assert not bad.any(), (bad.sum(), out[bad][:4], ref[bad][:4])
+
+
+@pytest.mark.parametrize("path", [0, 1])
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("i", range(len(SHAPES)))
+def test_smallest_v_scales(i, code, path):
+    """Every V group at the smallest scales that a write makes."""
+    c = cache_of("least", i, code)
+    g = np.random.default_rng(i)
+    c.scales[1][:] = (LEAST[code] * 2.0 ** g.uniform(0, 1.8, c.scales[1].shape)).astype(np.float32)
+    check(c, i, path)

@@ -67,7 +67,7 @@ constexpr float kLBiasInv = 1.1920928955078125e-7f;  // 2^-(kPBias + kLBias)
 constexpr float kNoMax = -3e38f;             // maximum of a row that has seen no key: finite, so that no difference is inf - inf
 constexpr float kHalfMin = 6.103515625e-5f;  // 2^-14: fp16's smallest normal number
 constexpr int kFew = 8;
-constexpr float kMinVs = 6.162975822039155e-33f;  // 2^-107: the smallest scale that the write makes
+constexpr float kMinVs = 1.5407439555097887e-33f;  // 2^-109: below the smallest scale that a write makes, 2^-100 / 448 (e4m3)
 
 // DP: head dim rounded up to 64, 128 or 256.
 template <int DP> struct Kv8Base {
