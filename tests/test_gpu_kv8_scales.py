@@ -77,3 +77,42 @@ def test_smallest_v_scales(i, code, path):
     g = np.random.default_rng(i)
     c.scales[1][:] = (LEAST[code] * 2.0 ** g.uniform(0, 1.8, c.scales[1].shape)).astype(np.float32)
     check(c, i, path)
+
+
+KINDS = {  # scales of V's groups; one in `every` is `odd`, the others `usual` (exponents of 2, or 0)
+    "zeros beside large": (3, None, (36, 60)),
+    "few zeros beside large": (7, None, (36, 60)),
+    "small beside large": (2, (-100, -80), (40, 90)),
+    "few large": (9, (60, 100), (-4, 4)),
+    "all over": (2, (-108, 100), (-108, 100)),
+    "all zero but few": (5, (-3, 90), None),
+}
+
+
+@pytest.mark.parametrize("path", [1])
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("i", range(len(SHAPES)))
+def test_v_scales_far_apart(i, kind, code, path):
+    """Every key counts in the softmax whatever its group's V scale is beside
+    the others'; scales of 0 among them."""
+    c = cache_of(kind, i, code)
+    every, odd, usual = KINDS[kind]
+    g = np.random.default_rng(i)
+
+    def draw(span):
+        z = np.zeros(c.scales[1].shape)
+        return z if span is None else 2.0 ** g.uniform(*span, z.shape)
+
+    c.scales[1][:] = np.where(g.integers(0, every, c.scales[1].shape) == 0, draw(odd), draw(usual)).astype(np.float32)
+    check(c, i, path)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("i", range(len(SHAPES)))
+def test_largest_values_on_cuda_cores(i, code):
+    """Sums of values near fp32's largest stay finite before they are divided by the softmax's sum."""
+    c = cache_of("most", i, code)
+    top = 120 if code == "int8" else 118
+    c.scales[1][:] = (2.0 ** np.random.default_rng(i).uniform(top - 14, top, c.scales[1].shape)).astype(np.float32)
+    check(c, i, 1)

@@ -7,6 +7,11 @@
 // exponentials; every query row reads the cache again (64 x <= 8192 keys, 32 heads of
 // 128, bf16: 10.7 ms against 0.1 on tensor cores), so it serves the shapes that those
 // do not take.
+//
+// The values are summed against a reference of their own: with vs = 2^E v, 1/2 <= v
+// < 1, acc = sum_j 2^((s_j - rs) + (E_j - re)) v_j Vc_j, (rs, re) the score and the
+// exponent of the key with the largest s_j + E_j.  So a weight too small for fp32
+// under a large V keeps its part, and sums of values near fp32's largest stay finite.
 #include "kv8.cuh"
 
 namespace tak {
@@ -48,7 +53,8 @@ __global__ void __launch_bounds__(128) kv8_attention_generic_kernel(const Kv8Gen
     qr[e] = d < c.D ? Elem<T>::to_f(q[d * p.sq[3]]) : 0.f;
     acc[e] = 0.f;
   }
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f, rs = -INFINITY;
+  int re = 0;
   for (int64_t r = warp; r < lim; r += 4) {
     const int64_t page = kv8_page(c, s, r);
     const int row = static_cast<int>(r % c.P);
@@ -68,39 +74,63 @@ __global__ void __launch_bounds__(128) kv8_attention_generic_kernel(const Kv8Gen
     const float sc = kv8_score2(dot, p.scale, p.softcap);
     const float mn = fmaxf(m, sc);
     const float mu = mn == -INFINITY ? 0.f : mn;
-    const float a = exp2f(m - mu), e2 = exp2f(sc - mu);
-    l = l * a + e2;
+    l = l * exp2f(m - mu) + exp2f(sc - mu);
     m = mn;
+    if (vs == 0.f) continue;  // zero rows add to l only
+    int ve;
+    const float vm = frexpf(vs, &ve);
+    if (!(fabsf(vs) < INFINITY)) ve = 0;
+    if (rs == -INFINITY || (sc - rs) + (ve - re) > 0.f) {
+      const float a = rs == -INFINITY ? 0.f : exp2f((rs - sc) + (re - ve));
+      rs = sc;
+      re = ve;
+#pragma unroll
+      for (int e = 0; e < kKv8MaxPerLane; ++e) acc[e] *= a;
+    }
+    const float e2 = (rs == -INFINITY ? 0.f : exp2f((sc - rs) + (ve - re))) * vm;
 #pragma unroll
     for (int e = 0; e < kKv8MaxPerLane; ++e) {
       const int d = lane + 32 * e;
-      acc[e] *= a;
-      if (d < c.D && page >= 0) acc[e] += e2 * (vs * Kv8<CODE>::dec(vr[d * c.plane[1].sc[3]]));
+      if (d < c.D) acc[e] += e2 * Kv8<CODE>::dec(vr[d * c.plane[1].sc[3]]);
     }
   }
-  __shared__ float sm_m[4], sm_l[4];
+  __shared__ float sm_m[4], sm_l[4], sm_rs[4];
+  __shared__ int sm_re[4];
   __shared__ float sm_o[4][32 * kKv8MaxPerLane];
   if (lane == 0) {
     sm_m[warp] = m;
     sm_l[warp] = l;
+    sm_rs[warp] = rs;
+    sm_re[warp] = re;
   }
 #pragma unroll
   for (int e = 0; e < kKv8MaxPerLane; ++e) sm_o[warp][lane + 32 * e] = acc[e];
   __syncthreads();
   const float M = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
   const float Mu = (M == -INFINITY) ? 0.f : M;
-  float L = 0.f, f[4];
+  float L = 0.f, f[4], RS = -INFINITY;
+  int RE = 0;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    f[w] = exp2f(sm_m[w] - Mu);
-    L += sm_l[w] * f[w];
+    L += sm_l[w] * exp2f(sm_m[w] - Mu);
+    if (sm_rs[w] == -INFINITY) continue;
+    if (RS == -INFINITY || (sm_rs[w] - RS) + (sm_re[w] - RE) > 0.f) {
+      RS = sm_rs[w];
+      RE = sm_re[w];
+    }
   }
+#pragma unroll
+  for (int w = 0; w < 4; ++w) f[w] = sm_rs[w] == -INFINITY ? 0.f : exp2f((sm_rs[w] - RS) + (sm_re[w] - RE));
+  // 2^(RS - M + RE), its whole part as an exponent
+  const float diff = RS == -INFINITY ? 0.f : RS - Mu, whole = rintf(fmaxf(diff, -400.f));
+  const float part = exp2f(fmaxf(diff, -400.f) - whole);
   T* out = static_cast<T*>(p.out) + s * p.so[0] + i * p.so[1] + h * p.so[2];
   for (int d = threadIdx.x; d < c.D; d += 128) {
     float o = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) o += sm_o[w][d] * f[w];
-    out[d * p.so[3]] = Elem<T>::from_f(L != 0.f ? o / L : 0.f);  // NaN scores give NaN, no key gives 0
+    // NaN scores give NaN, no key gives 0
+    out[d * p.so[3]] = Elem<T>::from_f(L != 0.f ? ldexpf(o * part / L, static_cast<int>(whole) + RE) : 0.f);
   }
   if (threadIdx.x == 0) {
     const float lse2 = L != 0.f ? M + log2f(L) : -INFINITY;
