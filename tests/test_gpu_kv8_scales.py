@@ -89,7 +89,7 @@ KINDS = {  # scales of V's groups; one in `every` is `odd`, the others `usual` (
 }
 
 
-@pytest.mark.parametrize("path", [1])
+@pytest.mark.parametrize("path", [0, 1])
 @pytest.mark.parametrize("code", ["int8", "e4m3"])
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("i", range(len(SHAPES)))
@@ -116,3 +116,30 @@ def test_largest_values_on_cuda_cores(i, code):
     top = 120 if code == "int8" else 118
     c.scales[1][:] = (2.0 ** np.random.default_rng(i).uniform(top - 14, top, c.scales[1].shape)).astype(np.float32)
     check(c, i, 1)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("i", range(len(SHAPES)))
+def test_largest_v_scales(i, code):
+    """Values up to 2^127: the softmax's sum, in units of the largest value, is
+    near fp32's smallest numbers."""
+    c = cache_of("most", i, code)
+    top = 120 if code == "int8" else 118
+    c.scales[1][:] = (2.0 ** np.random.default_rng(i).uniform(top - 14, top, c.scales[1].shape)).astype(np.float32)
+    check(c, i, 0)
+
+
+def test_zero_v_scale_beside_a_large_one():
+    """Two keys of equal scores, V of one zero and of the other large: half of the large one."""
+    c = KC.make("half", 1, 1, 16, 16, 64, "int8", 32)
+    c.codes[0][:] = 1
+    c.scales[0][:] = 1
+    c.scales[1][c.table[0, 0]] = 0
+    c.scales[1][c.table[0, 1]] = 2.0 ** 40
+    c.codes[1][c.table[0, 1]] = 100
+    d = KC.to_device(c)
+    q = torch.ones(1, 4, 64, dtype=BF, device=DEV)
+    weights = torch.zeros(1, 1, 32, device=DEV)
+    out = paged_attention_kv8(q, *d, dev32([32]), weights=weights)
+    assert (out.float().cpu() / (50 * 2.0 ** 40) - 1).abs().max().item() < 2.0 ** -8
+    assert (weights.cpu() * 8 - 1).abs().max().item() < 1e-5

@@ -57,9 +57,12 @@ struct Kv8TcParams {
 // reaches 2^15 (fp16 ends at 2^16), and weights down to 2^-27 of the largest
 // keep fp16's full precision.  Smaller ones, down to 2^-61, are summed apart while a
 // row has fewer than kFew larger ones; below that a weight adds nothing to O (it
-// still does to l).  l holds sums of P / vs * 2^-kLBias, where P is
-// unbiased: that keeps it in range for V scales down to kMinVs over long
-// contexts.
+// still does to l).  l holds the sum of 2^(s - M - kLBias), formed as P / vs while
+// every V scale of the item lies within 2^kFar of 1.  From the first tile of another
+// scale on (0 among them) P may underflow where the score does not, or 1 / vs leave
+// fp32's normal numbers, so l is summed from the scores themselves (kv8_add_term).  With
+// M - s between -109 and 121 for the heaviest key, it stays in fp32 (at the upper end
+// with 18 bits) for up to 2^26 keys.
 constexpr float kPBias = 13.f;
 constexpr float kLag = 2.f;
 constexpr float kLBias = 10.f;
@@ -67,7 +70,11 @@ constexpr float kLBiasInv = 1.1920928955078125e-7f;  // 2^-(kPBias + kLBias)
 constexpr float kNoMax = -3e38f;             // maximum of a row that has seen no key: finite, so that no difference is inf - inf
 constexpr float kHalfMin = 6.103515625e-5f;  // 2^-14: fp16's smallest normal number
 constexpr int kFew = 8;
-constexpr float kMinVs = 1.5407439555097887e-33f;  // 2^-109: below the smallest scale that a write makes, 2^-100 / 448 (e4m3)
+constexpr float kFar = 48.f;
+// The smallest scale that a write makes is 2^-100 / 448 (e4m3); one of kMinVs or less
+// is 0.  Its keys count in the maximum as if it were kMinVs, for l's sake, and have P = 0.
+constexpr float kMinVs = 1.5407439555097887e-33f;  // 2^-109
+constexpr float kMinLv = kPBias - 109.f;
 
 // DP: head dim rounded up to 64, 128 or 256.
 template <int DP> struct Kv8Base {
@@ -81,7 +88,7 @@ template <int DP> struct Kv8Base {
   static constexpr int STAGE = 2 * PLANE;
   static constexpr int NS = DP == 64 ? 4 : 2;
   static constexpr int THREADS = (NW + 1) * 32;
-  static constexpr int META_OFF = NS * STAGE;           // [NS][3][NT] floats: ks, log2 vs + kPBias, 2^-23 / vs
+  static constexpr int META_OFF = NS * STAGE;           // [NS][3][NT] floats: ks, log2 vs + kPBias, 2^-23 / vs or 0
   static constexpr int BAR_OFF = META_OFF + NS * 3 * NT * 4;
   static constexpr int OWN_OFF = BAR_OFF + 2 * NS * 8;  // the kernel's own shared memory
 };
@@ -183,6 +190,20 @@ __device__ __forceinline__ void kv8_cap(float (&x)[4], float inv_cap, float cap2
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] = t[e] * cap2;
+}
+
+// l + 2^(x - kLBias), and l + v 2^d with h = 2^(d / 2): by two factors, as the product
+// may be subnormal (ex2 ends at 2^-126) and v 2^d be normal where 2^d is not
+__device__ __forceinline__ float kv8_add_term(float l, float x) {
+  const float h = fast_exp2(fmaf(0.5f, x, -0.5f * kLBias));
+  return fmaf(h, h, l);
+}
+__device__ __forceinline__ float kv8_add_down(float l, float v, float h) { return fmaf(v * h, h, l); }
+// out = o * pre * inv: 2^-(kPBias + kLBias) / l, in two factors where one would be subnormal
+__device__ __forceinline__ float2 kv8_over(float l) {
+  const bool large = l > 18446744073709551616.f;  // 2^64
+  const float inv = l != 0.f ? (large ? kLBiasInv * 18446744073709551616.f : kLBiasInv) / l : 0.f;
+  return make_float2(large ? 5.42101086242752217e-20f : 1.f, inv);
 }
 
 __device__ __forceinline__ int kv8_ctx(const Kv8TcParams& p, int s) {
@@ -333,6 +354,7 @@ __device__ __forceinline__ void kv8_produce(const Kv8TcParams& p, const CUtensor
   tma_prefetch_desc(&tmV);
   const int nbox = CH / p.box_rows, tiles_per_box = p.box_rows / 16;
   struct Meta { int64_t page; int row, kvh, ctx, tok0; float ks, vs; };
+  bool wide = false;  // a V scale of the item, up to this chunk, lies beyond 2^kFar
   auto fetch_page = [&](const Kv8Walk<CH>& w, bool live) {
     Meta m{};
     m.page = -1;
@@ -395,13 +417,15 @@ __device__ __forceinline__ void kv8_produce(const Kv8TcParams& p, const CUtensor
       }
     }
     fetch_scales(nxt);
+    const bool bad = !(cur.vs < INFINITY);  // NaN or inf
+    const bool past = cur.tok0 + lane * 16 >= cur.ctx;  // no key: a scale like any other's
+    const float v = bad || past ? 1.f : fmaxf(cur.vs, kMinVs), lv = v > kMinVs ? log2f(v) + kPBias : kMinLv;
+    wide = __any_sync(0xffffffffu, lane < NT && fabsf(lv - kPBias) > kFar) || (wide && cur.tok0 > 0);
     if (lane < NT) {
       float* mt = meta + st * 3 * NT;
-      const bool bad = !(cur.vs < INFINITY);  // NaN or inf
-      const float v = bad ? 1.f : fmaxf(cur.vs, kMinVs);
       mt[lane] = cur.ks;
-      mt[NT + lane] = bad ? __uint_as_float(0x7fffffffu) : log2f(v) + kPBias;
-      mt[2 * NT + lane] = kLBiasInv / v;
+      mt[NT + lane] = bad ? __uint_as_float(0x7fffffffu) : lv;
+      mt[2 * NT + lane] = wide ? 0.f : kLBiasInv / v;
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&full[st]);
@@ -646,9 +670,10 @@ __global__ void __launch_bounds__(Kv8Few<DP>::THREADS, Kv8Few<DP>::CTAS)
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
             const float mn = fmaxf(m[k], mx);
-            al[k] = fast_exp2(m[k] - mn);
+            const float h = fast_exp2(0.5f * (m[k] - mn));
+            al[k] = h * h;
             m[k] = mn;
-            l[k] *= al[k];
+            l[k] = kv8_add_down(0.f, l[k], h);
             above[k] = 0;
           }
 #pragma unroll
@@ -659,6 +684,14 @@ __global__ void __launch_bounds__(Kv8Few<DP>::THREADS, Kv8Few<DP>::CTAS)
             o[i][3] *= al[1];
           }
           many = false;
+        }
+        if (ivs[0] == 0.f) {  // a scale beyond 2^kFar in this chunk or before it
+#pragma unroll
+          for (int u = 0; u < TP; ++u) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) l[e & 1] = kv8_add_term(l[e & 1], x[u][e] - m[e & 1]);
+            if (lv[u] == kMinLv) lv[u] = -INFINITY;
+          }
         }
         uint32_t pb[TP][2];  // P^T fragments
 #pragma unroll
@@ -806,8 +839,8 @@ __global__ void __launch_bounds__(Kv8Few<DP>::THREADS, Kv8Few<DP>::CTAS)
 #pragma unroll
         for (int k = 0; k < NW; ++k) {
           const int at = k * 8 + row;
-          const float f = fast_exp2(mlbuf[at * 2] - Mu);
-          L = fmaf(mlbuf[at * 2 + 1], f, L);
+          const float hf = fast_exp2(0.5f * (mlbuf[at * 2] - Mu)), f = hf * hf;
+          L = kv8_add_down(L, mlbuf[at * 2 + 1], hf);
           const float4 v = *reinterpret_cast<const float4*>(obuf + at * C::OLD + d);
           a.x = fmaf(v.x, f, a.x);
           a.y = fmaf(v.y, f, a.y);
@@ -817,9 +850,9 @@ __global__ void __launch_bounds__(Kv8Few<DP>::THREADS, Kv8Few<DP>::CTAS)
         const int dd = dh * C::DH + d;
         if (whole) {
           const int i = grow / p.G, h = kvh * p.G + grow - i * p.G;
-          const float inv = L != 0.f ? kLBiasInv / L : 0.f;
+          const float2 over = kv8_over(L);
           uint16_t* out = static_cast<uint16_t*>(p.out) + s * p.so[0] + i * p.so[1] + h * p.so[2];
-          const float f[4] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv};
+          const float f[4] = {a.x * over.x * over.y, a.y * over.x * over.y, a.z * over.x * over.y, a.w * over.x * over.y};
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             if (dd + k < p.c.D)
@@ -1108,9 +1141,10 @@ __global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTA
             float mn = m[n][k];
 #pragma unroll
             for (int i = 0; i < NW; ++i) mn = fmaxf(mn, smax[i * RT + n * 8 + 2 * t4 + k]);
-            al[k] = fast_exp2(m[n][k] - mn);
+            const float h = fast_exp2(0.5f * (m[n][k] - mn));
+            al[k] = h * h;
             m[n][k] = mn;
-            l[n][k] *= al[k];
+            l[n][k] = kv8_add_down(0.f, l[n][k], h);
           }
           above[n] = 0;
 #pragma unroll
@@ -1126,17 +1160,31 @@ __global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTA
       // ---- this warp's weights, as P^T fragments for everyone ----
       bool apart = false;
       if (tok < ctx) {
+        if (ivs[0] == 0.f) {  // a scale beyond 2^kFar in this chunk or before it
 #pragma unroll
-        for (int u = 0; u < TP; ++u)
+          for (int u = 0; u < TP; ++u) {
+            const float lz = lv[u] == kMinLv ? -INFINITY : lv[u];
 #pragma unroll
-          for (int n = 0; n < NR; ++n)
+            for (int n = 0; n < NR; ++n)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float c0 = lv[u] - m[n][k];
-              x[u][n][k] = fast_exp2(x[u][n][k] + c0);
-              x[u][n][k + 2] = fast_exp2(x[u][n][k + 2] + c0);
-              l[n][k] = fmaf(x[u][n][k] + x[u][n][k + 2], ivs[u], l[n][k]);
-            }
+              for (int e = 0; e < 4; ++e) {
+                l[n][e & 1] = kv8_add_term(l[n][e & 1], x[u][n][e] - m[n][e & 1]);
+                x[u][n][e] = fast_exp2(x[u][n][e] + (lz - m[n][e & 1]));
+              }
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < TP; ++u)
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float c0 = lv[u] - m[n][k];
+                x[u][n][k] = fast_exp2(x[u][n][k] + c0);
+                x[u][n][k + 2] = fast_exp2(x[u][n][k + 2] + c0);
+                l[n][k] = fmaf(x[u][n][k] + x[u][n][k + 2], ivs[u], l[n][k]);
+              }
+        }
         if (!many) {  // weights below fp16's normal range go apart, as in the other kernel
           float least = 1.f;
           int fewest = kFew;
@@ -1284,14 +1332,14 @@ __global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTA
         const int d0 = warp * C::CW + 2 * g;
         if (whole) {
           const int i = grow / p.G, h = kvh * p.G + grow - i * p.G;
-          const float inv = L != 0.f ? kLBiasInv / L : 0.f;
+          const float2 over = kv8_over(L);
           uint16_t* out = static_cast<uint16_t*>(p.out) + s * p.so[0] + i * p.so[1] + h * p.so[2];
 #pragma unroll
           for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               const int d = d0 + mb * 16 + c;
-              const float f = o[mb][n][2 * c + k] * inv;
+              const float f = o[mb][n][2 * c + k] * over.x * over.y;
               if (d < p.c.D) out[d * p.so[3]] = p.bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f)) : __half_as_ushort(__float2half_rn(f));
             }
           if (warp == 0 && g == 0) {
@@ -1352,27 +1400,27 @@ __global__ void __launch_bounds__(DP) kv8_attention_join_kernel(const __grid_con
     float Mn = M;
 #pragma unroll
     for (int u = 0; u < 8; ++u) Mn = fmaxf(Mn, ml[u].x);
-    const float f0 = fast_exp2(M - Mn);
+    const float h0 = fast_exp2(0.5f * (M - Mn)), f0 = h0 * h0;
+    L = kv8_add_down(0.f, L, h0);
     M = Mn;
-    L *= f0;
     o.x *= f0;
     o.y *= f0;
     o.z *= f0;
     o.w *= f0;
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const float f = fast_exp2(ml[u].x - M);
-      L = fmaf(ml[u].y, f, L);
+      const float h = fast_exp2(0.5f * (ml[u].x - M)), f = h * h;
+      L = kv8_add_down(L, ml[u].y, h);
       o.x = fmaf(v[u].x, f, o.x);
       o.y = fmaf(v[u].y, f, o.y);
       o.z = fmaf(v[u].z, f, o.z);
       o.w = fmaf(v[u].w, f, o.w);
     }
   }
-  const float inv = L != 0.f ? kLBiasInv / L : 0.f;
+  const float2 over = kv8_over(L);
   const int i = grow / p.G, h = kvh * p.G + grow - i * p.G;
   uint16_t* out = static_cast<uint16_t*>(p.out) + s * p.so[0] + i * p.so[1] + h * p.so[2];
-  const float f[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+  const float f[4] = {o.x * over.x * over.y, o.y * over.x * over.y, o.z * over.x * over.y, o.w * over.x * over.y};
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if (d + k < p.c.D)
