@@ -30,6 +30,7 @@ struct Kv8EvictParams {
   int32_t* kept;      // [B, Hkv, budget]
   int32_t* new_lens;  // [B]
   int window;         // rows moved at a time, a multiple of group
+  int stages;         // windows in shared memory: 2, or 1 where two do not fit
 };
 
 __device__ __forceinline__ int kv8_evict_rows(const Kv8EvictParams& p, int s) {
@@ -327,14 +328,15 @@ __global__ void __launch_bounds__(kSelThreads, KPT <= 8 ? 2 : 1) kv8_evict_selec
 // so that four CTAs fit an SM: 10 % less where that saves a wave, 25 % more elsewhere.
 template <int CODE, int VEC>
 __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_constant__ Kv8EvictParams p) {
-  extern __shared__ __align__(16) uint8_t stage[];  // [2][window][D] codes, then per row:
+  extern __shared__ __align__(16) uint8_t stage[];  // [stages][window][D] codes, then per row:
   cg::cluster_group cluster = cg::this_cluster();
   const Kv8View& c = p.c;
   const int cs = cluster.num_blocks(), rank = cluster.block_rank();
   const int h = blockIdx.x / cs, s = blockIdx.y, tid = threadIdx.x, D = c.D, pieces = D / VEC;
   const Kv8Plane pl = blockIdx.z ? c.plane[1] : c.plane[0];
   const int win = p.window;
-  const uint8_t** src = reinterpret_cast<const uint8_t**>(stage + (2 * static_cast<size_t>(win) * D + 15) / 16 * 16);  // [2][win]
+  const int flip = p.stages - 1;  // step w uses stage w & flip
+  const uint8_t** src = reinterpret_cast<const uint8_t**>(stage + (p.stages * static_cast<size_t>(win) * D + 15) / 16 * 16);  // [2][win]
   struct alignas(16) Dst { uint8_t* row; float ratio; };
   Dst* dst = reinterpret_cast<Dst*>(const_cast<uint8_t**>(src + 2 * win));                           // [win]
   float* was = reinterpret_cast<float*>(dst + win);                                                  // [win] scales
@@ -373,7 +375,7 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
   };
   auto fetch = [&](int w) {  // the rows of step w, whose addresses are in src[w & 1]
     const int rows = max(0, min(win, m - (first + w * step)));
-    uint8_t* to = stage + static_cast<size_t>(w & 1) * win * D;
+    uint8_t* to = stage + static_cast<size_t>(w & flip) * win * D;
     const uint8_t** from = src + (w & 1) * win;
     if (VEC == 16 && 256 % pieces == 0) {
       const int d = (tid % pieces) * 16;
@@ -413,7 +415,7 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
     const int j0 = first + w * step, rows = max(0, min(win, m - j0));
     // loads for the steps ahead
     const float v1 = sc1 ? *sc1 : 0.f;
-    if (w + 1 < steps) fetch(w + 1);
+    if (flip && w + 1 < steps) fetch(w + 1);
     int row2, drow;
     const int page2 = page_of(i2, row2);
     const int i3 = position(w + 3);
@@ -440,7 +442,7 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
     }
     __syncthreads();
     // ---- write this step's rows ----
-    const uint8_t* from = stage + static_cast<size_t>(w & 1) * win * D;
+    const uint8_t* from = stage + static_cast<size_t>(w & flip) * win * D;
     auto store16 = [&](int r, int d) {
       uint8_t* y = dst[r].row;
       const float f = dst[r].ratio;
@@ -468,6 +470,10 @@ __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_consta
           dst[r].row[d * pl.sc[3]] = q;
         }
       }
+    }
+    if (!flip && w + 1 < steps) {  // one stage: the next step's rows once this one's are out of it
+      __syncthreads();
+      fetch(w + 1);
     }
     // ---- addresses two steps ahead (their slot's last reader was the fetch of step w) ----
     v0 = v1;
@@ -548,6 +554,29 @@ int kv8_evict_launch(const Kv8View& c, int code_type, const int32_t* context_len
   p.recent = static_cast<int>(recent);
   p.kept = kept;
   p.new_lens = new_lens;
+  // ---- move: windows of about 32 KB of rows, a multiple of the group; two of them in
+  // shared memory, one where a wide group leaves no room (at most 256 x 640 codes) ----
+  int64_t win = 32768 / c.D / c.group * c.group;
+  if (win < c.group) win = c.group;
+  if (win > 256) win = 256 / c.group * c.group;
+  p.window = static_cast<int>(win);
+  auto smem_of = [&](int64_t stages) { return (stages * win * c.D + 15) / 16 * 16 + 2 * win * 8 + win * 16 + win * 4; };
+  p.stages = smem_of(2) <= 200 * 1024 ? 2 : 1;
+  const int smem = static_cast<int>(smem_of(p.stages));
+  bool vec = c.D % 16 == 0;
+  for (const Kv8Plane& pl : c.plane)
+    vec = vec && pl.sc[3] == 1 && (reinterpret_cast<uintptr_t>(pl.code) & 15) == 0 && ((pl.sc[0] | pl.sc[1] | pl.sc[2]) & 15) == 0;
+  void (*move)(const Kv8EvictParams) = nullptr;
+  TAK_BY_CODE(code_type, move = vec ? kv8_evict_move_kernel<CODE, 16> : kv8_evict_move_kernel<CODE, 1>);
+  // (whatever can be refused is refused here: the selection already changes `weights`)
+  if (const int r = ensure_smem_attr(reinterpret_cast<const void*>(move), smem)) return r;
+  // a cluster per (sequence, head, K or V), of several CTAs where there are fewer
+  // of them than fill the SMs
+  const int64_t units = 2 * static_cast<int64_t>(c.Hkv) * c.num_seqs;
+  int move_cs = 1;
+  while (move_cs < 16 && units * move_cs < num_sms() && move_cs * win < budget) move_cs *= 2;
+  if (move_cs == 16 && !cluster16_ok(reinterpret_cast<const void*>(move), 256, static_cast<size_t>(smem))) move_cs = 8;
+
   // ---- selection: in registers up to 8 CTAs x 1024 threads x 16 weights ----
   const int64_t rows = width < c.max_rows ? width : c.max_rows;
   const int64_t sel = kSelThreads;
@@ -567,28 +596,7 @@ int kv8_evict_launch(const Kv8View& c, int code_type, const int32_t* context_len
   } else {
     kv8_evict_select_kernel<<<dim3(c.Hkv, c.num_seqs), kSelThreads, 0, st>>>(p);
   }
-  // ---- move: windows of about 32 KB of rows, a multiple of the group ----
-  int64_t win = 32768 / c.D / c.group * c.group;
-  if (win < c.group) win = c.group;
-  if (win > 256) win = 256 / c.group * c.group;
-  p.window = static_cast<int>(win);
-  const int64_t smem = (2 * win * c.D + 15) / 16 * 16 + 2 * win * 8 + win * 16 + win * 4;
-  if (smem > 200 * 1024) return set_error(2, "kv8 evict: group * head_dim is too large");
-  bool vec = c.D % 16 == 0;
-  for (const Kv8Plane& pl : c.plane)
-    vec = vec && pl.sc[3] == 1 && (reinterpret_cast<uintptr_t>(pl.code) & 15) == 0 && ((pl.sc[0] | pl.sc[1] | pl.sc[2]) & 15) == 0;
-  TAK_BY_CODE(code_type, {
-    auto kern = vec ? kv8_evict_move_kernel<CODE, 16> : kv8_evict_move_kernel<CODE, 1>;
-    if (const int r = ensure_smem_attr(reinterpret_cast<const void*>(kern), static_cast<int>(smem))) return r;
-    // a cluster per (sequence, head, K or V), of several CTAs where there are fewer
-    // of them than fill the SMs
-    const int64_t units = 2 * static_cast<int64_t>(c.Hkv) * c.num_seqs;
-    int cs = 1;
-    while (cs < 16 && units * cs < num_sms() && cs * win < budget) cs *= 2;
-    if (cs == 16 && !cluster16_ok(reinterpret_cast<const void*>(kern), 256, static_cast<size_t>(smem))) cs = 8;
-    return launch_cluster(kern, dim3(c.Hkv * cs, c.num_seqs, 2), 256, static_cast<size_t>(smem), cs, true, st, p);
-  });
-  return 0;
+  return launch_cluster(move, dim3(c.Hkv * move_cs, c.num_seqs, 2), 256, static_cast<size_t>(smem), move_cs, true, st, p);
 }
 
 }  // namespace tak
