@@ -410,7 +410,9 @@ int tak_kv8_read(const tak_kv8_cache* cache, const int32_t* cu_seqlens, const in
  * (keys at or past weights_width are left out).  workspace: at least
  * tak_kv8_attention_workspace_size() bytes, 16-byte aligned, no initialisation
  * needed; pass that function weights_width = 0 when weights is NULL.  It
- * returns -1 for arguments that the call would refuse.
+ * returns -1 for arguments that the call would refuse.  A call is two or three
+ * launches that hand data on through the workspace: calls whose launches may
+ * alternate (of several threads, or on several streams) need one each.
  */
 int64_t tak_kv8_attention_workspace_size(const tak_kv8_cache* cache, int64_t num_q_heads, int64_t num_queries,
                                          int64_t weights_width, int dtype);

@@ -1,0 +1,57 @@
+"""CPU-side checks of the scratch that calls share and of the 8-bit cache's limits."""
+
+import ctypes
+import threading
+
+import torch
+
+import _tak_b200 as T
+
+CPU = torch.device("cpu", 0)
+
+
+def scratch(stream, nbytes):
+    return T.workspace(CPU, ctypes.c_void_p(stream), nbytes)
+
+
+def test_threads_on_one_stream_have_their_own_scratch(monkeypatch):
+    """The launches of two threads' calls may alternate on a stream, so what one
+    call hands from launch to launch must not lie in the other's buffer."""
+    monkeypatch.setattr(T, "_ws", {})
+    both, got = threading.Barrier(2), {}
+
+    def work(name):
+        both.wait()
+        a = scratch(7, 64)
+        both.wait()  # both threads are alive: neither has the other's identity
+        b = scratch(7, 64)
+        got[name] = (a.data_ptr(), b.data_ptr(), T.workspace_of(0, 7, 64).data_ptr(), scratch(8, 64).data_ptr())
+        both.wait()
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in "ab"]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for first, again, by_index, other_stream in got.values():
+        assert first == again == by_index and other_stream != first
+    assert got["a"][0] != got["b"][0]
+
+
+def test_scratch_grows_and_is_kept(monkeypatch):
+    monkeypatch.setattr(T, "_ws", {})
+    a = scratch(3, 64)
+    assert scratch(3, a.numel()) is a
+    b = scratch(3, a.numel() + 1)
+    assert b.numel() > a.numel() and scratch(3, 64) is b and T.workspace_of(0, 3) is b
+
+
+def test_scratch_of_ended_threads_is_given_back(monkeypatch):
+    monkeypatch.setattr(T, "_ws", {})
+    mine = scratch(3, 64)
+    t = threading.Thread(target=scratch, args=(4, 64))
+    t.start()
+    t.join()
+    assert len(T._ws) == 2
+    scratch(5, 64)
+    assert sorted(k[1] for k in T._ws) == [3, 5] and scratch(3, 64) is mine

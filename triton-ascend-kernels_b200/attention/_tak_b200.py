@@ -165,19 +165,27 @@ _ws = {}
 def workspace_of(index, stream, nbytes=0):
     """The (device, stream)'s scratch buffer of workspace(), as it is or grown to
     nbytes, keyed by plain ints."""
-    buf = _ws.get((index, stream))
+    buf = _ws.get((index, stream, threading.get_ident()))
     if buf is None or buf.numel() < nbytes:
         buf = workspace(torch.device("cuda", index), ctypes.c_void_p(stream), nbytes)
     return buf
 
 
 def workspace(device, stream_handle, nbytes):
-    """Per-(device, stream) scratch buffer, grown on demand.  Its contents do
-    not matter between calls: the decode combine only reads split partials
-    written earlier in the same call (the zero fill is not relied on)."""
-    key = (device.index if device.index is not None else torch.cuda.current_device(), int(stream_handle.value or 0))
+    """Scratch buffer of a (device, stream) and the calling thread, grown on
+    demand.  Its contents do not matter between calls: a call only reads what
+    its own earlier launches wrote (the zero fill is not relied on).  Threads
+    on one stream have buffers of their own, as the launches of their calls
+    may alternate on it."""
+    key = (device.index if device.index is not None else torch.cuda.current_device(), int(stream_handle.value or 0),
+           threading.get_ident())
     buf = _ws.get(key)
     if buf is None or buf.numel() < nbytes:
+        # buffers of threads that ended go back to the allocator (their launches are
+        # on the stream already, so the memory is handed on behind them)
+        alive = {t.ident for t in threading.enumerate()}
+        for k in [k for k in list(_ws) if k[2] not in alive]:
+            _ws.pop(k, None)
         buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
         _ws[key] = buf
     return buf
