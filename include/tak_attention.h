@@ -403,7 +403,8 @@ int tak_kv8_read(const tak_kv8_cache* cache, const int32_t* cu_seqlens, const in
  * [num_seqs, num_queries, H, D]; context_lens [num_seqs] counts the cached rows,
  * the queries' own among them: query row i sees the first context_lens[s] -
  * num_queries + 1 + i rows (none: output 0, lse -inf).  KV head h / (H / H_kv).
- * softcap > 0 replaces a scaled score z by softcap * tanh(z / softcap).
+ * softcap > 0 (at least 2^-126) replaces a scaled score z by softcap *
+ * tanh(z / softcap); 0, and all above 2^126, infinity too, cap nothing.
  * lse (may be NULL) [num_seqs, num_queries, H] float32.  weights (may be NULL)
  * [num_seqs, H_kv, weights_width] float32: each key's attention weight, summed
  * over the query rows and the heads that share the KV head, is ADDED to it

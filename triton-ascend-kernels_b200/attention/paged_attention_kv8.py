@@ -12,6 +12,7 @@ import _tak_b200 as _t
 from kv8_cache import _lens, describe
 
 _KEEP = 256 << 20  # bytes of scratch that a stream keeps at most
+_MIN_CAP = 2.0 ** -126  # fp32's smallest normal number: its reciprocal is finite
 _S3, _S4 = struct.Struct("=3q").pack, struct.Struct("=4q").pack
 
 
@@ -27,7 +28,8 @@ def paged_attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_tables, con
         context_lens: [num_seqs] int32 cached rows, the new tokens' among
             them: query i of num_queries sees the first context_lens[s] -
             num_queries + 1 + i
-        softcap: > 0 caps the scaled scores: z -> softcap * tanh(z / softcap)
+        softcap: > 0 caps the scaled scores: z -> softcap * tanh(z / softcap);
+            0, and all above 2^126, cap nothing
         weights: [num_seqs, num_kv_heads, max_rows] float32; each key's
             attention weight, summed over the query rows and heads that share
             its KV head, is added to it (what kv8_cache_evict ranks by)
@@ -46,7 +48,7 @@ def paged_attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_tables, con
     assert B == seqs, "block_tables must have a row per sequence"
     assert D == d, f"head_dim of q ({D}) and of the cache ({d}) differ"
     assert H % hkv == 0, f"num_q_heads ({H}) must be divisible by num_kv_heads ({hkv})"
-    assert softcap >= 0.0, "softcap must be >= 0"
+    assert softcap == 0.0 or softcap >= _MIN_CAP, "softcap must be 0 (none) or at least 2^-126"
     cl = _lens(context_lens, index, seqs, "context_lens")
     st = q.stride()
     if len(st) == 3:

@@ -10,6 +10,10 @@ using namespace tak;
   } while (0)
 
 constexpr int64_t kMaxInt = 0x7fffffff;
+// Caps between these have fp32 reciprocals, and cap * log2(e) is finite.  Scores are
+// far below 2^126, where the cap is the identity: a larger one, infinity too, is none.
+constexpr float kMinCap = 1.17549435082228751e-38f;  // 2^-126
+constexpr float kMaxCap = 8.50705917302346159e37f;   // 2^126
 
 static void strides_to(int64_t* dst, const int64_t* src, int n) {
   for (int i = 0; i < n; ++i) dst[i] = src[i];
@@ -172,7 +176,7 @@ int tak_kv8_attention(const tak_kv8_cache* cache, const void* q, const int64_t* 
   if (const int r = make_view(&c, cache)) return r;
   TAK_REQUIRE(dtype >= 0 && dtype <= 2, "kv8 attention: unknown dtype");
   TAK_REQUIRE(weights_width >= 0 && weights_width <= kMaxInt, "kv8 attention: weights_width must be in [0, 2^31)");
-  TAK_REQUIRE(softcap >= 0.f, "kv8 attention: softcap must be >= 0 (0 = none)");
+  TAK_REQUIRE(softcap == 0.f || softcap >= kMinCap, "kv8 attention: softcap must be 0 (none) or at least 2^-126");
   Kv8AttnArgs a;
   if (const int r = make_attn(&a, c, num_q_heads, num_queries, weights_width, static_cast<int>(cache->code_type)))
     return r;
@@ -186,7 +190,7 @@ int tak_kv8_attention(const tak_kv8_cache* cache, const void* q, const int64_t* 
   a.weights = weights_width > 0 ? weights : nullptr;
   if (weights) strides_to(a.sw, weights_strides, 3);
   a.scale = scale;
-  a.softcap = softcap;
+  a.softcap = softcap <= kMaxCap ? softcap : 0.f;
   a.dtype = dtype;
   a.workspace = workspace;
   a.workspace_bytes = workspace ? workspace_bytes : 0;
