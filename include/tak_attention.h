@@ -425,10 +425,10 @@ int tak_kv8_attention(const tak_kv8_cache* cache, const void* q, const int64_t* 
 
 /*
  * Evicts rows in place.  For each sequence and KV head with n = min(
- * context_lens[s], weights_width, max_blocks * block_size) > budget rows, the
- * last `recent` rows stay and, of the others, the budget - recent with the
- * largest weights [num_seqs, H_kv, weights_width] (ties to the lowest position;
- * NaN counts as largest).  Kept rows move to the front in ascending order, and
+ * context_lens[s], max_blocks * block_size) > budget rows, the last `recent`
+ * rows stay and, of the others, the budget - recent with the largest weights
+ * [num_seqs, H_kv, weights_width] (ties to the lowest position; NaN counts as
+ * largest; rows at or past weights_width weigh 0).  Kept rows move to the front in ascending order, and
  * so do their weights; weights of the places freed become 0.  A group of the
  * result takes the largest scale of its rows, and rows from a smaller scale are
  * rounded again into it.  kept [num_seqs, H_kv, budget] receives the positions

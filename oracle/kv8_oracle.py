@@ -134,26 +134,27 @@ class Cache:
         return out, lse, weights, size, mass
 
     def evict(self, lens, weights, budget, recent):
-        """In place, weights [B, H, W] float32 too.  Returns (kept, new_lens)."""
+        """In place, weights [B, H, W] float32 too; rows past W weigh 0.  Returns (kept, new_lens)."""
         B, H, W = weights.shape
+        rows = self.table.shape[1] * self.P
         kept = np.full((B, H, budget), -1, np.int32)
         new = np.zeros(B, np.int32)
         for s in range(B):
-            n = max(0, min(int(lens[s]), W, self.table.shape[1] * self.P))
+            n = max(0, min(int(lens[s]), rows))
             m = new[s] = min(n, budget)
             for h in range(H):
-                idx = np.arange(n)
+                idx, held = np.arange(n), np.zeros(max(rows, W), F)
+                held[:W] = weights[s, h]
                 if n > budget:
-                    w = weights[s, h, :n - recent].astype(np.float64)
+                    w = held[:n - recent].astype(np.float64)
                     w = np.where(np.isnan(w), np.inf, w), np.isnan(w)
                     order = np.lexsort((np.arange(n - recent), -w[0], ~w[1]))
                     idx = np.sort(np.concatenate([order[:budget - recent], np.arange(n - recent, n)])).astype(int)
                 kept[s, h, :m] = idx
                 if n <= budget:
                     continue
-                moved = weights[s, h, idx].copy()
-                weights[s, h, :n] = 0
-                weights[s, h, :m] = moved
+                held[:m], held[m:n] = held[idx], 0
+                weights[s, h] = held[:W]
                 for w in (0, 1):
                     self._move(w, s, h, idx)
         return kept, new

@@ -66,3 +66,27 @@ def test_refused_evictions_change_nothing():
     assert call(d, 0, 0) == 1 and call(d, 100, 101) == 1 and call(d, 1 << 31, 10) == 1
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(before, (*d, w, kept, lens)))
+
+
+NARROW = [  # rows, width of weights, budget, recent
+    (700, 300, 200, 50), (700, 650, 200, 100), (700, 699, 300, 1), (700, 100, 400, 0), (700, 0, 300, 20),
+    (700, 0, 300, 0), (700, 0, 300, 300), (700, 256, 700, 10), (700, 5, 699, 3), (30000, 9000, 12000, 100),
+    (30000, 29999, 500, 0), (140001, 20000, 30000, 77), (200000, 150000, 1000, 10)]
+
+
+@pytest.mark.parametrize("kind", ["spread", "ties", "negative", "nan"])
+@pytest.mark.parametrize("i", range(len(NARROW)))
+def test_evict_weights_narrower_than_the_context(i, kind):
+    """Rows past `weights` count as weight 0: the newest stay, none is lost."""
+    rows, width, budget, recent = NARROW[i]
+    c = KC.make(("narrow", i), 2, 1, 64, 16, 16, "int8", rows)
+    g = np.random.default_rng(i)
+    w = (g.random((2, 1, width)) ** 8).astype(np.float32)
+    if kind == "ties":
+        w = np.round(w * 2).astype(np.float32)
+        w[w == 0] = np.where(g.random((w == 0).sum()) < 0.5, 0.0, -0.0)
+    if kind == "negative":  # rows without a weight rank above these
+        w = -w - np.float32(1)
+    if kind == "nan":
+        w[g.random(w.shape) < 0.1] = np.nan
+    compare(c, [rows, rows // 2], w, budget, recent)

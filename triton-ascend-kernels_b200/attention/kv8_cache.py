@@ -123,7 +123,8 @@ def kv8_cache_evict(k_cache, v_cache, k_scale, v_scale, block_tables, context_le
     Args:
         context_lens: [num_seqs] int32 rows that each sequence holds
         weights: [num_seqs, num_kv_heads, max_rows] float32 accumulated
-            attention weights (paged_attention_kv8's `weights`)
+            attention weights (paged_attention_kv8's `weights`); rows past
+            max_rows weigh 0
         budget: rows that stay
         recent: the last `recent` rows stay whatever their weight; the other
             budget - recent are those of the largest weight, ties to the lowest

@@ -2,7 +2,8 @@
 //
 // For each (sequence, KV head) with n > budget rows: the last `recent` rows
 // stay, and of the others the budget - recent with the largest accumulated
-// weight (ties to the lowest position, NaN above every number).  Kept rows
+// weight (ties to the lowest position, NaN above every number; rows past the end of
+// `weights` have accumulated none and weigh 0).  Kept rows
 // move to the front of the sequence in ascending order, in place.  A group of
 // the compacted rows takes the largest scale of the rows that it receives;
 // a row that came under a smaller one is requantised,
@@ -34,9 +35,10 @@ struct Kv8EvictParams {
 };
 
 __device__ __forceinline__ int kv8_evict_rows(const Kv8EvictParams& p, int s) {
-  const int64_t n = min(static_cast<int64_t>(p.context_lens[s]), min(p.width, p.c.max_rows));
+  const int64_t n = min(static_cast<int64_t>(p.context_lens[s]), p.c.max_rows);
   return n > 0 ? static_cast<int>(n) : 0;
 }
+constexpr uint32_t kZeroKey = 0x80000000u;  // weight_key(0)
 
 // unsigned key ordered as the floats are: -0 equals +0, NaN on top
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -92,6 +94,7 @@ __global__ void __launch_bounds__(kSelThreads) kv8_evict_select_kernel(const Kv8
   float* w = p.weights + s * p.sw[0] + h * p.sw[1];
   const int64_t ws = p.sw[2];
   const int cand = n - p.recent, take = p.budget - p.recent;
+  const int nw = static_cast<int>(min(static_cast<int64_t>(n), p.width));  // rows that have a weight
 
   // threshold: the take-th largest key of the candidates, digit by digit
   __shared__ uint32_t hist[256];
@@ -102,7 +105,7 @@ __global__ void __launch_bounds__(kSelThreads) kv8_evict_select_kernel(const Kv8
     if (tid < 256) hist[tid] = 0;
     __syncthreads();
     for (int i = tid; i < cand; i += kSelThreads) {
-      const uint32_t key = weight_key(w[i * ws]);
+      const uint32_t key = i < nw ? weight_key(w[i * ws]) : kZeroKey;
       if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1u);
     }
     __syncthreads();
@@ -128,7 +131,7 @@ __global__ void __launch_bounds__(kSelThreads) kv8_evict_select_kernel(const Kv8
     float v = 0.f;
     uint32_t gt = 0, eq = 0;
     if (i < n) {
-      v = w[i * ws];
+      if (i < nw) v = w[i * ws];
       if (i >= cand) {
         gt = 1;
       } else {
@@ -143,13 +146,13 @@ __global__ void __launch_bounds__(kSelThreads) kv8_evict_select_kernel(const Kv8
     if (gt || (eq && eq_before < ties)) {
       const uint32_t j = base_gt + ex.x + min(eq_before, ties);
       kept[j] = i;
-      w[j * ws] = v;
+      if (j < nw) w[j * ws] = v;
     }
     base_gt += tot.x;
     base_eq += tot.y;
   }
   __syncthreads();
-  for (int i = m + tid; i < n; i += kSelThreads) w[i * ws] = 0.f;
+  for (int i = m + tid; i < nw; i += kSelThreads) w[i * ws] = 0.f;
 }
 
 // Selection with the weights in registers: a cluster of CTAs holds one (sequence,
@@ -161,6 +164,10 @@ __global__ void __launch_bounds__(kSelThreads) kv8_evict_select_kernel(const Kv8
 // of up to 8192 in 25.  (Counting two bits at a time in registers, 16 cluster barriers
 // instead of three, took 75 us for 8 heads of 100000 weights; eight weights a thread in
 // clusters of 16, 56.)
+//
+// Rows past the end of `weights` are not held: they are one run of keys of weight 0
+// after all others, so their number goes into the counts, and the kept ones among them
+// follow the held rows in order.
 constexpr int kBins = 2048;
 
 template <int KPT>
@@ -181,6 +188,8 @@ __global__ void __launch_bounds__(kSelThreads, KPT <= 8 ? 2 : 1) kv8_evict_selec
   float* w = p.weights + s * p.sw[0] + h * p.sw[1];
   const int64_t ws = p.sw[2];
   const int cand = n - p.recent, take = p.budget - p.recent;
+  const int nw = static_cast<int>(min(static_cast<int64_t>(n), p.width));  // rows that have a weight
+  const int held = min(cand, nw), bare = cand - held;                      // candidates that have one, and the others
   const int base = rank * KPT * kSelThreads;  // the CTA's first position
 
   __shared__ uint32_t hist[3][kBins];         // one per digit: no barrier to clear them between
@@ -197,7 +206,7 @@ __global__ void __launch_bounds__(kSelThreads, KPT <= 8 ? 2 : 1) kv8_evict_selec
 #pragma unroll
   for (int k = 0; k < KPT; ++k) {
     const int i = base + k * kSelThreads + tid;
-    val[k] = i < n ? w[i * ws] : 0.f;
+    val[k] = i < nw ? w[i * ws] : 0.f;
   }
   for (int i = tid; i < 3 * kBins; i += kSelThreads) hist[0][i] = 0;
   __syncthreads();
@@ -212,9 +221,11 @@ __global__ void __launch_bounds__(kSelThreads, KPT <= 8 ? 2 : 1) kv8_evict_selec
     for (int k = 0; k < KPT; ++k) {
       const int i = base + k * kSelThreads + tid;
       const uint32_t key = weight_key(val[k]);
-      if (i < cand && (d == 0 || (key >> (d == 1 ? 21 : 10)) == (T >> (d == 1 ? 21 : 10))))
+      if (i < held && (d == 0 || (key >> (d == 1 ? 21 : 10)) == (T >> (d == 1 ? 21 : 10))))
         atomicAdd(&hist[d][(key >> shift) & (bins - 1)], 1u);
     }
+    if (at == 0 && bare > 0 && (d == 0 || (kZeroKey >> (d == 1 ? 21 : 10)) == (T >> (d == 1 ? 21 : 10))))
+      atomicAdd(&hist[d][(kZeroKey >> shift) & (bins - 1)], static_cast<uint32_t>(bare));
     everyone();
     // bins from the top: thread t has bins - 1 - 2 t and the one below
     uint32_t c0 = 0, c1 = 0;
@@ -260,8 +271,8 @@ __global__ void __launch_bounds__(kSelThreads, KPT <= 8 ? 2 : 1) kv8_evict_selec
   for (int k = 0; k < KPT; ++k) {
     const int i = base + k * kSelThreads + tid;
     const uint32_t key = weight_key(val[k]);
-    const unsigned gt = __ballot_sync(0xffffffffu, (i >= cand && i < n) || (i < cand && key > T));
-    const unsigned eq = __ballot_sync(0xffffffffu, i < cand && key == T && ties > 0);
+    const unsigned gt = __ballot_sync(0xffffffffu, (i >= cand && i < nw) || (i < held && key > T));
+    const unsigned eq = __ballot_sync(0xffffffffu, i < held && key == T && ties > 0);
     if (lane == 0) cnt[k * 32 + warp] = __popc(gt) | (__popc(eq) << 16);
   }
   __syncthreads();
@@ -301,7 +312,7 @@ __global__ void __launch_bounds__(kSelThreads, KPT <= 8 ? 2 : 1) kv8_evict_selec
   for (int k = 0; k < KPT; ++k) {
     const int i = base + k * kSelThreads + tid;
     const uint32_t key = weight_key(val[k]), c = cnt[k * 32 + warp];
-    const bool is_gt = (i >= cand && i < n) || (i < cand && key > T), is_eq = i < cand && key == T && ties > 0;
+    const bool is_gt = (i >= cand && i < nw) || (i < held && key > T), is_eq = i < held && key == T && ties > 0;
     const uint32_t g_before = gt0 + (c & 0xffffu) + __popc(__ballot_sync(0xffffffffu, is_gt) & below);
     const uint32_t e_before = eq0 + (c >> 16) + __popc(__ballot_sync(0xffffffffu, is_eq) & below);
     if (is_gt || (is_eq && e_before < ties)) {
@@ -310,7 +321,22 @@ __global__ void __launch_bounds__(kSelThreads, KPT <= 8 ? 2 : 1) kv8_evict_selec
       w[j * ws] = val[k];
     }
   }
-  for (int i = m + at; i < n; i += all) w[i * ws] = 0.f;
+  if (n > nw) {  // rows without a weight: the first `more` of the candidates, and the recent ones
+    uint32_t gts = 0, eqs = 0;
+    for (int r = 0; r < cs; ++r) {
+      const uint2 t = *cluster.map_shared_rank(&cta_total, r);
+      gts += t.x;
+      eqs += t.y;
+    }
+    const int front = static_cast<int>(gts + min(eqs, ties));
+    const int more = kZeroKey > T ? bare : kZeroKey == T ? static_cast<int>(ties - min(eqs, ties)) : 0;
+    for (int j = front + at; j < m; j += all) {
+      const int b = j - front;
+      kept[j] = b < more ? held + b : max(cand, nw) + (b - more);
+      if (j < nw) w[j * ws] = 0.f;
+    }
+  }
+  for (int i = m + at; i < nw; i += all) w[i * ws] = 0.f;
   everyone();  // no CTA leaves while another reads its totals
 }
 
