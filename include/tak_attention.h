@@ -360,7 +360,7 @@ enum { TAK_KV8_INT8 = 0, TAK_KV8_E4M3 = 1 };
  * [0, num_blocks), are never read or written: they read as zero rows (score 0,
  * value 0), and writes to them are dropped.  Limits: D <= 640, group <= 256
  * and dividing block_size, num_seqs and H_kv <= 65535,
- * max_blocks * block_size < 2^31.
+ * max_blocks * block_size <= 2^31 - 2^16.
  */
 typedef struct tak_kv8_cache {
   void* k_cache; int64_t k_strides[4];

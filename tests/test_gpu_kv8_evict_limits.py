@@ -90,3 +90,18 @@ def test_evict_weights_narrower_than_the_context(i, kind):
     if kind == "nan":
         w[g.random(w.shape) < 0.1] = np.nan
     compare(c, [rows, rows // 2], w, budget, recent)
+
+
+def test_evict_budget_of_all_that_32_bits_hold():
+    """No limit, written as the largest budget: every row stays, and kept is filled to its end."""
+    c = KC.make("nolimit", 1, 1, 16, 16, 64, "int8", 50)
+    d = KC.to_device(c)
+    before = [t.clone() for t in d]
+    w = torch.rand(1, 1, 64, device=DEV)
+    budget = 2 ** 31 - 1
+    kept, lens = C8.kv8_cache_evict(*d, dev32([50]), w, budget, 3)
+    assert kept.shape == (1, 1, budget) and lens.tolist() == [50]
+    assert kept[0, 0, :50].tolist() == list(range(50))
+    for part in kept[0, 0, 50:].split(1 << 28):
+        assert bool((part == -1).all())
+    assert all(torch.equal(a, b) for a, b in zip(before, d))

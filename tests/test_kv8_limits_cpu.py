@@ -1,11 +1,14 @@
 """CPU-side checks of the scratch that calls share and of the 8-bit cache's limits."""
 
 import ctypes
+import os
 import threading
 
+import pytest
 import torch
 
 import _tak_b200 as T
+import kv8_cache as C8
 
 CPU = torch.device("cpu", 0)
 
@@ -55,3 +58,20 @@ def test_scratch_of_ended_threads_is_given_back(monkeypatch):
     assert len(T._ws) == 2
     scratch(5, 64)
     assert sorted(k[1] for k in T._ws) == [3, 5] and scratch(3, 64) is mine
+
+
+def _cache(block, width):
+    p = 4096  # never dereferenced: the sizes alone are looked at
+    return C8._PACK.pack(p, 1, 1, 1, 1, p, 1, 1, 1, 1, p, 1, 1, 1, p, 1, 1, 1, p, 1, 1, 4, 2, block, 64, 16, 2, width, 0)
+
+
+def test_rows_of_a_table_stay_below_the_reach_of_32_bits():
+    """Kernels step past the last row in 32-bit positions: a table may not reach 2^31 - 2^16."""
+    if not os.path.exists(T.LIB_PATH):
+        pytest.skip("libtak_b200.so not built")
+    size = T.lib().tak_kv8_attention_workspace_size
+    for block in (16, 128, 65536):
+        most = (2 ** 31 - 2 ** 16) // block
+        assert size(_cache(block, most), 4, 1, 0, 1) >= 0  # accepted (these strides need no workspace)
+        assert size(_cache(block, most + 1), 4, 1, 0, 1) == -1
+        assert "max_blocks" in T.lib().tak_last_error().decode()

@@ -44,7 +44,7 @@ struct Kv8View {
   int64_t sbt[2];
   int Hkv, P, D, group, num_seqs, max_blocks;
   int64_t num_blocks;
-  int64_t max_rows;  // max_blocks * P, below 2^31
+  int64_t max_rows;  // max_blocks * P, at most 2^31 - 2^16
   Kv8Div by_P, by_group;
 };
 

@@ -10,6 +10,9 @@ using namespace tak;
   } while (0)
 
 constexpr int64_t kMaxInt = 0x7fffffff;
+// Rows of a sequence: positions are 32-bit, and the kernels look up to a step of
+// thousands of rows past the last one.
+constexpr int64_t kMaxRows = kMaxInt - 0xffff;
 // Caps between these have fp32 reciprocals, and cap * log2(e) is finite.  Scores are
 // far below 2^126, where the cap is the identity: a larger one, infinity too, is none.
 constexpr float kMinCap = 1.17549435082228751e-38f;  // 2^-126
@@ -30,8 +33,8 @@ static int make_view(Kv8View* out, const tak_kv8_cache* c) {
               "kv8: group must divide block_size and be in [1, 256]");
   TAK_REQUIRE(c->num_seqs >= 0 && c->num_seqs <= 65535, "kv8: num_seqs must be in [0, 65535]");
   TAK_REQUIRE(c->num_blocks >= 0 && c->num_blocks <= kMaxInt, "kv8: num_blocks must be in [0, 2^31)");
-  TAK_REQUIRE(c->max_blocks >= 0 && c->max_blocks <= kMaxInt / c->block_size,
-              "kv8: max_blocks * block_size must stay below 2^31");
+  TAK_REQUIRE(c->max_blocks >= 0 && c->max_blocks <= kMaxRows / c->block_size,
+              "kv8: max_blocks * block_size must be at most 2^31 - 2^16");
   Kv8View v{};
   v.Hkv = static_cast<int>(c->num_kv_heads);
   v.P = static_cast<int>(c->block_size);

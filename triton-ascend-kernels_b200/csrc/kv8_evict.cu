@@ -86,7 +86,8 @@ __global__ void __launch_bounds__(kSelThreads) kv8_evict_select_kernel(const Kv8
   const int n = kv8_evict_rows(p, s), m = min(n, p.budget);
   int32_t* kept = p.kept + (static_cast<int64_t>(s) * p.c.Hkv + h) * p.budget;
   if (h == 0 && tid == 0) p.new_lens[s] = m;
-  for (int j = m + tid; j < p.budget; j += kSelThreads) kept[j] = -1;
+  // (unsigned: with a budget near 2^31 the last step passes it)
+  for (uint32_t j = m + tid; j < static_cast<uint32_t>(p.budget); j += kSelThreads) kept[j] = -1;
   if (n <= p.budget) {
     for (int j = tid; j < n; j += kSelThreads) kept[j] = j;
     return;
@@ -180,7 +181,8 @@ __global__ void __launch_bounds__(kSelThreads, KPT <= 8 ? 2 : 1) kv8_evict_selec
   int32_t* kept = p.kept + (static_cast<int64_t>(s) * p.c.Hkv + h) * p.budget;
   const int all = cs * kSelThreads, at = rank * kSelThreads + tid;
   if (h == 0 && at == 0) p.new_lens[s] = m;
-  for (int j = m + at; j < p.budget; j += all) kept[j] = -1;
+  // (unsigned: with a budget near 2^31 the last step passes it)
+  for (uint32_t j = m + at; j < static_cast<uint32_t>(p.budget); j += all) kept[j] = -1;
   if (n <= p.budget) {
     for (int j = at; j < n; j += all) kept[j] = j;
     return;
