@@ -75,3 +75,13 @@ def test_rows_of_a_table_stay_below_the_reach_of_32_bits():
         assert size(_cache(block, most), 4, 1, 0, 1) >= 0  # accepted (these strides need no workspace)
         assert size(_cache(block, most + 1), 4, 1, 0, 1) == -1
         assert "max_blocks" in T.lib().tak_last_error().decode()
+
+
+def test_workspace_size_of_refused_arguments():
+    if not os.path.exists(T.LIB_PATH):
+        pytest.skip("libtak_b200.so not built")
+    size = T.lib().tak_kv8_attention_workspace_size
+    assert size(_cache(16, 4), 4, 1, 64, 1) >= 0
+    for bad in ((3, 1, 64, 1), (4, -1, 64, 1), (4, 65536, 64, 1), (4, 1, -1, 1), (4, 1, 2 ** 31, 1), (4, 1, 64, 3),
+                (4, 1, 64, -1)):
+        assert size(_cache(16, 4), *bad) == -1, bad

@@ -142,7 +142,9 @@ int tak_kv8_read(const tak_kv8_cache* cache, const int32_t* cu_seqlens, const in
 }
 
 static int make_attn(Kv8AttnArgs* out, const Kv8View& c, int64_t num_q_heads, int64_t num_queries, int64_t width,
-                     int code_type) {
+                     int code_type, int dtype) {
+  TAK_REQUIRE(dtype >= 0 && dtype <= 2, "kv8 attention: unknown dtype");
+  TAK_REQUIRE(width >= 0 && width <= kMaxInt, "kv8 attention: weights_width must be in [0, 2^31)");
   TAK_REQUIRE(num_q_heads > 0 && num_q_heads <= 65535 && num_q_heads % c.Hkv == 0,
               "kv8 attention: num_q_heads must be a multiple of num_kv_heads, at most 65535");
   TAK_REQUIRE(num_queries >= 0 && num_queries <= 65535, "kv8 attention: num_queries must be in [0, 65535]");
@@ -151,6 +153,7 @@ static int make_attn(Kv8AttnArgs* out, const Kv8View& c, int64_t num_q_heads, in
   a.Lq = static_cast<int>(num_queries);
   a.weights_width = width;
   a.code_type = code_type;
+  a.dtype = dtype;
   a.force_generic = kernel_path() == 1;
   *out = a;
   return 0;
@@ -161,11 +164,10 @@ int64_t tak_kv8_attention_workspace_size(const tak_kv8_cache* cache, int64_t num
   Kv8View c;
   Kv8AttnArgs a;
   if (make_view(&c, cache) || make_attn(&a, c, num_q_heads, num_queries, weights_width,
-                                        static_cast<int>(cache->code_type)))
+                                        static_cast<int>(cache->code_type), dtype))
     return -1;
   static float dummy;
   a.weights = weights_width > 0 ? &dummy : nullptr;
-  a.dtype = dtype;
   return kv8_attention_ws_bytes(c, a);
 }
 
@@ -177,11 +179,9 @@ int tak_kv8_attention(const tak_kv8_cache* cache, const void* q, const int64_t* 
   note_kernel("");
   Kv8View c;
   if (const int r = make_view(&c, cache)) return r;
-  TAK_REQUIRE(dtype >= 0 && dtype <= 2, "kv8 attention: unknown dtype");
-  TAK_REQUIRE(weights_width >= 0 && weights_width <= kMaxInt, "kv8 attention: weights_width must be in [0, 2^31)");
   TAK_REQUIRE(softcap == 0.f || softcap >= kMinCap, "kv8 attention: softcap must be 0 (none) or at least 2^-126");
   Kv8AttnArgs a;
-  if (const int r = make_attn(&a, c, num_q_heads, num_queries, weights_width, static_cast<int>(cache->code_type)))
+  if (const int r = make_attn(&a, c, num_q_heads, num_queries, weights_width, static_cast<int>(cache->code_type), dtype))
     return r;
   if (c.num_seqs == 0 || num_queries == 0) return 0;
   TAK_REQUIRE(q && q_strides && out && out_strides && context_lens, "kv8 attention: null pointer");
@@ -194,7 +194,6 @@ int tak_kv8_attention(const tak_kv8_cache* cache, const void* q, const int64_t* 
   if (weights) strides_to(a.sw, weights_strides, 3);
   a.scale = scale;
   a.softcap = softcap <= kMaxCap ? softcap : 0.f;
-  a.dtype = dtype;
   a.workspace = workspace;
   a.workspace_bytes = workspace ? workspace_bytes : 0;
   const int r = kv8_attention_launch(c, a, static_cast<cudaStream_t>(stream));
