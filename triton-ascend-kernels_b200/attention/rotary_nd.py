@@ -47,6 +47,8 @@ def rotary_nd(q, k, positions, inv_freq, sections, *, interleaved=False, inverse
         "inv_freq must be float32 with sum(sections) elements"
     assert 2 * pairs <= D, f"rot_dim ({2 * pairs}) exceeds head_dim ({D})"
     if pos.dtype is not _torch.int32:
+        assert not pos.is_floating_point() and not pos.is_complex(), \
+            f"positions must be integers, not {pos.dtype} (fractions would be cut off)"
         pos = pos.to(_torch.int32)
     if not inv_freq.is_contiguous():
         inv_freq = inv_freq.contiguous()
