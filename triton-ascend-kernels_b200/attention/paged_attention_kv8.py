@@ -19,6 +19,7 @@ _S3, _S4 = struct.Struct("=3q").pack, struct.Struct("=4q").pack
 def paged_attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, *, softcap=0.0,
                         weights=None, return_lse=False):
     """Attention of the newest tokens of each sequence over its cached rows.
+    Scores are q . k / sqrt(head_dim).
 
     Args:
         q: [num_seqs, num_q_heads, head_dim], or [num_seqs, num_queries,

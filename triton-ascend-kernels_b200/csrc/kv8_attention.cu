@@ -5,12 +5,16 @@
 // sum_j p_j vs_g Vc_j.  Both scales are constant over a tile of 16 keys (groups
 // are multiples of 16), so K's scale multiplies a tile's scores and V's goes
 // into the exponent: with lv = log2(vs),
-//   P_j = 2^(s_j + lv - M),  O = sum_j P_j Vc_j,  l = sum_j P_j / vs,  out = O / l,
-// where M is the running maximum of s_j + lv.  P stays within fp16 whatever the
-// scales are (a small V under a large weight and a large V under a small weight
-// are compared by their product), and codes are exact in fp16, so both products
-// run on fp16 tensor cores with fp32 sums; q is brought to fp16 by a power of
-// two per row, which is exact for elements within 2^-22 of the row's largest.
+//   P_j = 2^(s_j + lv - M),  O = sum_j P_j Vc_j,  l = sum_j 2^(s_j - M),  out = O / l,
+// where M is the running maximum of s_j + lv, and l's terms are P_j / vs unless V's
+// scales lie far apart (kFar).  P stays within fp16 whatever the scales are (a small V
+// under a large weight and a large V under a small weight are compared by their
+// product), and codes are exact in fp16, so both products run on fp16 tensor cores with
+// fp32 sums; q is brought to fp16 by a power of two per row, which is exact for
+// elements within 2^-22 of the row's largest.  P's rounding to fp16 (2^-11 of each
+// weight) is what the 16-bit product costs: nothing to be seen in a bf16 output (error
+// 1.7e-3 of its size with or without), but it takes fp16 outputs over long contexts
+// from 2.1e-4 to 2.8e-4.
 //
 // Work split.  A (sequence, KV head, chunk of query rows) is an item; an item is
 // cut into chunks of CH keys.  The chunks of all items, in order, are dealt out
@@ -164,7 +168,7 @@ __device__ __forceinline__ void codes_to_half(uint32_t r, uint32_t& lo, uint32_t
 
 // Four scores z to cap * tanh(z / cap), in base-2 units (cap2 = cap * log2(e)).
 // Below |z / cap| = 0.6, where ordinary scores lie, tanh is its odd polynomial
-// (fitted to 7e-8 relative); past it, 1 - 2 / (1 + e^(2 z / cap)), whose absolute
+// (fitted to 8.1e-8 relative); past it, 1 - 2 / (1 + e^(2 z / cap)), whose absolute
 // error of 1e-7 is small there.  A warp leaves the second out when it needs it for
 // no score.
 __device__ __forceinline__ void kv8_cap(float (&x)[4], float inv_cap, float cap2) {
@@ -440,13 +444,13 @@ __device__ __forceinline__ void kv8_produce(const Kv8TcParams& p, const CUtensor
 }
 
 // Up to eight query rows a KV head (a decode step with up to eight query heads for
-// each).  Bound by memory: 64 x <= 8192 keys of 8 heads x 128 (e4m3) in 100 us with
-// the join, 5.45 TB/s, 83 % of the measured copy rate; 3 x <= 131071 keys (int8, 8
-// rows, capped scores) in 102, 80 %.  What is missing is the first data's way (4 us)
-// and the end, where the CTAs finish within 10 % of each other.  Steps on the way,
-// both cases: rows on the MMA's M side, 4 or 8 of its 16 real, 139 and 148 us; with
-// three CTAs an SM, Q in shared memory, 120 and 133; keys on the M side 99 and 100
-// without the join.  One request of 777 keys takes 9.8 us: two launches and the chain
+// each).  Bound by memory: 64 x <= 8192 keys of 8 heads x 128 (e4m3) in 99 us with
+// the join, 5.54 TB/s, 84 % of the measured copy rate; 3 x <= 131071 keys (int8, 8
+// rows, capped scores) in 99, 83 %.  Head dim 64: 74 us (57 %), 256: 218 (77 %).  What
+// is missing is the first data's way (4 us) and the end, where the CTAs finish within
+// 10 % of each other.  Steps on the way, both cases: rows on the MMA's M side, 4 or 8
+// of its 16 real, 139 and 148 us; with three CTAs an SM, Q in shared memory, 120 and
+// 133; keys on the M side 99 and 100 without the join.  One request of 777 keys takes 10.2 us: two launches and the chain
 // of context, page, codes, join.
 template <int CODE, int DP>
 __global__ void __launch_bounds__(Kv8Few<DP>::THREADS, Kv8Few<DP>::CTAS)
@@ -875,10 +879,12 @@ __global__ void __launch_bounds__(Kv8Few<DP>::THREADS, Kv8Few<DP>::CTAS)
 }
 
 // 16 and 32 query rows.  Bound by the issue slots and latencies of the conversions and
-// MMAs (two consumer warps a scheduler): 64 x <= 8192 keys of 8 heads, 32 rows, in 190
-// us, 16 rows in 127; 24 x <= 6000 keys of 4 heads, 32 rows (int8), in 47, 61 with the
-// weights.  Where each warp held eight rows and walked all keys, every code was
-// converted once for each warp (57 and 69 us).  Chunks of 64 keys with three CTAs an SM
+// MMAs (two consumer warps a scheduler): 64 x <= 8192 keys of 8 heads, 32 rows, in 203
+// us, 16 rows in 125 (head dim 64: 154 and 103; 256: 381 and 249); 24 x <= 6000 keys of
+// 4 heads, 32 rows (int8), in 49, 65 with the weights.  The branch for V scales far
+// apart costs 32 rows up to 9 us of that: as a loop of its own it spilled (252 us for
+// the first), with its sums in shared memory it took 207.  Where each warp held eight rows and walked all keys, every code was
+// converted once for each warp (57 and 69 us, then against 47 and 61).  Chunks of 64 keys with three CTAs an SM
 // took 251 us for the first, 61 without weights for the last.
 template <int CODE, int DP, int NR>
 __global__ void __launch_bounds__(Kv8Many<DP, NR>::THREADS, Kv8Many<DP, NR>::CTAS)

@@ -5,7 +5,7 @@
 // from a second launch, one warp per key, that recomputes the scores against
 // the finished log-sum-exp.  Bound by issue slots and the row's chain of shuffles and
 // exponentials; every query row reads the cache again (64 x <= 8192 keys, 32 heads of
-// 128, bf16: 10.7 ms against 0.1 on tensor cores), so it serves the shapes that those
+// 128, bf16: 11.0 ms against 0.1 on tensor cores), so it serves the shapes that those
 // do not take.
 //
 // The values are summed against a reference of their own: with vs = 2^E v, 1/2 <= v

@@ -78,9 +78,11 @@ __device__ __forceinline__ uint2 block_scan2(uint32_t a, uint32_t b, uint2* part
   return make_uint2(before.x + x - a, before.y + y - b);
 }
 
-// Selection for sequences too long for the registers of a cluster (over 131072
-// rows): one CTA per (sequence, head) that reads its weights once for each of four
-// eight-bit digits and once more to compact them.
+// Selection for sequences too long for the registers of a cluster (where table and
+// weights both pass 131072 rows): one CTA per (sequence, head) that reads its weights
+// once for each of four eight-bit digits and once more to compact them.  Bound by that
+// CTA's latency: 8 heads of 131073 weights in 314 us, of 262144 in 608, of 4096 in such
+// a table in 29.
 __global__ void __launch_bounds__(kSelThreads) kv8_evict_select_kernel(const Kv8EvictParams p) {
   const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
   const int n = kv8_evict_rows(p, s), m = min(n, p.budget);
@@ -161,8 +163,8 @@ __global__ void __launch_bounds__(kSelThreads) kv8_evict_select_kernel(const Kv8
 // and 10 bits): each CTA counts its keys in shared memory, the cluster's counts are
 // added through distributed shared memory, and every CTA finds the digit in which
 // the take-th largest key lies.  Bound by latency, the cluster barriers and the rounds
-// through distributed shared memory: 8 heads of 100000 weights in 31 us, 48 x 8 heads
-// of up to 8192 in 25.  (Counting two bits at a time in registers, 16 cluster barriers
+// through distributed shared memory: 8 heads of 100000 weights in 28 us, 48 x 8 heads
+// of up to 8192 in 22.  (Counting two bits at a time in registers, 16 cluster barriers
 // instead of three, took 75 us for 8 heads of 100000 weights; eight weights a thread in
 // clusters of 16, 56.)
 //
@@ -349,10 +351,11 @@ __global__ void __launch_bounds__(kSelThreads, KPT <= 8 ? 2 : 1) kv8_evict_selec
 // after row r of the windows: its position is read three steps ahead, its page two,
 // its scale one, so that no step waits for a chain of loads.
 //
-// Bound by the issue slots of the requantisation and the row lookups (58 % issue),
-// then by memory: 36 x 8 heads x 2048 rows of 128, K and V, in 71 us (302 MB moved,
-// 4.3 TB/s, 65 % of the measured copy rate); one sequence's 8 heads x 16384 rows, over
-// clusters of 16, in 29.  Windows of 16 KB took 14 % longer.  Pieces held in registers
+// Bound by the issue slots of the requantisation and the row lookups (57 % issue),
+// then by memory: 36 x 8 heads x 2048 rows of 128, K and V, in 75 us (302 MB moved,
+// 4.0 TB/s, 61 % of the measured copy rate; 66 us over a cache that an eviction has
+// compacted, where no row changes its scale); one sequence's 8 heads x 16384 rows, over
+// clusters of 16, in 26.  Windows of 16 KB took 14 % longer.  Pieces held in registers
 // so that four CTAs fit an SM: 10 % less where that saves a wave, 25 % more elsewhere.
 template <int CODE, int VEC>
 __global__ void __launch_bounds__(256) kv8_evict_move_kernel(const __grid_constant__ Kv8EvictParams p) {
@@ -611,7 +614,7 @@ int kv8_evict_launch(const Kv8View& c, int code_type, const int32_t* context_len
   note_kernel("kv8_evict");
   if (rows <= 16 * 8 * sel) {
     // eight weights a thread let two CTAs fit an SM; past 8 CTAs of that, sixteen
-    // (8 heads of 100000 weights: 28 us; eight a thread in clusters of 16: 56 us)
+    // (8 heads of 100000 weights: half the time of eight a thread in clusters of 16)
     const int kpt = rows <= 4 * sel ? 4 : rows <= 8 * 8 * sel ? 8 : 16;
     int cs = 1;
     while (rows > kpt * sel * cs) cs *= 2;
