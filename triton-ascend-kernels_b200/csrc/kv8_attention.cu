@@ -13,8 +13,8 @@
 // fp32 sums; q is brought to fp16 by a power of two per row, which is exact for
 // elements within 2^-22 of the row's largest.  P's rounding to fp16 (2^-11 of each
 // weight) is what the 16-bit product costs: nothing to be seen in a bf16 output (error
-// 1.7e-3 of its size with or without), but it takes fp16 outputs over long contexts
-// from 2.1e-4 to 2.8e-4.
+// 1.7e-3 of its size with or without), but it takes fp16 outputs from 2.1e-4 to as
+// much as 2.8e-4 (131071 keys).
 //
 // Work split.  A (sequence, KV head, chunk of query rows) is an item; an item is
 // cut into chunks of CH keys.  The chunks of all items, in order, are dealt out
